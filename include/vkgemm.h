@@ -45,7 +45,8 @@ typedef enum vk_status {
 
 typedef enum vk_dtype {
     VK_DTYPE_F16 = 0, /* IEEE binary16 in and out (playground::float16_t = half) */
-    VK_DTYPE_F32 = 1  /* IEEE binary32 in and out                                */
+    VK_DTYPE_F32 = 1, /* IEEE binary32 in and out                                */
+    VK_DTYPE_BF16 = 2 /* bfloat16; the 8-bit linear layer only                   */
 } vk_dtype;
 
 typedef enum vk_acc {
@@ -183,6 +184,115 @@ int vk_matmul_f16(int version, size_t m, size_t n, size_t k, const void* A, cons
 /* Replaces: template<> matmul<float32_t, V>(m, n, k, A, B, C), matmul.hpp:16-19 with
  * DType = float32_t.  version 1 = FFMA SGEMM.  Default stream. */
 int vk_matmul_f32(int version, size_t m, size_t n, size_t k, const float* A, const float* B, float* C);
+
+/* 8-bit operands (no counterpart in the reference): the linear layers of a language model with their operands held
+ * in 8 bits, forward and backward.  A matrix in 8 bits is row-major e4m3 (one byte per value, leading dimension in
+ * bytes) and e8m0 scales (one byte s per block of 128 values, standing for 2^(s - 127); 255 is NaN):
+ *   VK_FP8_ROW   a block is 128 neighbouring values of a row: scales are rows x ceil(cols / 128), row-major;
+ *   VK_FP8_TILE  a block is a tile of 128 x 128: scales are ceil(rows / 128) x ceil(cols / 128).
+ * The value of an element is q * 2^(s - 127).  A block's scale is the smallest power of two with
+ * max|v| <= 448 * scale (1 for a block of zeros, at least 2^-127); q is v / scale rounded once to nearest even.  A
+ * block that holds an infinity or a NaN gets the NaN scale and NaN values.
+ *
+ * These calls are asynchronous on `stream`, allocate nothing, and can be captured into a CUDA graph.  A leading
+ * dimension of 0 stands for the row's length.  The results of a call do not change from run to run.  Rows of operands
+ * that start at 16-byte boundaries run on the tensor cores; any other alignment is taken by a (slow) CUDA-core kernel.
+ * Outputs must not overlap inputs, except where said. */
+typedef enum vk_fp8_scaling { VK_FP8_ROW = 0, VK_FP8_TILE = 1 } vk_fp8_scaling;
+
+/* Q, scale = the 8-bit form of X[rows x cols] (fp16, bf16 or fp32). */
+typedef struct vk_quantize_fp8_args {
+    const void* X;
+    void* Q;
+    void* scale;
+    int64_t rows, cols;
+    int64_t ldx, ldq, ld_scale;
+    int32_t dtype;   /* vk_dtype of X */
+    int32_t scaling; /* vk_fp8_scaling */
+    void* stream;
+} vk_quantize_fp8_args;
+int vk_quantize_fp8(const vk_quantize_fp8_args* args);
+
+/* RMS norm of each row with an 8-bit output (fp16 or bf16; statistics and products in fp32):
+ *   H = X + residual (rounded to the type; without a residual H is X and must be NULL here)
+ *   rstd = 1 / sqrt(mean(H^2) + eps);   Q, scale = 8-bit form (VK_FP8_ROW) of H * rstd * weight
+ * H may be X or residual itself (same leading dimension).  cols >= 1. */
+typedef struct vk_rmsnorm_fp8_args {
+    const void* X;
+    const void* residual; /* may be NULL */
+    const void* weight;   /* cols values of the same type */
+    void* Q;
+    void* scale;
+    void* H;              /* given with a residual and only then */
+    float* rstd;          /* one per row */
+    int64_t rows, cols;
+    int64_t ldx, ld_residual, ldq, ld_scale, ldh;
+    float eps;
+    int32_t dtype;        /* VK_DTYPE_F16 or VK_DTYPE_BF16 */
+    void* stream;
+} vk_rmsnorm_fp8_args;
+int vk_rmsnorm_fp8(const vk_rmsnorm_fp8_args* args);
+
+/* The norm's backward pass, from the gradient dY of its output (the rounding to 8 bits passes gradients on unchanged):
+ *   dX = rstd * (g - xhat * mean(g * xhat)) + dres,   g = dY * weight, xhat = H * rstd
+ *   dweight = sum over rows of dY * xhat   (fp32, overwritten)
+ * dX is the gradient of X and of the residual alike; dres (may be NULL) is the gradient that reaches H from elsewhere.
+ * dX may be dY or dres itself (same leading dimension).  The workspace (vk_rmsnorm_fp8_workspace bytes, 16-byte
+ * aligned) belongs to the call until it has run: calls that can overlap need one each. */
+typedef struct vk_rmsnorm_fp8_backward_args {
+    const void* dY;
+    const void* H;
+    const void* weight;
+    const float* rstd;
+    const void* dres;
+    void* dX;
+    float* dweight;
+    void* workspace;
+    size_t workspace_bytes;
+    int64_t rows, cols;
+    int64_t lddy, ldh, ld_dres, lddx;
+    int32_t dtype; /* VK_DTYPE_F16 or VK_DTYPE_BF16 */
+    void* stream;
+} vk_rmsnorm_fp8_backward_args;
+int vk_rmsnorm_fp8_workspace(int64_t rows, int64_t cols, size_t* bytes);
+int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* args);
+
+/* C[m x n] = A * op(B) of 8-bit operands, fp32 accumulation, C in fp16, bf16 or fp32.  A is m x k.  With trans_b B is
+ * stored n x k (a layer's weights in its forward pass); without, k x n (the same weights in the input's gradient),
+ * which needs VK_FP8_TILE scales. */
+typedef struct vk_gemm_fp8_args {
+    const void* A;
+    const void* B;
+    const void* a_scale;
+    const void* b_scale;
+    void* C;
+    int64_t m, n, k;
+    int64_t lda, ldb, ldc;
+    int64_t ld_a_scale, ld_b_scale;
+    int32_t a_scaling, b_scaling; /* vk_fp8_scaling */
+    int32_t trans_b;
+    int32_t dtype;                /* vk_dtype of C */
+    void* stream;
+} vk_gemm_fp8_args;
+int vk_gemm_fp8(const vk_gemm_fp8_args* args);
+
+/* dW[n x k] = dY^T * X (accumulate = 1: dW += it): a layer's weight gradient from its output's gradient dY[tokens x n]
+ * in 16 bits and its input X[tokens x k] as the forward pass kept it, in 8 bits with VK_FP8_ROW scales.  X's values are
+ * used in dY's type: bf16 holds each of them exactly; fp16 rounds what lies below its smallest normal number and
+ * holds what lies above its largest at that.  fp32 accumulation; dW in fp16, bf16 or fp32. */
+typedef struct vk_wgrad_fp8_args {
+    const void* dY;
+    const void* X;
+    const void* x_scale;
+    void* dW;
+    int64_t tokens, n, k;
+    int64_t lddy, ldx, ld_x_scale, lddw;
+    int32_t dtype;     /* of dY: VK_DTYPE_F16 or VK_DTYPE_BF16 */
+    int32_t out_dtype; /* vk_dtype of dW */
+    int32_t accumulate;
+    void* stream;
+} vk_wgrad_fp8_args;
+int vk_wgrad_fp8(const vk_wgrad_fp8_args* args);
 
 /* Multi-GPU row-block sharding (no counterpart in the reference, which is single-GPU,
  * README.md:161; this is the layer BASELINE.json asks for).  GPU r of `ngpu` computes rows

@@ -9,6 +9,9 @@ constexpr int kMaxPeers = 7;
 
 // Records a thread-local error message (read back by vk_last_error_string) and returns `code`.
 int set_error(int code, const char* fmt, ...);
+struct DeviceState;
+// The current device, initialised (and refused when it is no sm_100 device).  st_out may be NULL.
+int current_device(int* dev_out, DeviceState** st_out);
 // Frees per-device scratch owned by the library (vk_shutdown).
 void release_device_state();
 // Frees the host-buffer pipeline's staging buffers and streams (vk_shutdown).

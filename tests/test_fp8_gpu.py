@@ -1,0 +1,548 @@
+"""GPU: the 8-bit linear layer against its definition in 64 bits (oracle/fp8.py, numpy and torch float64).
+
+Tolerances, all from arithmetic (u = 2^-24, half a step of fp32; h(t) = eps/2, half a step of the output's type):
+  quantize   bit for bit: v * 2^-e is exact, so one rounding decides, the same one
+  rstd       the sum of squares adds at most 100 terms one after the other on any path: relative error < 100 u
+  norm       y carries rstd's error and two products': < 104 u; its 8-bit form may be half an e4m3 step off
+             (2^-4 of the value, 2^-10 of the scale below e4m3's normal numbers), and a scale one power of two off
+             only where the block's largest value is within 104 u of the border
+  backward   sums as above: 104 u of the sum of magnitudes, and one rounding to the output's type; dweight adds
+             rows/296 terms in one thread, and 37 + 8 partial sums
+  products   fp32 accumulation in any order: k u of the sum of magnitudes, and one rounding
+"""
+import itertools
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from oracle import fp8  # noqa: E402
+
+U = 2.0 ** -24
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+HALF = {F16: 2.0 ** -11, BF16: 2.0 ** -8, F32: 2.0 ** -24}
+TINY = {F16: 2.0 ** -25, BF16: 2.0 ** -134, F32: 2.0 ** -150}  # half a step below the smallest normal number
+
+
+@pytest.fixture(scope="module")
+def vk():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import vibekernel_b200 as vkm
+    return vkm
+
+
+@pytest.fixture(autouse=True)
+def no_device_error(vk):
+    yield
+    torch.cuda.synchronize()
+    assert vk.device_error(0) == 0
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _rand(shape, dtype, seed, std=1.0):
+    return (torch.randn(*shape, generator=_gen(seed), device="cuda") * std).to(dtype)
+
+
+def _bytes(t):
+    return t.contiguous().view(torch.uint8).cpu().numpy()
+
+
+def _inside(shape, dtype, lead, tail, fill=0x55):
+    """A [rows, cols] view that starts `lead` elements into its rows, with `tail` more behind; all filled with `fill`."""
+    size = torch.empty((), dtype=dtype).element_size()
+    room = torch.full((shape[0] + 2, (lead + shape[1] + tail) * size), fill, dtype=torch.uint8, device="cuda").view(dtype)
+    return room[1:-1, lead:lead + shape[1]], room
+
+
+def _untouched(room, view_shape, lead, fill=0x55):
+    b = room.view(torch.uint8).reshape(room.shape[0], room.shape[1], -1)
+    rows, cols = view_shape
+    assert (b[0] == fill).all() and (b[-1] == fill).all()
+    assert (b[:, :lead] == fill).all() and (b[:, lead + cols:] == fill).all()
+
+
+def _deq(q, s, tile=False):
+    """Values in float64 on the GPU."""
+    w = torch.from_numpy(fp8.E4M3).cuda()[q.contiguous().view(torch.uint8).long()]
+    e = torch.from_numpy(fp8.E8M0).cuda()[s.contiguous().view(torch.uint8).long()]
+    e = e.repeat_interleave(128, 0)[: q.shape[0]] if tile else e
+    return w * e.repeat_interleave(128, 1)[:, : q.shape[1]]
+
+
+def _quantized(shape, seed, tile=False, std=1.0, pad=True):
+    """An 8-bit operand made by the oracle's own rounding (rows padded to 16 bytes, or dense)."""
+    v = np.random.default_rng(seed).standard_normal(shape) * std
+    v *= np.exp(np.random.default_rng(seed + 1).standard_normal((1, shape[1])))
+    codes, s = fp8.quantize(v.astype(np.float32), tile)
+    q, _ = _inside(shape, torch.float8_e4m3fn, 0, -shape[1] % 16 if pad else 0, 0x7f)  # NaN around it
+    q.copy_(torch.from_numpy(codes).cuda().view(torch.float8_e4m3fn))
+    return q, torch.from_numpy(s).cuda().view(torch.float8_e8m0fnu)
+
+
+# ------------------------------------------------------------------------------------------ quantize
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 4096), (3, 127), (129, 128), (128, 129), (300, 1000), (7, 3000), (1000, 64), (0, 5)])
+def test_quantize_bitwise(vk, shape, tile, dtype):
+    x = _rand(shape, dtype, 1)
+    if shape[0] > 1:
+        x[1] *= 1e-4
+        x[shape[0] // 2, ::3] = 0
+    q, s = vk.quantize_fp8(x, tile=tile)
+    codes, scale = fp8.quantize(x.double().cpu().numpy(), tile)
+    assert q.dtype == torch.float8_e4m3fn and s.dtype == torch.float8_e8m0fnu
+    np.testing.assert_array_equal(_bytes(s), scale)
+    np.testing.assert_array_equal(_bytes(q), codes)
+
+
+@pytest.mark.parametrize("tile", [False, True])
+def test_quantize_special_values(vk, tile):
+    """Zeros, subnormal and huge values, values on a scale's border, infinities and NaN, each in a block of its own."""
+    x = torch.zeros(256, 128 * 9)
+    x[0, 5] = 1e-44
+    x[0, 128:256] = torch.finfo(F32).max
+    x[0, 256] = 448.0
+    x[0, 384] = float(np.nextafter(np.float32(448.0), np.float32(500)))
+    x[0, 512] = float("inf")
+    x[0, 640] = float("nan")
+    x[0, 768:896] = torch.linspace(-2.0 ** -130, 2.0 ** -127, 128)
+    x[0, 896:1024] = torch.linspace(-1, 1, 128) * 2.0 ** -9
+    q, s = vk.quantize_fp8(x.cuda(), tile=tile)
+    codes, scale = fp8.quantize(x.double().numpy(), tile)
+    np.testing.assert_array_equal(_bytes(s), scale)
+    np.testing.assert_array_equal(_bytes(q), codes)
+    assert scale[0, 4] == 255 and scale[0, 5] == 255 and scale[0, 8] == 127
+
+
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("lead,tail", [(0, 0), (1, 0), (8, 8), (3, 6)])
+def test_quantize_strides_and_surroundings(vk, tile, lead, tail):
+    shape = (150, 333)
+    x, _ = _inside(shape, BF16, lead, tail, 0x7f)
+    x.copy_(_rand(shape, BF16, 2))
+    q, qroom = _inside(shape, torch.float8_e4m3fn, lead, tail)
+    s_shape = (2 if tile else 150, 3)
+    s, sroom = _inside(s_shape, torch.float8_e8m0fnu, lead, tail)
+    vk.quantize_fp8(x, tile=tile, q=q, scale=s)
+    codes, scale = fp8.quantize(x.double().cpu().numpy(), tile)
+    np.testing.assert_array_equal(_bytes(q), codes)
+    np.testing.assert_array_equal(_bytes(s), scale)
+    _untouched(qroom, shape, lead)
+    _untouched(sroom, s_shape, lead)
+
+
+# ------------------------------------------------------------------------------------------ norm
+def _check_norm(x, w, residual, eps, q, s, h, rstd):
+    want_h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    assert torch.equal(h, want_h)
+    h64 = want_h.double()
+    r64 = (h64.square().mean(dim=1) + eps).rsqrt()
+    assert ((rstd.double() - r64).abs() <= 100 * U * r64).all()
+    y = h64 * r64[:, None] * w.double()
+    yn = y.cpu().numpy()
+    top = fp8.tops(yn, False)
+    scale = fp8.E8M0[_bytes(s)]
+    near = 104 * U
+    some = top > 0
+    assert (scale[~some] == 1).all()
+    assert (top[some] * (1 - near) <= 448 * scale[some]).all()
+    assert ((top[some] * (1 + near) > 224 * scale[some]) | (scale[some] == 2.0 ** -127)).all()
+    deq = _deq(q, s).cpu().numpy()
+    per = fp8.spread(scale, yn.shape, False)
+    assert (np.abs(deq - yn) <= np.maximum(2.0 ** -4 * np.abs(yn), 2.0 ** -10 * per) * (1 + 2.0 ** -12) + near * np.abs(yn)).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 4096), (2, 127), (5, 128), (33, 1000), (9, 2048), (4, 2056), (3, 4100), (6, 8192),
+                                   (3, 8200), (2, 20001), (1000, 64)])
+def test_norm(vk, shape, with_residual, dtype):
+    x, w = _rand(shape, dtype, 3, 2.0), _rand((shape[1],), dtype, 4)
+    r = _rand(shape, dtype, 5, 3.0) if with_residual else None
+    out = vk.rmsnorm_fp8(x, w, residual=r, eps=1e-5)
+    _check_norm(x, w, r, 1e-5, *out)
+
+
+@pytest.mark.parametrize("cols", [333, 4096, 9000])
+@pytest.mark.parametrize("lead,tail", [(1, 2), (8, 8)])
+def test_norm_strides_and_surroundings(vk, cols, lead, tail):
+    shape = (5, cols)
+    x, _ = _inside(shape, BF16, lead, tail, 0x7f)
+    r, _ = _inside(shape, BF16, lead, tail, 0x7f)
+    x.copy_(_rand(shape, BF16, 6))
+    r.copy_(_rand(shape, BF16, 7))
+    h, hroom = _inside(shape, BF16, lead, tail)
+    q, qroom = _inside(shape, torch.float8_e4m3fn, lead, tail)
+    s_shape = (5, (cols + 127) // 128)
+    s, sroom = _inside(s_shape, torch.float8_e8m0fnu, lead, tail)
+    w = _rand((cols + 1,), BF16, 8)[1:]
+    out = vk.rmsnorm_fp8(x, w, residual=r, q=q, scale=s, h=h)
+    _check_norm(x, w, r, 1e-6, *out)
+    for room, sh in ((hroom, shape), (qroom, shape), (sroom, s_shape)):
+        _untouched(room, sh, lead)
+
+
+@pytest.mark.parametrize("cols", [1000, 4096, 9000])
+def test_norm_in_place(vk, cols):
+    x, r, w = _rand((7, cols), F16, 9), _rand((7, cols), F16, 10), _rand((cols,), F16, 11)
+    want = vk.rmsnorm_fp8(x, w, residual=r)
+    for which in (0, 1):
+        a, b = x.clone(), r.clone()
+        got = vk.rmsnorm_fp8(a, w, residual=b, h=(a, b)[which])
+        assert got[2] is (a, b)[which]
+        for g, e in zip(got, want):
+            assert torch.equal(g.view(torch.uint8), e.view(torch.uint8))
+
+
+def test_norm_rows_of_zeros_and_non_finite_rows(vk):
+    x = _rand((4, 512), BF16, 12)
+    x[1] = 0
+    x[2, 300] = float("inf")
+    x[3, 10] = float("nan")
+    q, s, h, rstd = vk.rmsnorm_fp8(x, torch.ones(512, dtype=BF16, device="cuda"), eps=1e-6)
+    assert (_bytes(q)[1] & 127 == 0).all() and (_bytes(s)[1] == 127).all() and abs(rstd[1].item() - 1e3) < 1e3 * 100 * U
+    # an infinity: rstd is 0 and 0 * inf is NaN in its block, 0 in the others
+    assert rstd[2].item() == 0 and _bytes(s)[2].tolist() == [127, 127, 255, 127]
+    assert np.isnan(rstd[3].item()) and (_bytes(s)[3] == 255).all() and (_bytes(q)[3] & 127 == 127).all()
+    clean = vk.rmsnorm_fp8(x[:1], torch.ones(512, dtype=BF16, device="cuda"), eps=1e-6)
+    assert torch.equal(q[:1].view(torch.uint8), clean[0].view(torch.uint8))
+
+
+def _check_norm_back(dy, h, w, rstd, dres, dx, dw):
+    n, rows = dy.shape[1], dy.shape[0]
+    a, b, g64, r = dy.double(), h.double(), w.double(), rstd.double()[:, None]
+    g, xhat = a * g64, b * r
+    mean = (g * xhat).mean(dim=1, keepdim=True)
+    want = r * (g - xhat * mean)
+    size = r * (g.abs() + xhat.abs() * (g * xhat).abs().mean(dim=1, keepdim=True))
+    if dres is not None:
+        want, size = want + dres.double(), size + dres.double().abs()
+    tol = 104 * U * size + HALF[dy.dtype] * (1 + 2.0 ** -8) * want.abs() + TINY[dy.dtype]
+    assert ((dx.double() - want).abs() <= tol).all()
+    wsize = (a * xhat).abs().sum(dim=0)
+    depth = -(-rows // 296) + 37 + 8 + 4
+    assert ((dw.double() - (a * xhat).sum(dim=0)).abs() <= depth * U * wsize).all()
+    assert dw.dtype == F32 and dx.dtype == dy.dtype and n == dw.shape[0]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("with_res", [False, True])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 4096), (2, 127), (300, 128), (777, 1000), (297, 2048), (5, 2056), (400, 4096),
+                                   (6, 8192), (3, 8200), (600, 8193), (2, 20001)])
+def test_norm_backward(vk, shape, with_res, dtype):
+    dy, h, w = _rand(shape, dtype, 13, 0.1), _rand(shape, dtype, 14, 2.0), _rand((shape[1],), dtype, 15)
+    rstd = (h.float().square().mean(dim=1) + 1e-6).rsqrt()
+    dres = _rand(shape, dtype, 16, 0.1) if with_res else None
+    dx, dw = vk.rmsnorm_fp8_backward(dy, h, w, rstd, dres=dres)
+    _check_norm_back(dy, h, w, rstd, dres, dx, dw)
+
+
+@pytest.mark.parametrize("cols", [333, 4096, 9000])
+def test_norm_backward_strides_in_place_and_surroundings(vk, cols):
+    shape = (310, cols)
+    rstd = torch.rand(310, generator=_gen(17), device="cuda") + 0.5
+    w = _rand((cols + 1,), F16, 18)[1:]
+    mats = []
+    for i in range(3):
+        m, _ = _inside(shape, F16, 1, 2, 0x7f)
+        m.copy_(_rand(shape, F16, 19 + i))
+        mats.append(m)
+    dy, h, dres = mats
+    dx, room = _inside(shape, F16, 1, 2)
+    dx, dw = vk.rmsnorm_fp8_backward(dy, h, w, rstd, dres=dres, dx=dx)
+    _check_norm_back(dy, h, w, rstd, dres, dx, dw)
+    _untouched(room, shape, 1)
+    for which in (0, 2):
+        copies = [m.clone() for m in mats]
+        got, dw2 = vk.rmsnorm_fp8_backward(copies[0], copies[1], w, rstd, dres=copies[2], dx=copies[which])
+        assert torch.equal(got, dx) and torch.equal(dw2, dw)
+
+
+def test_norm_backward_of_no_rows(vk):
+    e = torch.empty((0, 256), dtype=BF16, device="cuda")
+    dw = torch.full((256,), 7.0, device="cuda")
+    dx, dw = vk.rmsnorm_fp8_backward(e, e, torch.ones(256, dtype=BF16, device="cuda"), torch.empty(0, device="cuda"), dweight=dw)
+    assert dx.shape == (0, 256) and (dw == 0).all()
+
+
+def test_norm_backward_against_differences(vk):
+    """dx and dweight against central differences of the norm in 64 bits."""
+    shape = (3, 40)
+    dy, h, w = _rand(shape, BF16, 23), _rand(shape, BF16, 24), _rand((40,), BF16, 25)
+    rstd = (h.double().square().mean(dim=1) + 1e-6).rsqrt().float()
+    dx, dw = vk.rmsnorm_fp8_backward(dy, h, w, rstd)
+
+    def loss(hh, ww):
+        return (dy.double() * hh * (hh.square().mean(dim=1, keepdim=True) + 1e-6).rsqrt() * ww).sum()
+
+    step = 1e-5
+    h64, w64 = h.double(), w.double()
+    for r, c in itertools.product(range(3), (0, 17, 39)):
+        d = torch.zeros_like(h64)
+        d[r, c] = step
+        diff = (loss(h64 + d, w64) - loss(h64 - d, w64)) / (2 * step)
+        assert abs(diff - dx[r, c].double()) <= HALF[BF16] * abs(diff) + 1e-6
+    for c in (0, 17, 39):
+        d = torch.zeros_like(w64)
+        d[c] = step
+        diff = (loss(h64, w64 + d) - loss(h64, w64 - d)) / (2 * step)
+        assert abs(diff - dw[c].double()) <= 1e-5
+
+
+# ------------------------------------------------------------------------------------------ products
+def _check_product(got, want, size, k, base=None):
+    t = got.dtype
+    if base is not None:
+        want, size = want + base.double(), size + base.double().abs()
+    tol = max(k, 1) * U * size + HALF[t] * (1 + 2.0 ** -8) * want.abs() + TINY[t]
+    assert got.shape == want.shape
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+SHAPES = [(1, 1, 1), (1, 128, 128), (1, 4096, 512), (3, 130, 129), (8, 1000, 4096), (16, 256, 3000), (17, 136, 200), (33, 520, 640),
+          (64, 300, 1032), (65, 264, 130), (128, 128, 1), (129, 257, 384), (200, 136, 72), (256, 256, 512), (300, 520, 1000),
+          (513, 1025, 2049), (1024, 768, 3000)]
+
+
+@pytest.mark.parametrize("out", [F16, BF16, F32])
+@pytest.mark.parametrize("layout", ["nt_tile", "nt_row", "nn"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gemm(vk, shape, layout, out):
+    m, n, k = shape
+    tile, trans = layout != "nt_row", layout != "nn"
+    a, sa = _quantized((m, k), 30)
+    b, sb = _quantized((n, k) if trans else (k, n), 31, tile, 0.05)
+    c = vk.gemm_fp8(a, sa, b, sb, trans_b=trans, out_dtype=out)
+    av, bv = _deq(a, sa), _deq(b, sb, tile)
+    bv = bv.t() if trans else bv
+    _check_product(c, av @ bv, av.abs() @ bv.abs(), k)
+
+
+@pytest.mark.parametrize("m", [4, 200])
+def test_gemm_tile_scales_of_a(vk, m):
+    a, sa = _quantized((m, 1000), 32, True)
+    b, sb = _quantized((300, 1000), 33, True)
+    c = vk.gemm_fp8(a, sa, b, sb, trans_b=True, out_dtype=F32)
+    av, bv = _deq(a, sa, True), _deq(b, sb, True).t()
+    _check_product(c, av @ bv, av.abs() @ bv.abs(), 1000)
+
+
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("m", [5, 150])
+@pytest.mark.parametrize("lead,tail", [(1, 2), (16, 16), (0, 3)])
+def test_gemm_strides_and_surroundings(vk, m, lead, tail, layout):
+    """Views inside larger NaN-filled matrices: aligned ones and ones that the tensor-core loads cannot take."""
+    n, k = 264, 333
+    trans = layout == "nt"
+    a0, sa0 = _quantized((m, k), 34)
+    b0, sb0 = _quantized((n, k) if trans else (k, n), 35, True)
+
+    def placed(t, dtype, fill):
+        v, _ = _inside(tuple(t.shape), dtype, lead, tail + (-(lead + t.shape[1] + tail) % 16 if lead % 16 == 0 and tail != 3 else 0), fill)
+        return v.copy_(t)
+
+    a, b = placed(a0, torch.float8_e4m3fn, 0x7f), placed(b0, torch.float8_e4m3fn, 0x7f)
+    sa, sb = placed(sa0, torch.float8_e8m0fnu, 0xff), placed(sb0, torch.float8_e8m0fnu, 0xff)
+    c, room = _inside((m, n), BF16, lead, tail)
+    vk.gemm_fp8(a, sa, b, sb, c, trans_b=trans)
+    av, bv = _deq(a, sa), _deq(b, sb, True)
+    bv = bv.t() if trans else bv
+    _check_product(c, av @ bv, av.abs() @ bv.abs(), k)
+    _untouched(room, (m, n), lead)
+
+
+@pytest.mark.parametrize("m", [2, 300])
+def test_gemm_of_nothing(vk, m):
+    a = torch.empty((m, 0), dtype=torch.float8_e4m3fn, device="cuda")
+    b = torch.empty((40, 0), dtype=torch.float8_e4m3fn, device="cuda")
+    sa, sb = torch.empty((m, 0), dtype=torch.float8_e8m0fnu, device="cuda"), torch.empty((1, 0), dtype=torch.float8_e8m0fnu, device="cuda")
+    c = torch.full((m, 40), 3.0, dtype=F16, device="cuda")
+    assert (vk.gemm_fp8(a, sa, b, sb, c, trans_b=True) == 0).all()
+
+
+@pytest.mark.parametrize("m", [2, 300])
+def test_gemm_nan_block_stays_in_its_row(vk, m):
+    """A NaN scale makes the whole row of C NaN and nothing else; scales at both ends of their range are exact."""
+    a, sa = _quantized((m, 512), 36)
+    b, sb = _quantized((256, 512), 37, True)
+    raw = sa.view(torch.uint8)
+    raw[1, 2] = 255
+    raw[0, :] = 127 - 100
+    sb.view(torch.uint8)[:] = 127 + 60
+    c = vk.gemm_fp8(a, sa, b, sb, trans_b=True, out_dtype=F32)
+    assert c[1].isnan().all() and not c[[0, *range(2, m)]].isnan().any()
+    av, bv = _deq(a, sa), _deq(b, sb, True).t()
+    keep = [0, *range(2, m)]
+    _check_product(c[keep], av[keep] @ bv, av[keep].abs() @ bv.abs(), 512)
+
+
+def test_gemm_refusals(vk):
+    a, sa = _quantized((8, 256), 38)
+    b, sb = _quantized((256, 256), 39)
+    with pytest.raises(vk.VkError, match="tile scales"):
+        vk.gemm_fp8(a, sa, b, sb)
+    with pytest.raises(ValueError, match="b_scale"):
+        vk.gemm_fp8(a, sa, b, sb[:5], trans_b=True)
+    with pytest.raises(ValueError, match="trans_b"):
+        vk.gemm_fp8(a, sa, b[:, :128], sb[:, :1], trans_b=True)
+    with pytest.raises(TypeError):
+        vk.gemm_fp8(a.view(torch.uint8), sa, b, sb, trans_b=True)
+    with pytest.raises(ValueError, match="overlapping"):
+        vk.gemm_fp8(a[:1].expand(8, 256), sa, b, sb, trans_b=True)
+    with pytest.raises(ValueError, match="unit column stride"):
+        vk.gemm_fp8(a, sa, b.t(), sb, trans_b=True)
+    with pytest.raises(TypeError):
+        vk.gemm_fp8(a, sa, b, sb, trans_b=True, out_dtype=torch.int8)
+
+
+WG_SHAPES = [(1, 1, 1), (1, 128, 128), (5, 8, 40), (64, 128, 128), (100, 136, 129), (300, 264, 200), (128, 512, 640), (777, 256, 300),
+             (2000, 128, 256), (5000, 200, 136), (1000, 520, 1032)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("out", [None, F32])
+@pytest.mark.parametrize("shape", WG_SHAPES)
+def test_wgrad(vk, shape, dtype, out):
+    t, n, k = shape
+    dy = _rand((t, n), dtype, 40, 0.1)
+    x, sx = _quantized((t, k), 41)
+    dw = vk.wgrad_fp8(dy, x, sx, out_dtype=out)
+    assert dw.dtype == (out or dtype)
+    d, xv = dy.double().t(), _deq(x, sx)
+    _check_product(dw, d @ xv, d.abs() @ xv.abs(), t)
+    base = _rand((n, k), out or dtype, 42)
+    acc = vk.wgrad_fp8(dy, x, sx, base.clone(), accumulate=True)
+    _check_product(acc, d @ xv, d.abs() @ xv.abs(), t, base)
+
+
+@pytest.mark.parametrize("lead,tail", [(1, 2), (16, 16)])
+def test_wgrad_strides_and_surroundings(vk, lead, tail):
+    t, n, k = 333, 264, 200
+    dy, _ = _inside((t, n), BF16, lead, tail + (-(lead + n + tail) % 8 if lead == 16 else 0), 0x7f)
+    dy.copy_(_rand((t, n), BF16, 43))
+    x0, s0 = _quantized((t, k), 44)
+    x, _ = _inside((t, k), torch.float8_e4m3fn, lead, tail + (-(lead + k + tail) % 16 if lead == 16 else 0), 0x7f)
+    s, _ = _inside((t, 2), torch.float8_e8m0fnu, lead, tail, 0xff)
+    x.copy_(x0)
+    s.copy_(s0)
+    dw, room = _inside((n, k), BF16, lead, tail)
+    vk.wgrad_fp8(dy, x, s, dw)
+    d, xv = dy.double().t(), _deq(x, s)
+    _check_product(dw, d @ xv, d.abs() @ xv.abs(), t)
+    _untouched(room, (n, k), lead)
+
+
+def test_wgrad_of_no_tokens(vk):
+    dy = torch.empty((0, 64), dtype=BF16, device="cuda")
+    x = torch.empty((0, 40), dtype=torch.float8_e4m3fn, device="cuda")
+    s = torch.empty((0, 1), dtype=torch.float8_e8m0fnu, device="cuda")
+    assert (vk.wgrad_fp8(dy, x, s) == 0).all()
+    base = _rand((64, 40), F32, 45)
+    assert torch.equal(vk.wgrad_fp8(dy, x, s, base.clone(), accumulate=True), base)
+
+
+def test_wgrad_values_outside_fp16(vk):
+    """fp16 holds a checkpoint's values above its range at its largest number, and is exact for what it can hold."""
+    x = torch.zeros((64, 128), dtype=BF16, device="cuda")
+    x[:, 0], x[:, 1], x[:, 2] = 1e6, 65504.0, 2.0 ** -12
+    q, s = vk.quantize_fp8(x)
+    dy = torch.ones((64, 8), dtype=F16, device="cuda") / 64
+    dw = vk.wgrad_fp8(dy, q, s, out_dtype=F32)
+    want = _deq(q, s).clamp(-65504, 65504)[0]
+    assert torch.equal(dw[0].double(), want)
+
+
+# ------------------------------------------------------------------------------------------ together
+def _layer(vk, x, res, wn, wq, ws, dy, dres):
+    """A linear layer behind a norm, forward and backward, as a training step calls it."""
+    q, s, h, rstd = vk.rmsnorm_fp8(x, wn, residual=res)
+    y = vk.gemm_fp8(q, s, wq, ws, trans_b=True, out_dtype=BF16)
+    dyq, dys = vk.quantize_fp8(dy)
+    dn = vk.gemm_fp8(dyq, dys, wq, ws, out_dtype=BF16)
+    dw = vk.wgrad_fp8(dy, q, s, out_dtype=F32)
+    dx, dwn = vk.rmsnorm_fp8_backward(dn, h, wn, rstd, dres=dres)
+    return {"q": q, "s": s, "h": h, "rstd": rstd, "y": y, "dyq": dyq, "dys": dys, "dn": dn, "dw": dw, "dx": dx, "dwn": dwn}
+
+
+def _layer_inputs(seed, t=300, k=640, n=520):
+    x, res, wn = _rand((t, k), BF16, seed), _rand((t, k), BF16, seed + 1, 3.0), _rand((k,), BF16, seed + 2)
+    wq, ws = _quantized((n, k), seed + 3, True, 0.05)
+    return [x, res, wn, wq, ws, _rand((t, n), BF16, seed + 4, 0.1), _rand((t, k), BF16, seed + 5, 0.1)]
+
+
+def _check_layer(o, x, res, wn, wq, ws, dy, dres):
+    _check_norm(x, wn, res, 1e-6, o["q"], o["s"], o["h"], o["rstd"])
+    a, w, d = _deq(o["q"], o["s"]), _deq(wq, ws, True), _deq(o["dyq"], o["dys"])
+    _check_product(o["y"], a @ w.t(), a.abs() @ w.t().abs(), a.shape[1])
+    codes, scale = fp8.quantize(dy.double().cpu().numpy())
+    np.testing.assert_array_equal(_bytes(o["dyq"]), codes)
+    np.testing.assert_array_equal(_bytes(o["dys"]), scale)
+    _check_product(o["dn"], d @ w, d.abs() @ w.abs(), w.shape[0])
+    _check_product(o["dw"], dy.double().t() @ a, dy.double().abs().t() @ a.abs(), a.shape[0])
+    _check_norm_back(o["dn"], o["h"], wn, o["rstd"], dres, o["dx"], o["dwn"])
+
+
+@pytest.mark.parametrize("sizes", [(1, 4096, 512), (300, 640, 520), (520, 1000, 264)])
+def test_layer_forward_and_backward(vk, sizes):
+    t, k, n = sizes
+    data = _layer_inputs(50, t, k, n)
+    _check_layer(_layer(vk, *data), *data)
+
+
+def test_layer_is_the_same_every_time(vk):
+    data = _layer_inputs(60, 700, 1032, 1000)
+    first = _layer(vk, *data)
+    for _ in range(5):
+        for name, v in _layer(vk, *data).items():
+            assert torch.equal(v.view(torch.uint8), first[name].view(torch.uint8)), name
+
+
+def test_layer_captured_and_replayed(vk):
+    """Two graphs of the same calls, replayed on new inputs at the same time on two streams."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    held = [_layer_inputs(70 + 10 * i) for i in range(2)]
+    graphs, outs = [], []
+    for st, data in zip(streams, held):
+        with torch.cuda.stream(st):
+            _layer(vk, *data)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            outs.append(_layer(vk, *data))
+        graphs.append(g)
+    for i, data in enumerate(held):
+        for old, new in zip(data, _layer_inputs(90 + 10 * i)):
+            old.copy_(new)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, data in zip(outs, held):
+        _check_layer(o, *data)
+
+
+def test_calls_on_a_given_stream(vk):
+    data = _layer_inputs(120)
+    want = _layer(vk, *data)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    x, res, wn, wq, ws, dy, dres = data
+    q, s, h, rstd = vk.rmsnorm_fp8(x, wn, residual=res, stream=st)
+    y = vk.gemm_fp8(q, s, wq, ws, trans_b=True, out_dtype=BF16, stream=st.cuda_stream)
+    dyq, dys = vk.quantize_fp8(dy, stream=st)
+    dn = vk.gemm_fp8(dyq, dys, wq, ws, out_dtype=BF16, stream=st)
+    dw = vk.wgrad_fp8(dy, q, s, out_dtype=F32, stream=st)
+    dx, dwn = vk.rmsnorm_fp8_backward(dn, h, wn, rstd, dres=dres, stream=st)
+    st.synchronize()
+    for got, name in ((q, "q"), (y, "y"), (dn, "dn"), (dw, "dw"), (dx, "dx"), (dwn, "dwn")):
+        assert torch.equal(got.view(torch.uint8), want[name].view(torch.uint8)), name

@@ -27,7 +27,8 @@ VK_ERR_NO_DEVICE = -5
 VK_ERR_NCCL = -6
 VK_ERR_ALIGNMENT = -7
 
-DTYPE_F16, DTYPE_F32 = 0, 1
+DTYPE_F16, DTYPE_F32, DTYPE_BF16 = 0, 1, 2
+FP8_ROW, FP8_TILE = 0, 1
 ACC_F32, ACC_F16 = 0, 1
 ALGO_AUTO, ALGO_TC_2SM, ALGO_TC_1SM, ALGO_FFMA, ALGO_SIMT = 0, 1, 2, 3, 4
 
@@ -42,6 +43,8 @@ EXPORTED = (
     "vk_gemm_host", "vk_gemm_ex", "vk_read_trace_cta", "vk_ipc_export", "vk_ipc_import", "vk_ipc_release",
     "vk_copy_async", "vk_debug_schedule", "vk_gemm_peers", "vk_gemm_mc", "vk_mc_supported", "vk_mc_alloc",
     "vk_mc_free", "vk_mc_create", "vk_mc_import", "vk_mc_attach", "vk_mc_detach", "vk_debug_watchdog",
+    "vk_quantize_fp8", "vk_rmsnorm_fp8", "vk_rmsnorm_fp8_workspace", "vk_rmsnorm_fp8_backward", "vk_gemm_fp8",
+    "vk_wgrad_fp8",
 )
 
 
@@ -84,6 +87,48 @@ class ShardArgs(ctypes.Structure):
 
 class IpcHandle(ctypes.Structure):
     _fields_ = [("handle", ctypes.c_uint8 * 64), ("offset", ctypes.c_uint64)]
+
+
+_P, _I64, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+
+
+class QuantizeFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("X", _P), ("Q", _P), ("scale", _P), ("rows", _I64), ("cols", _I64), ("ldx", _I64), ("ldq", _I64),
+        ("ld_scale", _I64), ("dtype", _I32), ("scaling", _I32), ("stream", _P),
+    ]
+
+
+class RmsnormFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("X", _P), ("residual", _P), ("weight", _P), ("Q", _P), ("scale", _P), ("H", _P), ("rstd", _P),
+        ("rows", _I64), ("cols", _I64), ("ldx", _I64), ("ld_residual", _I64), ("ldq", _I64), ("ld_scale", _I64),
+        ("ldh", _I64), ("eps", ctypes.c_float), ("dtype", _I32), ("stream", _P),
+    ]
+
+
+class RmsnormFp8BackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("dY", _P), ("H", _P), ("weight", _P), ("rstd", _P), ("dres", _P), ("dX", _P), ("dweight", _P),
+        ("workspace", _P), ("workspace_bytes", ctypes.c_size_t), ("rows", _I64), ("cols", _I64), ("lddy", _I64),
+        ("ldh", _I64), ("ld_dres", _I64), ("lddx", _I64), ("dtype", _I32), ("stream", _P),
+    ]
+
+
+class GemmFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("A", _P), ("B", _P), ("a_scale", _P), ("b_scale", _P), ("C", _P), ("m", _I64), ("n", _I64), ("k", _I64),
+        ("lda", _I64), ("ldb", _I64), ("ldc", _I64), ("ld_a_scale", _I64), ("ld_b_scale", _I64), ("a_scaling", _I32),
+        ("b_scaling", _I32), ("trans_b", _I32), ("dtype", _I32), ("stream", _P),
+    ]
+
+
+class WgradFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("dY", _P), ("X", _P), ("x_scale", _P), ("dW", _P), ("tokens", _I64), ("n", _I64), ("k", _I64), ("lddy", _I64),
+        ("ldx", _I64), ("ld_x_scale", _I64), ("lddw", _I64), ("dtype", _I32), ("out_dtype", _I32), ("accumulate", _I32),
+        ("stream", _P),
+    ]
 
 
 def _load() -> ctypes.CDLL:
@@ -163,6 +208,13 @@ def _load() -> ctypes.CDLL:
     lib.vk_debug_watchdog.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, i32p,
                                       ctypes.POINTER(ctypes.c_int64)]
     lib.vk_debug_watchdog.restype = ctypes.c_int
+    for name, args in (("quantize_fp8", QuantizeFp8Args), ("rmsnorm_fp8", RmsnormFp8Args), ("gemm_fp8", GemmFp8Args),
+                       ("rmsnorm_fp8_backward", RmsnormFp8BackwardArgs), ("wgrad_fp8", WgradFp8Args)):
+        fn = getattr(lib, "vk_" + name)
+        fn.argtypes = [ctypes.POINTER(args)]
+        fn.restype = ctypes.c_int
+    lib.vk_rmsnorm_fp8_workspace.argtypes = [_I64, _I64, ctypes.POINTER(ctypes.c_size_t)]
+    lib.vk_rmsnorm_fp8_workspace.restype = ctypes.c_int
     return lib
 
 
@@ -525,3 +577,274 @@ def debug_schedule(tiles: int, num_kb: int, max_units: int, k: int, split: bool 
 def row_blocks(m: int, parts: int):
     """Row offsets of the balanced split used by the sharded layer: GPU r owns [off[r], off[r+1])."""
     return [m * r // parts for r in range(parts + 1)]
+
+
+# ------------------------------------------------------------------------------------------
+# 8-bit linear layer
+# ------------------------------------------------------------------------------------------
+def _fp8_types():
+    import torch
+    return {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32, "q": torch.float8_e4m3fn,
+            "scale": torch.float8_e8m0fnu}
+
+
+def _dtype_code(t, *, f32: bool, what: str) -> int:
+    import torch
+    code = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32 if f32 else None}.get(t)
+    if code is None:
+        raise TypeError(f"{what} must be float16{', bfloat16 or float32' if f32 else ' or bfloat16'}, not {t}")
+    return code
+
+
+def _matrix(t, what: str, shape=None, dtypes=None, device=None) -> int:
+    """Checks a row-major CUDA matrix and returns its row pitch in elements."""
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor (no CPU fallback)")
+    if t.dim() != 2 or not _unit_col(t):
+        raise ValueError(f"{what} must be 2-D with unit column stride")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {tuple(shape)}, not {tuple(t.shape)}")
+    if dtypes is not None and t.dtype not in dtypes:
+        raise TypeError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what} is on {t.device}, not on {device}")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what} must not have overlapping rows")
+    return max(_row_pitch(t), 1)
+
+
+def _vector(t, what: str, n: int, dtype, device) -> None:
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or t.device != device:
+        raise ValueError(f"{what} must be a contiguous {dtype} vector of length {n} on {device}")
+
+
+class _On:
+    """The device of a call's tensors made current, and the stream it runs on: allocations inside belong to that stream."""
+
+    def __init__(self, device, stream):
+        import torch
+        self.device = device
+        self.guards = []
+        if torch.cuda.current_device() != device.index:
+            self.guards.append(torch.cuda.device(device))
+        if stream is not None:
+            if not hasattr(stream, "cuda_stream"):
+                stream = torch.cuda.ExternalStream(int(stream), device=device) if int(stream) else torch.cuda.default_stream(device)
+            self.guards.append(torch.cuda.stream(stream))
+
+    def __enter__(self):
+        import torch
+        for g in self.guards:
+            g.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream or None
+
+    def __exit__(self, *exc):
+        for g in reversed(self.guards):
+            g.__exit__(*exc)
+
+
+def _empty_fp8(rows: int, cols: int, device):
+    """A new 8-bit matrix whose rows start at 16-byte boundaries (what the tensor-core kernels' loads need)."""
+    import torch
+    q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)
+    return q if q.shape[1] == cols else q[:, :cols]
+
+
+def quantize_fp8(x, *, tile: bool = False, q=None, scale=None, stream=None):
+    """The 8-bit form (q, scale) of a matrix (``vk_quantize_fp8``): e4m3 values and power-of-two (e8m0) scales.
+
+    x is [rows, cols], float16, bfloat16 or float32, with unit column stride.  q is a float8_e4m3fn [rows, cols] tensor
+    (rows padded to 16 bytes when allocated here), scale a float8_e8m0fnu tensor: [rows, ceil(cols / 128)], a scale for
+    each 128 neighbouring values of a row (activations: what :func:`gemm_fp8` reads and what is kept for
+    :func:`wgrad_fp8`), or with ``tile`` [ceil(rows / 128), ceil(cols / 128)], one for each 128 x 128 (weights: the
+    same form serves the product with W^T and the one with W).  The value of an element is q * scale; a block with an
+    infinity or a NaN becomes NaN.  Asynchronous on ``stream`` (default: torch's current stream).
+    """
+    import torch
+    T = _fp8_types()
+    a = QuantizeFp8Args()
+    a.dtype = _dtype_code(x.dtype, f32=True, what="x")
+    a.ldx = _matrix(x, "x")
+    rows, cols = x.shape
+    s_shape = ((rows + 127) // 128 if tile else rows, (cols + 127) // 128)
+    with _On(x.device, stream) as handle:
+        if q is None:
+            q = _empty_fp8(rows, cols, x.device)
+        if scale is None:
+            scale = torch.empty(s_shape, dtype=T["scale"], device=x.device)
+        a.ldq = _matrix(q, "q", (rows, cols), (T["q"],), x.device)
+        a.ld_scale = _matrix(scale, "scale", s_shape, (T["scale"],), x.device)
+        a.X, a.Q, a.scale = x.data_ptr(), q.data_ptr(), scale.data_ptr()
+        a.rows, a.cols = rows, cols
+        a.scaling = FP8_TILE if tile else FP8_ROW
+        a.stream = handle
+        check(lib.vk_quantize_fp8(ctypes.byref(a)))
+    return q, scale
+
+
+def rmsnorm_fp8(x, weight, *, residual=None, eps: float = 1e-6, q=None, scale=None, h=None, rstd=None, stream=None):
+    """RMS norm of each row with an 8-bit output (``vk_rmsnorm_fp8``): returns (q, scale, h, rstd).
+
+    h = x + residual (in x's type; x itself without a residual), rstd = 1 / sqrt(mean(h^2) + eps) (float32, one per
+    row), and (q, scale) is the 8-bit form by rows of h * rstd * weight (see :func:`quantize_fp8`).  x and residual are
+    [rows, cols], float16 or bfloat16, weight a vector of the same type.  ``h`` may be x or residual itself (in place).
+    Outputs that are not given are allocated.
+    """
+    import torch
+    T = _fp8_types()
+    a = RmsnormFp8Args()
+    a.dtype = _dtype_code(x.dtype, f32=False, what="x")
+    a.ldx = _matrix(x, "x")
+    rows, cols = x.shape
+    dev = x.device
+    _vector(weight, "weight", cols, x.dtype, dev)
+    s_shape = (rows, (cols + 127) // 128)
+    with _On(dev, stream) as handle:
+        if residual is not None:
+            a.ld_residual = _matrix(residual, "residual", (rows, cols), (x.dtype,), dev)
+            if h is None:
+                h = torch.empty((rows, cols), dtype=x.dtype, device=dev)
+            a.ldh = _matrix(h, "h", (rows, cols), (x.dtype,), dev)
+            a.residual, a.H = residual.data_ptr(), h.data_ptr()
+        elif h is not None:
+            raise ValueError("h is given with a residual only (without one it is x)")
+        else:
+            h = x
+        if q is None:
+            q = _empty_fp8(rows, cols, dev)
+        if scale is None:
+            scale = torch.empty(s_shape, dtype=T["scale"], device=dev)
+        if rstd is None:
+            rstd = torch.empty((rows,), dtype=torch.float32, device=dev)
+        a.ldq = _matrix(q, "q", (rows, cols), (T["q"],), dev)
+        a.ld_scale = _matrix(scale, "scale", s_shape, (T["scale"],), dev)
+        _vector(rstd, "rstd", rows, torch.float32, dev)
+        a.X, a.weight, a.Q, a.scale, a.rstd = x.data_ptr(), weight.data_ptr(), q.data_ptr(), scale.data_ptr(), rstd.data_ptr()
+        a.rows, a.cols, a.eps = rows, cols, eps
+        a.stream = handle
+        check(lib.vk_rmsnorm_fp8(ctypes.byref(a)))
+    return q, scale, h, rstd
+
+
+def rmsnorm_fp8_backward(dy, h, weight, rstd, *, dres=None, dx=None, dweight=None, stream=None):
+    """The backward pass of :func:`rmsnorm_fp8` (``vk_rmsnorm_fp8_backward``): returns (dx, dweight).
+
+    dy is the gradient of the normalised output (the rounding to 8 bits passes gradients on unchanged), h and rstd are
+    what the forward pass returned, dres (optional) is the gradient that reaches h from elsewhere.  dx, in dy's type,
+    is the gradient of x and of the residual alike and may be dy or dres itself; dweight is float32.
+    """
+    import torch
+    a = RmsnormFp8BackwardArgs()
+    a.dtype = _dtype_code(dy.dtype, f32=False, what="dy")
+    a.lddy = _matrix(dy, "dy")
+    rows, cols = dy.shape
+    dev = dy.device
+    a.ldh = _matrix(h, "h", (rows, cols), (dy.dtype,), dev)
+    _vector(weight, "weight", cols, dy.dtype, dev)
+    _vector(rstd, "rstd", rows, torch.float32, dev)
+    if dres is not None:
+        a.ld_dres = _matrix(dres, "dres", (rows, cols), (dy.dtype,), dev)
+        a.dres = dres.data_ptr()
+    need = ctypes.c_size_t(0)
+    check(lib.vk_rmsnorm_fp8_workspace(rows, cols, ctypes.byref(need)))
+    with _On(dev, stream) as handle:
+        if dx is None:
+            dx = torch.empty((rows, cols), dtype=dy.dtype, device=dev)
+        if dweight is None:
+            dweight = torch.empty((cols,), dtype=torch.float32, device=dev)
+        a.lddx = _matrix(dx, "dx", (rows, cols), (dy.dtype,), dev)
+        _vector(dweight, "dweight", cols, torch.float32, dev)
+        work = torch.empty((need.value,), dtype=torch.uint8, device=dev)
+        a.dY, a.H, a.weight, a.rstd = dy.data_ptr(), h.data_ptr(), weight.data_ptr(), rstd.data_ptr()
+        a.dX, a.dweight, a.workspace, a.workspace_bytes = dx.data_ptr(), dweight.data_ptr(), work.data_ptr(), need.value
+        a.rows, a.cols = rows, cols
+        a.stream = handle
+        check(lib.vk_rmsnorm_fp8_backward(ctypes.byref(a)))
+    return dx, dweight
+
+
+def _scaling(scale, rows: int, cols: int, what: str, device):
+    """(vk_fp8_scaling, pitch) of the scales of a [rows, cols] matrix, told by their shape."""
+    T = _fp8_types()
+    blocks = (cols + 127) // 128
+    ld = _matrix(scale, what, None, (T["scale"],), device)
+    if tuple(scale.shape) == (rows, blocks):
+        return FP8_ROW, ld
+    if tuple(scale.shape) == ((rows + 127) // 128, blocks):
+        return FP8_TILE, ld
+    raise ValueError(f"{what} must be {(rows, blocks)} or {((rows + 127) // 128, blocks)}, not {tuple(scale.shape)}")
+
+
+def gemm_fp8(A, a_scale, B, b_scale, C=None, *, trans_b: bool = False, out_dtype=None, stream=None):
+    """C = A @ op(B) of 8-bit operands (``vk_gemm_fp8``), fp32 accumulation.
+
+    A is [m, k] and B [k, n], or [n, k] with ``trans_b``, float8_e4m3fn with float8_e8m0fnu scales as
+    :func:`quantize_fp8` makes them; a matrix's scales are taken by rows or by tiles according to their shape.  A B that
+    is stored [k, n] needs tile scales.  C is [m, n] in ``out_dtype`` (default float16; bfloat16 and float32 too).
+    Operands whose rows start at 16-byte boundaries run on the tensor cores; any others on a slow kernel.
+    """
+    import torch
+    T = _fp8_types()
+    a = GemmFp8Args()
+    a.lda = _matrix(A, "A", None, (T["q"],))
+    dev = A.device
+    a.ldb = _matrix(B, "B", None, (T["q"],), dev)
+    m, k = A.shape
+    n, kb = (B.shape[0], B.shape[1]) if trans_b else (B.shape[1], B.shape[0])
+    if kb != k:
+        raise ValueError(f"A is {tuple(A.shape)} and B is {tuple(B.shape)} with trans_b={bool(trans_b)}")
+    a.a_scaling, a.ld_a_scale = _scaling(a_scale, m, k, "a_scale", dev)
+    a.b_scaling, a.ld_b_scale = _scaling(b_scale, B.shape[0], B.shape[1], "b_scale", dev)
+    if not trans_b and B.shape[0] == 1:
+        a.b_scaling = FP8_TILE  # one row: both forms are the same scales
+    if C is not None:
+        out_dtype = out_dtype or C.dtype
+    out_dtype = out_dtype or torch.float16
+    a.dtype = _dtype_code(out_dtype, f32=True, what="out_dtype")
+    with _On(dev, stream) as handle:
+        if C is None:
+            C = torch.empty((m, n), dtype=out_dtype, device=dev)
+        a.ldc = _matrix(C, "C", (m, n), (out_dtype,), dev)
+        a.A, a.B, a.a_scale, a.b_scale, a.C = A.data_ptr(), B.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), C.data_ptr()
+        a.m, a.n, a.k = m, n, k
+        a.trans_b = int(bool(trans_b))
+        a.stream = handle
+        check(lib.vk_gemm_fp8(ctypes.byref(a)))
+    return C
+
+
+def wgrad_fp8(dY, X, x_scale, dW=None, *, accumulate: bool = False, out_dtype=None, stream=None):
+    """dW = dY^T @ X, or dW += it with ``accumulate`` (``vk_wgrad_fp8``): a linear layer's weight gradient.
+
+    dY is [tokens, n], float16 or bfloat16; X is [tokens, k] in 8 bits with scales by rows, as the forward pass kept it
+    (:func:`quantize_fp8`, or the output of :func:`rmsnorm_fp8`).  dW is [n, k] in ``out_dtype`` (default dY's type;
+    float32 too), fp32 accumulation.  X's values enter the product in dY's type (exact in bfloat16).
+    """
+    import torch
+    T = _fp8_types()
+    a = WgradFp8Args()
+    a.dtype = _dtype_code(dY.dtype, f32=False, what="dY")
+    a.lddy = _matrix(dY, "dY")
+    dev = dY.device
+    tokens, n = dY.shape
+    a.ldx = _matrix(X, "X", None, (T["q"],), dev)
+    if X.shape[0] != tokens:
+        raise ValueError(f"dY is {tuple(dY.shape)} and X is {tuple(X.shape)}")
+    k = X.shape[1]
+    a.ld_x_scale = _matrix(x_scale, "x_scale", (tokens, (k + 127) // 128), (T["scale"],), dev)
+    if accumulate and dW is None:
+        raise ValueError("accumulate needs dW")
+    if dW is not None:
+        out_dtype = out_dtype or dW.dtype
+    out_dtype = out_dtype or dY.dtype
+    a.out_dtype = _dtype_code(out_dtype, f32=True, what="out_dtype")
+    with _On(dev, stream) as handle:
+        if dW is None:
+            dW = torch.empty((n, k), dtype=out_dtype, device=dev)
+        a.lddw = _matrix(dW, "dW", (n, k), (out_dtype,), dev)
+        a.dY, a.X, a.x_scale, a.dW = dY.data_ptr(), X.data_ptr(), x_scale.data_ptr(), dW.data_ptr()
+        a.tokens, a.n, a.k = tokens, n, k
+        a.accumulate = int(bool(accumulate))
+        a.stream = handle
+        check(lib.vk_wgrad_fp8(ctypes.byref(a)))
+    return dW
