@@ -4,9 +4,12 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstring>
+#include <type_traits>
 
 #include "vkgemm.h"
+#include "fp8_gemm.cuh"
 #include "fp8_rows.cuh"
 #include "fp8_simt.cuh"
 #include "vk_internal.h"
@@ -69,7 +72,120 @@ int launched()
     return VK_OK;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encoder()
+{
+    static const EncodeTiledFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    return fn;
+}
+
+// Map of a row-major matrix of 1-, 2- or 4-byte elements (bits are only moved): box_cols x box_rows boxes, zeros outside.
+int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, long long ld, int esize, uint32_t box_cols,
+             uint32_t box_rows, CUtensorMapSwizzle swizzle)
+{
+    const EncodeTiledFn encode = encoder();
+    if (encode == nullptr) return set_error(VK_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * esize};
+    const cuuint32_t box[2] = {box_cols, box_rows}, steps[2] = {1, 1};
+    const CUtensorMapDataType type = esize == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+    const CUresult r = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(VK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) rows=%lld cols=%lld ld=%lld", (int)r,
+                         (long long)rows, (long long)cols, ld);
+    return VK_OK;
+}
+
+bool tma_ok(const void* p, long long ld, int esize) { return rows_at(p, ld, esize, 16) && ld * esize < (1LL << 40); }
+
+int make_out_map(CUtensorMap* map, void* c, int64_t m, int64_t n, long long ldc, int dtype, int* c_tma)
+{
+    const int esize = static_cast<int>(bytes_of(dtype));
+    memset(map, 0, sizeof(*map));
+    *c_tma = tma_ok(c, ldc, esize);
+    if (!*c_tma) return VK_OK;
+    return make_map(map, c, m, n, ldc, esize, 32, 32, esize == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// Clusters of each kernel that fit on each device (0: not asked yet; its shared-memory attribute is set by then).
+constexpr int kKernels = 16, kDevices = 64;
+std::atomic<int> g_clusters[kKernels][kDevices];
+
+template <typename Kernel>
+int prepare_kernel(Kernel fn, int id, int smem, int threads, int cluster, int* clusters)
+{
+    int dev = 0;
+    F8_CUDA_TRY(cudaGetDevice(&dev));
+    std::atomic<int>& known = g_clusters[id][dev];
+    *clusters = known.load(std::memory_order_acquire);
+    if (*clusters > 0) return VK_OK;
+    F8_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    int sms = 0;
+    F8_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(sms / cluster * cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    F8_CUDA_TRY(cudaOccupancyMaxActiveClusters(clusters, fn, &cfg));
+    if (*clusters <= 0) return set_error(VK_ERR_CUDA, "kernel cannot be resident (%d bytes of shared memory)", smem);
+    known.store(*clusters, std::memory_order_release);
+    return VK_OK;
+}
+
+template <typename Kernel, typename... Args>
+int launch_clusters(Kernel fn, int clusters, int cluster, int threads, int smem, cudaStream_t stream, const Args&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(clusters * cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    F8_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, args...));
+    return VK_OK;
+}
+
 }  // namespace
+
+namespace vk {
+void release_fp8_state()
+{
+    for (auto& kernel : g_clusters)
+        for (auto& device : kernel) device.store(0, std::memory_order_release);
+}
+
+cudaError_t fp8_error_word(unsigned long long* word, bool clear)
+{
+    cudaError_t e = cudaMemcpyFromSymbol(word, g_device_error, sizeof(*word));
+    const unsigned long long zero = 0;
+    if (e == cudaSuccess && clear && *word != 0) e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
+    return e;
+}
+}  // namespace vk
 
 // ------------------------------------------------------------------------------------------
 // Quantization
@@ -271,6 +387,29 @@ static int launch_simt(const LA& la, const LB& lb, const F8Output& out, int64_t 
     return launched();
 }
 
+template <int OUT>
+static int launch_gemm(const F8GemmParams& p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, cudaStream_t stream)
+{
+    int most = 0;
+    const int rc = prepare_kernel(gemm_fp8_kernel<OUT>, OUT, kF8SmemBytes, kF8Threads, 2, &most);
+    if (rc != VK_OK) return rc;
+    const int tiles = p.tiles_m * p.tiles_n;
+    return launch_clusters(gemm_fp8_kernel<OUT>, tiles < most ? tiles : most, 2, kF8Threads, kF8SmemBytes, stream, ta, tb, tc, p);
+}
+
+// Scales as the tensor-core kernels read them: strides per output index (or tile) and per k-block.
+static ScaleSource scales(const void* p, long long ld, int64_t count, int scaling, bool along_row)
+{
+    ScaleSource s;
+    s.p = static_cast<const uint8_t*>(p);
+    s.si = along_row ? ld : 1;
+    s.st = along_row ? 1 : ld;
+    s.count = static_cast<int>(count);
+    s.tile = scaling == VK_FP8_TILE;
+    s.words = along_row && rows_at(p, ld, 1, 4);
+    return s;
+}
+
 extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
 {
     static const char* const name = "vk_gemm_fp8";
@@ -300,6 +439,35 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: A, B, a_scale or b_scale is NULL", name);
     rc = use_device();
     if (rc != VK_OK) return rc;
+    const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+    if (a->k > 0 && tma_ok(a->A, lda, 1) && tma_ok(a->B, ldb, 1)) {
+        const int64_t tiles = (a->m + 255) / 256 * ((a->n + 255) / 256);
+        if (tiles > kMaxDim) return set_error(VK_ERR_UNSUPPORTED, "%s: too many tiles", name);
+        F8GemmParams p;
+        p.M = static_cast<int>(a->m);
+        p.N = static_cast<int>(a->n);
+        p.K = static_cast<int>(a->k);
+        p.tiles_m = static_cast<int>((a->m + 255) / 256);
+        p.tiles_n = static_cast<int>((a->n + 255) / 256);
+        p.num_st = static_cast<int>((a->k + 255) / 256);
+        p.raster_group = 8;
+        p.sa = scales(a->a_scale, ldas, a->m, a->a_scaling, true);
+        p.sb = scales(a->b_scale, ldbs, a->n, a->b_scaling, a->trans_b);
+        p.b_k = a->trans_b;
+        p.C = a->C;
+        p.ldc = ldc;
+        p.timeout_ns = wait_timeout_ns();
+        CUtensorMap ta, tb, tc;
+        rc = make_map(&ta, a->A, a->m, a->k, lda, 1, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc == VK_OK)
+            rc = a->trans_b ? make_map(&tb, a->B, a->n, a->k, ldb, 1, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)
+                            : make_map(&tb, a->B, a->k, a->n, ldb, 1, 128, 256, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc == VK_OK) rc = make_out_map(&tc, a->C, a->m, a->n, ldc, a->dtype, &p.c_tma);
+        if (rc != VK_OK) return rc;
+        return a->dtype == VK_DTYPE_F16   ? launch_gemm<VK_DTYPE_F16>(p, ta, tb, tc, stream)
+               : a->dtype == VK_DTYPE_F32 ? launch_gemm<VK_DTYPE_F32>(p, ta, tb, tc, stream)
+                                          : launch_gemm<VK_DTYPE_BF16>(p, ta, tb, tc, stream);
+    }
     const int tile_a = a->a_scaling == VK_FP8_TILE ? 7 : 0, tile_b = a->b_scaling == VK_FP8_TILE ? 7 : 0;
     const F8Operand fa{static_cast<const uint8_t*>(a->A), static_cast<const uint8_t*>(a->a_scale), lda, 1, ldas, 1, tile_a, 7};
     F8Operand fb{static_cast<const uint8_t*>(a->B), static_cast<const uint8_t*>(a->b_scale), ldb, 1, ldbs, 1, tile_b, 7};
@@ -310,7 +478,7 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
         fb.st = ldbs;
     }
     const F8Output out{a->C, ldc, a->dtype, 0};
-    return launch_simt(fa, fb, out, a->m, a->n, a->k, static_cast<cudaStream_t>(a->stream));
+    return launch_simt(fa, fb, out, a->m, a->n, a->k, stream);
 }
 
 extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)

@@ -11,8 +11,8 @@ namespace vk {
 // ------------------------------------------------------------------------------------------
 // Device error word.  Any bounded wait that gives up records (code << 32 | detail) here with
 // atomicCAS (the first error wins) and the kernel unwinds; the host reads it back through
-// vk_device_error().  Defined here because exactly one translation unit (vkgemm.cu) holds all
-// device code of the library.
+// vk_device_error().  Each translation unit with device code (vkgemm.cu, fp8.cu) has a word of its
+// own, and vk_device_error() reads them all.
 // ------------------------------------------------------------------------------------------
 __device__ unsigned long long g_device_error = 0ull;
 

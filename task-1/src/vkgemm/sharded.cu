@@ -438,5 +438,6 @@ extern "C" int vk_shutdown(void)
     cudaSetDevice(prev);
     vk::release_device_state();
     vk::release_host_pipes();
+    vk::release_fp8_state();
     return VK_OK;
 }

@@ -3,6 +3,8 @@
 
 #include <cstddef>
 
+#include <cuda_runtime.h>
+
 namespace vk {
 // Most peer C buffers one launch of the fused all-gather (vk_gemm_peers) stores into: an 8-GPU node.
 constexpr int kMaxPeers = 7;
@@ -12,6 +14,11 @@ int set_error(int code, const char* fmt, ...);
 struct DeviceState;
 // The current device, initialised (and refused when it is no sm_100 device).  st_out may be NULL.
 int current_device(int* dev_out, DeviceState** st_out);
+// Limit of the kernels' bounded waits, nanoseconds (option "wait_timeout_ns").
+unsigned long long wait_timeout_ns();
+// The 8-bit kernels' part of vk_shutdown and of vk_device_error (current device).
+void release_fp8_state();
+cudaError_t fp8_error_word(unsigned long long* word, bool clear);
 // Frees per-device scratch owned by the library (vk_shutdown).
 void release_device_state();
 // Frees the host-buffer pipeline's staging buffers and streams (vk_shutdown).

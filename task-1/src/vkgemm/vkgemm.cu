@@ -160,6 +160,8 @@ long long gather_timeout_ms() { return g_gather_timeout_ms.load(std::memory_orde
 static std::atomic<int> g_sgemm_attr_mask[3] = {{0}, {0}, {0}};
 static std::atomic<int> g_trace_on{0};
 
+unsigned long long wait_timeout_ns() { return g_timeout_ns.load(std::memory_order_relaxed); }
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1246,6 +1248,9 @@ extern "C" int vk_device_error(int device, uint64_t* out_word, int clear)
                 e = cudaMemset(st.scratch[i].counters, 0, st.ctr_bytes);
         }
     }
+    unsigned long long w8 = 0;
+    if (e == cudaSuccess) e = fp8_error_word(&w8, clear != 0);
+    if (w == 0) w = w8;
     cudaSetDevice(prev);
     if (e != cudaSuccess) return cuda_fail(e, "vk_device_error");
     *out_word = w;
