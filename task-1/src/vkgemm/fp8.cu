@@ -12,6 +12,7 @@
 #include "fp8_gemm.cuh"
 #include "fp8_rows.cuh"
 #include "fp8_simt.cuh"
+#include "fp8_wgrad.cuh"
 #include "vk_internal.h"
 
 using namespace vk;
@@ -481,6 +482,26 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     return launch_simt(fa, fb, out, a->m, a->n, a->k, stream);
 }
 
+// Pairs of CTAs per tile: as many as fill the GPU when the tiles alone do not, each with at least eight stages.
+static int wgrad_slices(int64_t tiles, int num_st)
+{
+    for (int s = 4; s > 1; --s)
+        if (tiles * s <= 74 && num_st >= 8 * s) return s;
+    return 1;
+}
+
+template <typename T, int OUT>
+static int launch_wgrad(WgradParams p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, cudaStream_t stream)
+{
+    constexpr int kId = 3 + 3 * (std::is_same_v<T, __half> ? 0 : 1) + OUT;
+    int most = 0;
+    const int rc = prepare_kernel(wgrad_fp8_kernel<T, OUT>, kId, kWgSmemBytes, kWgThreads, 2, &most);
+    if (rc != VK_OK) return rc;
+    const int tiles = p.tiles_m * p.tiles_n;
+    const int clusters = p.slices > 1 || tiles < most ? tiles : most;
+    return launch_clusters(wgrad_fp8_kernel<T, OUT>, clusters, 2 * p.slices, kWgThreads, kWgSmemBytes, stream, ta, tb, tc, p);
+}
+
 extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
 {
     static const char* const name = "vk_wgrad_fp8";
@@ -506,6 +527,37 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
     rc = use_device();
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
+    if (a->tokens > 0 && tma_ok(a->dY, lddy, 2) && tma_ok(a->X, ldx, 1)) {
+        const int64_t tiles = (a->n + 255) / 256 * ((a->k + 255) / 256);
+        if (tiles > kMaxDim) return set_error(VK_ERR_UNSUPPORTED, "%s: too many tiles", name);
+        WgradParams p;
+        p.M = static_cast<int>(a->n);
+        p.N = static_cast<int>(a->k);
+        p.K = static_cast<int>(a->tokens);
+        p.tiles_m = static_cast<int>((a->n + 255) / 256);
+        p.tiles_n = static_cast<int>((a->k + 255) / 256);
+        p.num_st = static_cast<int>((a->tokens + kWgBK - 1) / kWgBK);
+        p.raster_group = 8;
+        p.slices = wgrad_slices(tiles, p.num_st);
+        p.scale = static_cast<const uint8_t*>(a->x_scale);
+        p.lds = ldxs;
+        p.C = a->dW;
+        p.ldc = lddw;
+        p.accumulate = a->accumulate;
+        p.timeout_ns = wait_timeout_ns();
+        CUtensorMap ta, tb, tc;
+        rc = make_map(&ta, a->dY, a->tokens, a->n, lddy, 2, 64, kWgBK, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (rc == VK_OK) rc = make_map(&tb, a->X, a->tokens, a->k, ldx, 1, 128, kWgBK, CU_TENSOR_MAP_SWIZZLE_NONE);
+        if (rc == VK_OK) rc = make_out_map(&tc, a->dW, a->n, a->k, lddw, a->out_dtype, &p.c_tma);
+        if (rc != VK_OK) return rc;
+        p.c_vec = p.c_tma;
+        return for_type(a->dtype, [&](auto t) {
+            using T = std::conditional_t<std::is_same_v<decltype(t), __half>, __half, __nv_bfloat16>;
+            return a->out_dtype == VK_DTYPE_F16   ? launch_wgrad<T, VK_DTYPE_F16>(p, ta, tb, tc, stream)
+                   : a->out_dtype == VK_DTYPE_F32 ? launch_wgrad<T, VK_DTYPE_F32>(p, ta, tb, tc, stream)
+                                                  : launch_wgrad<T, VK_DTYPE_BF16>(p, ta, tb, tc, stream);
+        });
+    }
     const F8Operand fx{static_cast<const uint8_t*>(a->X), static_cast<const uint8_t*>(a->x_scale), 1, ldx, 1, ldxs, 7, 0};
     const F8Output out{a->dW, lddw, a->out_dtype, a->accumulate};
     if (a->dtype == VK_DTYPE_F16) {
