@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
                 dst[64] = b1;
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(mapa_shared(sf_full_bar(slot), 0));
+                if (lane == 0) mbar_arrive_pair(mapa_shared(sf_full_bar(slot), 0));
                 if (++slot == kF8SfSlots) {
                     slot = 0;
                     phase ^= 1u;
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
                 if (j == 0) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar, 0));
+                    if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar, 0));
                 }
                 const int col = tn * 256 + c;
                 if (col >= p.N) continue;

@@ -6,11 +6,11 @@
 // its way from TMA to the MMAs, inside shared memory: q * 2^e is exact in bf16, and the product is that of the 16-bit
 // kernel.  X costs half the bytes of a 16-bit checkpoint in memory and on the way into the SM.
 //
-// Roles (320 threads per CTA, pairs of CTAs on one 256 x 256 tile, 64 tokens a stage):
+// Roles (448 threads per CTA, pairs of CTAs on one 256 x 256 tile, 64 tokens a stage):
 //   warp 0      TMA loads: dY (128 of the tile's rows, M-major) and X's bytes (this CTA's 128 columns).
 //   warp 1      tensor memory, and in the pair's leader the MMAs (one lane).
 //   warps 2..5  epilogue: tensor memory -> registers -> swizzled staging -> TMA stores.
-//   warps 6..9  X's bytes -> 16-bit values in the 128-byte swizzled layout of an N-major operand.
+//   warps 6..13 X's bytes -> 16-bit values in the 128-byte swizzled layout of an N-major operand; four warps to a stage.
 //
 // A tile's tokens can be split over the pairs of a larger cluster (p.slices): each pair sums its share, leaves it in its
 // own shared memory, and adds its part of the columns from all of them in slice order.
@@ -41,7 +41,8 @@ constexpr int kWgBBytes = 128 * kWgBK * 2;
 constexpr int kWgStageBytes = kWgABytes + kWgRawBytes + kWgBBytes;
 constexpr int kWgBars = 4 * kWgStages + 4;
 constexpr int kWgSmemBytes = 1024 + kWgStages * kWgStageBytes + 4 * kF8EpiWarpBytes + kWgBars * 8 + 16;
-constexpr int kWgThreads = 320;
+constexpr int kWgGroups = 2;  // of four conversion warps, taking turns at the stages
+constexpr int kWgThreads = 192 + 128 * kWgGroups;
 static_assert(kWgSmemBytes <= 232448, "shared memory per CTA");
 static_assert(kWgStages * kWgStageBytes >= 128 * 256 * 4, "a slice's partial sums fit the stages");
 
@@ -229,8 +230,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     } else if (warp >= 6) {
         // Lanes 8g .. 8g+7 hold the 16-byte chunks c of two rows, 0..3 of one and 4..7 of the next: the reads cover all
         // banks once, and so do the writes (chunks 2(c%4), 2(c%4)+1 of 64-column atom c/4, xor row % 8).
-        const int w = warp - 6, c = lane & 7, g = (lane >> 3) ^ (c >> 2);
-        int stage = 0;
+        const int w = warp & 3, group = (warp - 6) >> 2, c = lane & 7, g = (lane >> 3) ^ (c >> 2);
+        int stage = 0, count = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int t = cluster_id; ok && t < tiles; t += num_clusters) {
@@ -242,33 +243,40 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 const int row = st * kWgBK + w * 16 + (lane & 15);
                 return in && row < p.K ? static_cast<uint32_t>(p.scale[row * p.lds + blk]) : 127u;
             };
-            uint32_t next = scale_of(st0);
-            for (int st = st0; st < st1; ++st) {
-                const float mine = e8m0_scale(next);
-                if (st + 1 < st1) next = scale_of(st + 1);
-                if (!mbar_wait(x_bar(stage), phase, p.timeout_ns, kErrWaitMma, 300 + stage)) {
-                    ok = false;
-                    break;
-                }
-                const uint8_t* src = sX + stage * kWgRawBytes;
-                uint8_t* dst = sB + stage * kWgBBytes + (c >> 2) * (kWgBK * 128);
+            // this group's stages of the tile
+            const int first = st0 + (group - count % kWgGroups + kWgGroups) % kWgGroups;
+            uint32_t next = scale_of(first), after = scale_of(first + kWgGroups);
+            for (int st = st0; st < st1; ++st, ++count) {
+                if (count % kWgGroups == group) {
+                    const float mine = e8m0_scale(next);
+                    if (!mbar_wait(x_bar(stage), phase, p.timeout_ns, kErrWaitMma, 300 + stage)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint8_t* src = sX + stage * kWgRawBytes;
+                    uint8_t* dst = sB + stage * kWgBBytes + (c >> 2) * (kWgBK * 128);
+                    uint4 v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = w * 16 + 4 * i + g;
-                    const uint4 v = *reinterpret_cast<const uint4*>(src + row * 128 + c * 16);
-                    const float s = __shfl_sync(0xffffffffu, mine, 4 * i + g);
-                    const uint4 lo = make_uint4(scaled_pair<T>(v.x & 0xffffu, s), scaled_pair<T>(v.x >> 16, s),
-                                                scaled_pair<T>(v.y & 0xffffu, s), scaled_pair<T>(v.y >> 16, s));
-                    const uint4 hi = make_uint4(scaled_pair<T>(v.z & 0xffffu, s), scaled_pair<T>(v.z >> 16, s),
-                                                scaled_pair<T>(v.w & 0xffffu, s), scaled_pair<T>(v.w >> 16, s));
-                    uint4* out = reinterpret_cast<uint4*>(dst + row * 128);
-                    const int first = (c & 3) * 2;
-                    out[first ^ (row & 7)] = lo;
-                    out[(first + 1) ^ (row & 7)] = hi;
+                    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(src + (w * 16 + 4 * i + g) * 128 + c * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = w * 16 + 4 * i + g;
+                        const float s = __shfl_sync(0xffffffffu, mine, 4 * i + g);
+                        const uint4 lo = make_uint4(scaled_pair<T>(v[i].x & 0xffffu, s), scaled_pair<T>(v[i].x >> 16, s),
+                                                    scaled_pair<T>(v[i].y & 0xffffu, s), scaled_pair<T>(v[i].y >> 16, s));
+                        const uint4 hi = make_uint4(scaled_pair<T>(v[i].z & 0xffffu, s), scaled_pair<T>(v[i].z >> 16, s),
+                                                    scaled_pair<T>(v[i].w & 0xffffu, s), scaled_pair<T>(v[i].w >> 16, s));
+                        uint4* out = reinterpret_cast<uint4*>(dst + row * 128);
+                        const int chunk = (c & 3) * 2;
+                        out[chunk ^ (row & 7)] = lo;
+                        out[(chunk + 1) ^ (row & 7)] = hi;
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_pair(mapa_shared(ready_bar(stage), lead));
+                    next = after;
+                    after = scale_of(st + 2 * kWgGroups);
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(mapa_shared(ready_bar(stage), lead));
                 if (++stage == kWgStages) {
                     stage = 0;
                     phase ^= 1u;
@@ -315,7 +323,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_shared(tempty_bar(acc), lead));
+            if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar(acc), lead));
         }
     }
     if (p.slices > 1) {

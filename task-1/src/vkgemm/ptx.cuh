@@ -122,6 +122,14 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar)
                  : "memory");
 }
 
+// The same for what this thread ordered by itself: data written in this CTA's own shared memory and handed to the async
+// proxy with fence_proxy_async_smem().  Without the cluster scope the arrive waits for no memory traffic of the thread
+// (with it, a load in flight to global memory holds the arrive back).
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_bar)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
 {
     uint32_t ok;
