@@ -118,38 +118,102 @@ int make_out_map(CUtensorMap* map, void* c, int64_t m, int64_t n, long long ldc,
     memset(map, 0, sizeof(*map));
     *c_tma = tma_ok(c, ldc, esize);
     if (!*c_tma) return VK_OK;
-    return make_map(map, c, m, n, ldc, esize, 32, 32, esize == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    return make_map(map, c, m, n, ldc, esize, 64 / esize, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// Clusters of each kernel that fit on each device (0: not asked yet; its shared-memory attribute is set by then).
+// Clusters of 1 to 4 pairs of each kernel that fit on each device (0: not asked yet; the kernel's shared-memory attribute
+// is set by then).
 constexpr int kKernels = 16, kDevices = 64;
-std::atomic<int> g_clusters[kKernels][kDevices];
+std::atomic<int> g_clusters[kKernels][kDevices][4];
 
 template <typename Kernel>
-int prepare_kernel(Kernel fn, int id, int smem, int threads, int cluster, int* clusters)
+int prepare_kernel(Kernel fn, int id, int smem, int threads, int clusters[4])
 {
     int dev = 0;
     F8_CUDA_TRY(cudaGetDevice(&dev));
-    std::atomic<int>& known = g_clusters[id][dev];
-    *clusters = known.load(std::memory_order_acquire);
-    if (*clusters > 0) return VK_OK;
-    F8_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    int sms = 0;
-    F8_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(sms / cluster * cluster);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    F8_CUDA_TRY(cudaOccupancyMaxActiveClusters(clusters, fn, &cfg));
-    if (*clusters <= 0) return set_error(VK_ERR_CUDA, "kernel cannot be resident (%d bytes of shared memory)", smem);
-    known.store(*clusters, std::memory_order_release);
+    std::atomic<int>* known = g_clusters[id][dev];
+    if (known[0].load(std::memory_order_acquire) == 0) {
+        F8_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        int sms = 0;
+        F8_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        for (int pairs = 4; pairs >= 1; --pairs) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 2 * pairs;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3(2 * pairs * sms);
+            cfg.blockDim = dim3(threads);
+            cfg.dynamicSmemBytes = smem;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            F8_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, fn, &cfg));
+            if (n <= 0 && pairs == 1) return set_error(VK_ERR_CUDA, "kernel cannot be resident (%d bytes of shared memory)", smem);
+            known[pairs - 1].store(n, std::memory_order_release);
+        }
+    }
+    for (int i = 0; i < 4; ++i) clusters[i] = known[i].load(std::memory_order_acquire);
     return VK_OK;
+}
+
+// Workspace of a product whose last tiles are cut into slices: counters, then fp32 sums of at most one slice per pair.
+constexpr int kMaxPairs = 74;
+constexpr size_t kCounterBytes = 8192;
+constexpr size_t kSliceBytes = 2 * 128 * 256 * sizeof(float);
+
+int grains_of(const TileWork& w) { return (w.stages + w.grain - 1) / w.grain; }
+
+// Shares the tiles out.  Fewer tiles than clusters of several pairs: as many pairs to a tile as can all run at once.
+// Otherwise the tiles of a partial last wave are cut into up to 4 slices (more would have more sums to join than the whole
+// tiles after them hide), none shorter than `least` grains.
+void plan_work(TileWork& w, const int clusters[4], int least, void* workspace, int* launch)
+{
+    const long long tiles = static_cast<long long>(w.tiles_m) * w.tiles_n;
+    const int grains = grains_of(w), pairs = clusters[0] < kMaxPairs ? clusters[0] : kMaxPairs;
+    w.raster_group = 8;
+    w.pairs = w.split = 1;
+    w.tail = 0;
+    w.ws = nullptr;
+    w.counters = nullptr;
+    for (int s = 4; s >= 2; --s)
+        if (tiles <= clusters[s - 1] && grains >= s * least) {
+            w.pairs = s;
+            *launch = static_cast<int>(tiles);
+            return;
+        }
+    const long long rest = tiles % pairs;
+    if (workspace != nullptr && rest > 0) {
+        long long s = pairs / rest;
+        if (s > 4) s = 4;
+        if (s > grains / least) s = grains / least;
+        if (s >= 2) {
+            w.tail = static_cast<int>(rest);
+            w.split = static_cast<int>(s);
+            w.counters = static_cast<int*>(workspace);
+            w.ws = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+        }
+    }
+    const int units = work_units(w);
+    *launch = units < pairs ? units : pairs;
+}
+
+int clear_counters(const TileWork& w, cudaStream_t stream)
+{
+    if (w.tail > 0) F8_CUDA_TRY(cudaMemsetAsync(w.counters, 0, static_cast<size_t>(w.tail) * 16 * sizeof(int), stream));
+    return VK_OK;
+}
+
+int check_workspace(const char* name, const void* p, size_t bytes, size_t need)
+{
+    if (p != nullptr && (bytes < need || !aligned(p, 16)))
+        return set_error(VK_ERR_INVALID_ARGUMENT, "%s: a workspace has %zu bytes and is 16-byte aligned (%s_workspace), or is NULL", name, need, name);
+    return VK_OK;
+}
+
+size_t product_workspace(int64_t m, int64_t n, int64_t k)
+{
+    return m > 0 && n > 0 && k > 0 ? kCounterBytes + kMaxPairs * kSliceBytes : 0;
 }
 
 template <typename Kernel, typename... Args>
@@ -176,7 +240,7 @@ namespace vk {
 void release_fp8_state()
 {
     for (auto& kernel : g_clusters)
-        for (auto& device : kernel) device.store(0, std::memory_order_release);
+        for (auto& device : kernel) device[0].store(0, std::memory_order_release);
 }
 
 cudaError_t fp8_error_word(unsigned long long* word, bool clear)
@@ -388,14 +452,38 @@ static int launch_simt(const LA& la, const LB& lb, const F8Output& out, int64_t 
     return launched();
 }
 
-template <int OUT>
-static int launch_gemm(const F8GemmParams& p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, cudaStream_t stream)
+extern "C" int vk_gemm_fp8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes)
 {
-    int most = 0;
-    const int rc = prepare_kernel(gemm_fp8_kernel<OUT>, OUT, kF8SmemBytes, kF8Threads, 2, &most);
+    static const char* const name = "vk_gemm_fp8_workspace";
+    if (bytes == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: bytes is NULL", name);
+    if (m < 0 || m > kMaxDim) return bad_size(name, "m", m);
+    if (n < 0 || n > kMaxDim) return bad_size(name, "n", n);
+    if (k < 0 || k > kMaxDim) return bad_size(name, "k", k);
+    *bytes = product_workspace(m, n, k);
+    return VK_OK;
+}
+
+extern "C" int vk_wgrad_fp8_workspace(int64_t tokens, int64_t n, int64_t k, size_t* bytes)
+{
+    static const char* const name = "vk_wgrad_fp8_workspace";
+    if (bytes == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: bytes is NULL", name);
+    if (tokens < 0 || tokens > kMaxDim) return bad_size(name, "tokens", tokens);
+    if (n < 0 || n > kMaxDim) return bad_size(name, "n", n);
+    if (k < 0 || k > kMaxDim) return bad_size(name, "k", k);
+    *bytes = product_workspace(n, k, tokens);
+    return VK_OK;
+}
+
+template <int OUT>
+static int launch_gemm(F8GemmParams p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, void* workspace, cudaStream_t stream)
+{
+    int fit[4], clusters = 0;
+    int rc = prepare_kernel(gemm_fp8_kernel<OUT>, OUT, kF8SmemBytes, kF8Threads, fit);
     if (rc != VK_OK) return rc;
-    const int tiles = p.tiles_m * p.tiles_n;
-    return launch_clusters(gemm_fp8_kernel<OUT>, tiles < most ? tiles : most, 2, kF8Threads, kF8SmemBytes, stream, ta, tb, tc, p);
+    plan_work(p.work, fit, 2, workspace, &clusters);
+    rc = clear_counters(p.work, stream);
+    if (rc != VK_OK) return rc;
+    return launch_clusters(gemm_fp8_kernel<OUT>, clusters, 2 * p.work.pairs, kF8Threads, kF8SmemBytes, stream, ta, tb, tc, p);
 }
 
 // Scales as the tensor-core kernels read them: strides per output index (or tile) and per k-block.
@@ -434,6 +522,8 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     if (rc == VK_OK) rc = ld_of(name, "ld_a_scale", a->ld_a_scale, kb, &ldas);
     if (rc == VK_OK) rc = ld_of(name, "ld_b_scale", a->ld_b_scale, (b_row + 127) / 128, &ldbs);
     if (rc != VK_OK) return rc;
+    rc = check_workspace(name, a->workspace, a->workspace_bytes, product_workspace(a->m, a->n, a->k));
+    if (rc != VK_OK) return rc;
     if (a->m == 0 || a->n == 0) return VK_OK;
     if (a->C == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: C is NULL", name);
     if (a->k > 0 && (a->A == nullptr || a->B == nullptr || a->a_scale == nullptr || a->b_scale == nullptr))
@@ -448,10 +538,10 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
         p.M = static_cast<int>(a->m);
         p.N = static_cast<int>(a->n);
         p.K = static_cast<int>(a->k);
-        p.tiles_m = static_cast<int>((a->m + 255) / 256);
-        p.tiles_n = static_cast<int>((a->n + 255) / 256);
-        p.num_st = static_cast<int>((a->k + 255) / 256);
-        p.raster_group = 8;
+        p.work.tiles_m = static_cast<int>((a->m + 255) / 256);
+        p.work.tiles_n = static_cast<int>((a->n + 255) / 256);
+        p.work.stages = static_cast<int>((a->k + 255) / 256);
+        p.work.grain = 2;  // a slice begins with a whole set of scales
         p.sa = scales(a->a_scale, ldas, a->m, a->a_scaling, true);
         p.sb = scales(a->b_scale, ldbs, a->n, a->b_scaling, a->trans_b);
         p.b_k = a->trans_b;
@@ -465,9 +555,9 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
                             : make_map(&tb, a->B, a->k, a->n, ldb, 1, 128, 256, CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc == VK_OK) rc = make_out_map(&tc, a->C, a->m, a->n, ldc, a->dtype, &p.c_tma);
         if (rc != VK_OK) return rc;
-        return a->dtype == VK_DTYPE_F16   ? launch_gemm<VK_DTYPE_F16>(p, ta, tb, tc, stream)
-               : a->dtype == VK_DTYPE_F32 ? launch_gemm<VK_DTYPE_F32>(p, ta, tb, tc, stream)
-                                          : launch_gemm<VK_DTYPE_BF16>(p, ta, tb, tc, stream);
+        return a->dtype == VK_DTYPE_F16   ? launch_gemm<VK_DTYPE_F16>(p, ta, tb, tc, a->workspace, stream)
+               : a->dtype == VK_DTYPE_F32 ? launch_gemm<VK_DTYPE_F32>(p, ta, tb, tc, a->workspace, stream)
+                                          : launch_gemm<VK_DTYPE_BF16>(p, ta, tb, tc, a->workspace, stream);
     }
     const int tile_a = a->a_scaling == VK_FP8_TILE ? 7 : 0, tile_b = a->b_scaling == VK_FP8_TILE ? 7 : 0;
     const F8Operand fa{static_cast<const uint8_t*>(a->A), static_cast<const uint8_t*>(a->a_scale), lda, 1, ldas, 1, tile_a, 7};
@@ -482,24 +572,17 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     return launch_simt(fa, fb, out, a->m, a->n, a->k, stream);
 }
 
-// Pairs of CTAs per tile: as many as fill the GPU when the tiles alone do not, each with at least eight stages.
-static int wgrad_slices(int64_t tiles, int num_st)
-{
-    for (int s = 4; s > 1; --s)
-        if (tiles * s <= 74 && num_st >= 8 * s) return s;
-    return 1;
-}
-
 template <typename T, int OUT>
-static int launch_wgrad(WgradParams p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, cudaStream_t stream)
+static int launch_wgrad(WgradParams p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, void* workspace, cudaStream_t stream)
 {
     constexpr int kId = 3 + 3 * (std::is_same_v<T, __half> ? 0 : 1) + OUT;
-    int most = 0;
-    const int rc = prepare_kernel(wgrad_fp8_kernel<T, OUT>, kId, kWgSmemBytes, kWgThreads, 2, &most);
+    int fit[4], clusters = 0;
+    int rc = prepare_kernel(wgrad_fp8_kernel<T, OUT>, kId, kWgSmemBytes, kWgThreads, fit);
     if (rc != VK_OK) return rc;
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int clusters = p.slices > 1 || tiles < most ? tiles : most;
-    return launch_clusters(wgrad_fp8_kernel<T, OUT>, clusters, 2 * p.slices, kWgThreads, kWgSmemBytes, stream, ta, tb, tc, p);
+    plan_work(p.work, fit, 4, workspace, &clusters);
+    rc = clear_counters(p.work, stream);
+    if (rc != VK_OK) return rc;
+    return launch_clusters(wgrad_fp8_kernel<T, OUT>, clusters, 2 * p.work.pairs, kWgThreads, kWgSmemBytes, stream, ta, tb, tc, p);
 }
 
 extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
@@ -520,6 +603,8 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
     if (rc == VK_OK) rc = ld_of(name, "ld_x_scale", a->ld_x_scale, (a->k + 127) / 128, &ldxs);
     if (rc == VK_OK) rc = ld_of(name, "lddw", a->lddw, a->k, &lddw);
     if (rc != VK_OK) return rc;
+    rc = check_workspace(name, a->workspace, a->workspace_bytes, product_workspace(a->n, a->k, a->tokens));
+    if (rc != VK_OK) return rc;
     if (a->n == 0 || a->k == 0) return VK_OK;
     if (a->dW == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: dW is NULL", name);
     if (a->tokens > 0 && (a->dY == nullptr || a->X == nullptr || a->x_scale == nullptr))
@@ -534,11 +619,10 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
         p.M = static_cast<int>(a->n);
         p.N = static_cast<int>(a->k);
         p.K = static_cast<int>(a->tokens);
-        p.tiles_m = static_cast<int>((a->n + 255) / 256);
-        p.tiles_n = static_cast<int>((a->k + 255) / 256);
-        p.num_st = static_cast<int>((a->tokens + kWgBK - 1) / kWgBK);
-        p.raster_group = 8;
-        p.slices = wgrad_slices(tiles, p.num_st);
+        p.work.tiles_m = static_cast<int>((a->n + 255) / 256);
+        p.work.tiles_n = static_cast<int>((a->k + 255) / 256);
+        p.work.stages = static_cast<int>((a->tokens + kWgBK - 1) / kWgBK);
+        p.work.grain = 1;
         p.scale = static_cast<const uint8_t*>(a->x_scale);
         p.lds = ldxs;
         p.C = a->dW;
@@ -547,15 +631,14 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
         p.timeout_ns = wait_timeout_ns();
         CUtensorMap ta, tb, tc;
         rc = make_map(&ta, a->dY, a->tokens, a->n, lddy, 2, 64, kWgBK, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc == VK_OK) rc = make_map(&tb, a->X, a->tokens, a->k, ldx, 1, 128, kWgBK, CU_TENSOR_MAP_SWIZZLE_NONE);
+        if (rc == VK_OK) rc = make_map(&tb, a->X, a->tokens, a->k, ldx, 1, 128, kWgXK, CU_TENSOR_MAP_SWIZZLE_NONE);
         if (rc == VK_OK) rc = make_out_map(&tc, a->dW, a->n, a->k, lddw, a->out_dtype, &p.c_tma);
         if (rc != VK_OK) return rc;
-        p.c_vec = p.c_tma;
         return for_type(a->dtype, [&](auto t) {
             using T = std::conditional_t<std::is_same_v<decltype(t), __half>, __half, __nv_bfloat16>;
-            return a->out_dtype == VK_DTYPE_F16   ? launch_wgrad<T, VK_DTYPE_F16>(p, ta, tb, tc, stream)
-                   : a->out_dtype == VK_DTYPE_F32 ? launch_wgrad<T, VK_DTYPE_F32>(p, ta, tb, tc, stream)
-                                                  : launch_wgrad<T, VK_DTYPE_BF16>(p, ta, tb, tc, stream);
+            return a->out_dtype == VK_DTYPE_F16   ? launch_wgrad<T, VK_DTYPE_F16>(p, ta, tb, tc, a->workspace, stream)
+                   : a->out_dtype == VK_DTYPE_F32 ? launch_wgrad<T, VK_DTYPE_F32>(p, ta, tb, tc, a->workspace, stream)
+                                                  : launch_wgrad<T, VK_DTYPE_BF16>(p, ta, tb, tc, a->workspace, stream);
         });
     }
     const F8Operand fx{static_cast<const uint8_t*>(a->X), static_cast<const uint8_t*>(a->x_scale), 1, ldx, 1, ldxs, 7, 0};

@@ -16,6 +16,13 @@
 // accumulator begins at column 224: the two share 32 columns, which the epilogue reads first; the next tile's MMAs start
 // once it has.  Columns 480..511 hold two sets of scales (4 columns for A's 128 rows, 8 for B's 256), each for 512 of k.
 //
+// How tiles are handed out (TileWork): pairs walk over whole tiles.  The tiles of a partial last wave are cut along k into
+// slices, numbered first, so that joining them overlaps the whole tiles that follow: each (slice, CTA, epilogue warp)
+// counts its arrival; all but the last to arrive write their fp32 sums to the workspace and count that too, and the last
+// adds all slices' sums in slice order, whoever it is, so a result never depends on timing.  It waits (bounded) only for
+// CTAs that have arrived.  When there are fewer tiles than pairs, a cluster of 2 to 4 pairs shares one tile instead: each
+// pair sums its share of k, leaves it in its own shared memory, and adds its part of the columns from all of them.
+//
 // Scales in shared memory and tensor memory: row r's word (4 k-blocks) of a unit of 128 rows sits at byte
 // (r % 32) * 16 + (r / 32) * 4; tcgen05.cp.32x128b.warpx4 makes that lane r % 32, column r / 32, in all four lane quarters.
 #pragma once
@@ -47,10 +54,58 @@ struct ScaleSource {
     }
 };
 
+// How the 256 x 256 tiles of an output are shared out over clusters.
+struct TileWork {
+    int tiles_m, tiles_n, raster_group;
+    int stages;          // k-stages of a tile
+    int grain;           // stages that a slice's boundaries are multiples of
+    int pairs;           // pairs of CTAs that share each tile through their cluster's shared memory (1: none)
+    int tail, split;     // the last `tail` tiles are cut into `split` slices each, joined through the workspace
+    float* ws;           // [tail tile][slice][CTA of the pair][epilogue warp][32 rows x 256 columns] fp32
+    int* counters;       // [tail tile][CTA of the pair][epilogue warp][arrived, written], zero at the launch
+};
+
+// A pair's next piece of work: stages [st0, st1) of a tile.
+struct Work {
+    int tm, tn, st0, st1;
+    int slice;           // of a tail tile, -1 for a whole one
+    int index;           // of the tail tile
+};
+
+__host__ __device__ __forceinline__ int work_units(const TileWork& w)
+{
+    return w.tiles_m * w.tiles_n + w.tail * (w.split - 1);
+}
+
+// Unit u; `part`: which of w.pairs this pair is.
+__host__ __device__ __forceinline__ Work work_unit(const TileWork& w, int u, int part)
+{
+    Work r;
+    int t = u - w.tail * w.split, cut = w.pairs, piece = part;
+    r.slice = r.index = -1;
+    if (t < 0) {
+        r.index = u / w.split;
+        r.slice = piece = u - r.index * w.split;
+        cut = w.split;
+        t = w.tiles_m * w.tiles_n - w.tail + r.index;
+    }
+    const int grains = (w.stages + w.grain - 1) / w.grain;
+    r.st0 = static_cast<int>(static_cast<long long>(grains) * piece / cut) * w.grain;
+    r.st1 = static_cast<int>(static_cast<long long>(grains) * (piece + 1) / cut) * w.grain;
+    if (r.st1 > w.stages) r.st1 = w.stages;
+    const int per_group = w.raster_group * w.tiles_n;
+    const int g = t / per_group;
+    const int first_m = g * w.raster_group;
+    const int rows = w.tiles_m - first_m < w.raster_group ? w.tiles_m - first_m : w.raster_group;
+    const int in = t - g * per_group;
+    r.tm = first_m + in % rows;
+    r.tn = in / rows;
+    return r;
+}
+
 struct F8GemmParams {
     int M, N, K;
-    int tiles_m, tiles_n, num_st;  // 256-deep stages
-    int raster_group;
+    TileWork work;
     ScaleSource sa, sb;
     int b_k;                       // B stored n x k
     void* C;
@@ -65,7 +120,7 @@ constexpr int kF8BBytes = 128 * 256;
 constexpr int kF8StageBytes = kF8ABytes + kF8BBytes;
 constexpr int kF8SfSlots = 3;
 constexpr int kF8SfBytes = 512 + 1024;  // a slot: A's unit, B's two
-constexpr int kF8EpiWarpBytes = 4096;   // two 32 x 32 boxes of 16-bit results, or one of fp32
+constexpr int kF8EpiWarpBytes = 4096;   // two boxes of 32 rows x 64 bytes
 constexpr int kF8Bars = 2 * kF8Stages + 3 + 2 * kF8SfSlots;
 constexpr int kF8SmemBytes =
     1024 + kF8Stages * kF8StageBytes + 4 * kF8EpiWarpBytes + kF8SfSlots * kF8SfBytes + kF8Bars * 8 + 16;
@@ -107,17 +162,6 @@ __host__ __device__ constexpr uint32_t idesc_mxf8(int M, int N, bool b_n_major)
            (static_cast<uint32_t>(M >> 7) << 27);
 }
 
-__device__ __forceinline__ void f8_tile_coords(int t, int tiles_m, int tiles_n, int group, int& tm, int& tn)
-{
-    const int per_group = group * tiles_n;
-    const int g = t / per_group;
-    const int first_m = g * group;
-    const int gsz = min(tiles_m - first_m, group);
-    const int r = t - g * per_group;
-    tm = first_m + r % gsz;
-    tn = r / gsz;
-}
-
 template <int OUT>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi)
 {
@@ -130,56 +174,214 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi)
     }
 }
 
-// Where an epilogue warp's 32 x 32 boxes go.  OUT: vk_dtype of C.
+// Where an epilogue warp's results go.  OUT: vk_dtype of C.
 struct BoxOut {
-    const CUtensorMap* map;  // boxes of 32 x 32, 64-byte (16-bit) or 128-byte (fp32) swizzle
+    const CUtensorMap* map;  // boxes of 32 rows x 64 bytes, 64-byte swizzle
     void* C;
     long long ldc;
     int M, N;
-    int c_tma;
+    int c_tma;               // C can take TMA stores (and 16-byte accesses)
+    int accumulate;          // C += the results
 };
 
-// This lane's row (row0 + lane), columns col .. col + 31.  `turn` counts the boxes of this warp.
-template <int OUT>
-__device__ __forceinline__ void store_box(const BoxOut& o, uint8_t* stg, int row0, int lane, int col, const float (&f)[32], uint32_t& turn)
+// Results col .. col + 31 of this lane's row (row0 + lane).  BUFS boxes of staging take turns; `turn` counts them.
+template <int OUT, int BUFS>
+__device__ __forceinline__ void store_box(const BoxOut& o, uint8_t* stg, int row0, int lane, int col, float (&f)[32], uint32_t& turn)
 {
-    if (o.c_tma) {
-        if constexpr (OUT == 1) {
-            if (lane == 0) bulk_wait_group_read<0>();
-            __syncwarp();
-            uint4* row = reinterpret_cast<uint4*>(stg + lane * 128);
+    using T = std::conditional_t<OUT == 0, __half, std::conditional_t<OUT == 1, float, __nv_bfloat16>>;
+    const int row = row0 + lane;
+    T* c = static_cast<T*>(o.C) + static_cast<long long>(row) * o.ldc + col;
+    if (o.accumulate && row < o.M) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                row[j ^ (lane & 7)] = make_uint4(__float_as_uint(f[4 * j]), __float_as_uint(f[4 * j + 1]),
-                                                 __float_as_uint(f[4 * j + 2]), __float_as_uint(f[4 * j + 3]));
-        } else {
-            stg += (turn & 1u) * 2048;
-            if (lane == 0) bulk_wait_group_read<1>();
-            __syncwarp();
-            uint4* row = reinterpret_cast<uint4*>(stg + lane * 64);
+        for (int j = 0; j < 4; ++j) {
+            const int n = o.N - col - 8 * j;
+            const Vec8<T> v = load8(c + (n > 0 ? 8 * j : 0), n, o.c_tma);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                row[j ^ ((lane >> 1) & 3)] =
-                    make_uint4(pack16<OUT>(f[8 * j], f[8 * j + 1]), pack16<OUT>(f[8 * j + 2], f[8 * j + 3]),
-                               pack16<OUT>(f[8 * j + 4], f[8 * j + 5]), pack16<OUT>(f[8 * j + 6], f[8 * j + 7]));
+            for (int i = 0; i < 8; ++i) f[8 * j + i] += to_f32(v.v[i]);
         }
-        ++turn;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && row0 < o.M) {
-            tma_store_2d(o.map, smem_u32(stg), col, row0);
-            bulk_commit_group();
+    }
+    if (o.c_tma) {
+        constexpr int kCols = 64 / sizeof(T);  // of a box
+#pragma unroll
+        for (int h = 0; h < 32 / kCols; ++h) {
+            if (col + h * kCols >= o.N) break;
+            uint8_t* box = stg + (turn % BUFS) * 2048;
+            if (lane == 0) bulk_wait_group_read<BUFS - 1>();
+            __syncwarp();
+            uint4* to = reinterpret_cast<uint4*>(box + lane * 64);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint4 v;
+                if constexpr (OUT == 1) {
+                    const float* g = f + 16 * h + 4 * j;
+                    v = make_uint4(__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]), __float_as_uint(g[3]));
+                } else {
+                    v = make_uint4(pack16<OUT>(f[8 * j], f[8 * j + 1]), pack16<OUT>(f[8 * j + 2], f[8 * j + 3]),
+                                   pack16<OUT>(f[8 * j + 4], f[8 * j + 5]), pack16<OUT>(f[8 * j + 6], f[8 * j + 7]));
+                }
+                to[j ^ ((lane >> 1) & 3)] = v;  // the 64-byte swizzle
+            }
+            ++turn;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < o.M) {
+                tma_store_2d(o.map, smem_u32(box), col + h * kCols, row0);
+                bulk_commit_group();
+            }
         }
         return;
     }
-    const int row = row0 + lane;
     if (row >= o.M) return;
-    using T = std::conditional_t<OUT == 0, __half, std::conditional_t<OUT == 1, float, __nv_bfloat16>>;
-    T* c = static_cast<T*>(o.C) + static_cast<long long>(row) * o.ldc + col;
 #pragma unroll
     for (int i = 0; i < 32; ++i)
         if (col + i < o.N) c[i] = from_f32<T>(f[i]);
 }
+
+__device__ __forceinline__ void tmem_chunk(uint32_t addr, float (&f)[32])
+{
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(addr, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// An epilogue warp's way with one unit's accumulator: columns acc .. acc + 255 of its lane quarter, read in chunks of 32
+// beginning with chunk `first`; `early()` is called once that one has been read.  part: where a pair that shares its
+// tile leaves its sums (null otherwise).
+template <int OUT, int BUFS, typename Early>
+__device__ __forceinline__ void finish_unit(const TileWork& w, const Work& u, const BoxOut& out, uint8_t* stg, float4* part, uint32_t acc,
+                                            int first, int half, int q, int lane, uint32_t& turn, unsigned long long timeout_ns,
+                                            const Early& early)
+{
+    const int row0 = u.tm * 256 + half * 128 + q * 32;
+    const uint32_t base = acc + (static_cast<uint32_t>(q * 32) << 16);
+    float f[32];
+    if (u.slice < 0) {
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+            const int ch = (j + first) & 7;
+            tmem_chunk(base + static_cast<uint32_t>(ch * 32), f);
+            if (j == 0) early();
+            const int col = u.tn * 256 + ch * 32;
+            if (part != nullptr) {
+                float4* to = part + ch * 8 * 128 + q * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) to[i * 128] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+            } else if (col < out.N) {
+                store_box<OUT, BUFS>(out, stg, row0, lane, col, f, turn);
+            }
+        }
+        return;
+    }
+    constexpr long long kWarp = 32 * 256;
+    int* ctr = w.counters + ((u.index * 2 + half) * 4 + q) * 2;
+    auto sums_of = [&](int slice) {
+        return reinterpret_cast<float4*>(w.ws + ((static_cast<long long>(u.index * w.split + slice) * 2 + half) * 4 + q) * kWarp) + lane;
+    };
+    int arrived = 0;
+    if (lane == 0) arrived = atomicAdd(&ctr[0], 1);
+    arrived = __shfl_sync(0xffffffffu, arrived, 0);
+    if (arrived < w.split - 1) {
+        float4* mine = sums_of(u.slice);
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+            const int ch = (j + first) & 7;
+            tmem_chunk(base + static_cast<uint32_t>(ch * 32), f);
+            if (j == 0) early();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                __stcg(mine + (ch * 8 + i) * 32, make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]));
+        }
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) atomicAdd(&ctr[1], 1);
+        return;
+    }
+    float own[32];
+    tmem_chunk(base + static_cast<uint32_t>(first * 32), own);
+    early();
+    int ok = 1;
+    if (lane == 0) ok = wait_count_at_least(&ctr[1], w.split - 1, timeout_ns, kErrWaitEpilogue, 300 + q);
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    __threadfence();
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+        const int ch = (j + first) & 7;
+        if (j > 0) tmem_chunk(base + static_cast<uint32_t>(ch * 32), own);
+        const int col = u.tn * 256 + ch * 32;
+        if (!ok || col >= out.N) continue;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = 0.f;
+#pragma unroll 1
+        for (int s = 0; s < w.split; ++s) {
+            float4 v[8];
+            const float4* from = sums_of(s) + ch * 8 * 32;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = s == u.slice ? make_float4(own[4 * i], own[4 * i + 1], own[4 * i + 2], own[4 * i + 3]) : __ldcg(from + i * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f[4 * i] += v[i].x;
+                f[4 * i + 1] += v[i].y;
+                f[4 * i + 2] += v[i].z;
+                f[4 * i + 3] += v[i].w;
+            }
+        }
+        store_box<OUT, BUFS>(out, stg, row0, lane, col, f, turn);
+    }
+}
+
+// The columns of a shared tile that fall to pair `part`, added from all pairs' shared memory.
+template <int OUT, int BUFS>
+__device__ __forceinline__ void finish_shared(const TileWork& w, const Work& u, const BoxOut& out, uint8_t* stg, const float4* sums,
+                                              int part, int half, int q, int lane, uint32_t& turn)
+{
+    const int row0 = u.tm * 256 + half * 128 + q * 32;
+#pragma unroll 1
+    for (int ch = 8 * part / w.pairs; ch < 8 * (part + 1) / w.pairs; ++ch) {
+        const int col = u.tn * 256 + ch * 32;
+        if (col >= out.N) break;
+        const uint32_t at = smem_u32(sums + ch * 8 * 128 + q * 32 + lane);
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = 0.f;
+#pragma unroll 1
+        for (int s = 0; s < w.pairs; ++s) {
+            const uint32_t from = mapa_shared(at, static_cast<uint32_t>(2 * s + half));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 v = ld_cluster_f4(from + static_cast<uint32_t>(i * 128 * 16));
+                f[4 * i] += v.x;
+                f[4 * i + 1] += v.y;
+                f[4 * i + 2] += v.z;
+                f[4 * i + 3] += v.w;
+            }
+        }
+        store_box<OUT, BUFS>(out, stg, row0, lane, col, f, turn);
+    }
+}
+
+// A place in a ring of stages and the parity of its barriers.
+struct Ring {
+    int at = 0, size;
+    uint32_t phase = 0;
+    __device__ __forceinline__ explicit Ring(int n) : size(n) {}
+    __device__ __forceinline__ void next()
+    {
+        if (++at == size) {
+            at = 0;
+            phase ^= 1u;
+        }
+    }
+};
 
 template <int OUT>
 __global__ void __launch_bounds__(kF8Threads, 1)
@@ -206,9 +408,11 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
-    const int cluster_id = blockIdx.x / 2;
-    const int num_clusters = gridDim.x / 2;
-    const int tiles = p.tiles_m * p.tiles_n;
+    const uint32_t lead = rank & ~1u;  // the pair's leader
+    const int half = static_cast<int>(rank & 1u), part = static_cast<int>(rank >> 1);
+    const int cluster_id = blockIdx.x / (2 * p.work.pairs);
+    const int num_clusters = gridDim.x / (2 * p.work.pairs);
+    const int units = work_units(p.work);
 
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&tmap_a);
@@ -239,22 +443,19 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 
     if (warp == 0) {
         if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
+            Ring r(kF8Stages);
             bool ok = true;
-            for (int t = cluster_id; ok && t < tiles; t += num_clusters) {
-                int tm, tn;
-                f8_tile_coords(t, p.tiles_m, p.tiles_n, p.raster_group, tm, tn);
-                const int m0 = tm * 256 + static_cast<int>(rank) * 128;
-                const int n0 = tn * 256 + static_cast<int>(rank) * 128;
-                for (int st = 0; st < p.num_st; ++st) {
-                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns, kErrWaitProducer, stage)) {
+            for (int u = cluster_id; ok && u < units; u += num_clusters) {
+                const Work w = work_unit(p.work, u, part);
+                const int m0 = w.tm * 256 + half * 128, n0 = w.tn * 256 + half * 128;
+                for (int st = w.st0; st < w.st1; ++st, r.next()) {
+                    if (!mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitProducer, r.at)) {
                         ok = false;
                         break;
                     }
-                    if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), 2 * kF8StageBytes);
-                    const uint32_t bar = mapa_shared(full_bar(stage), 0);
-                    const uint32_t a_dst = smem_u32(sA + stage * kF8ABytes), b_dst = smem_u32(sB + stage * kF8BBytes);
+                    if (half == 0) mbar_arrive_expect_tx(full_bar(r.at), 2 * kF8StageBytes);
+                    const uint32_t bar = mapa_shared(full_bar(r.at), lead);
+                    const uint32_t a_dst = smem_u32(sA + r.at * kF8ABytes), b_dst = smem_u32(sB + r.at * kF8BBytes);
                     const int k0 = st * 256;
                     tma_load_2d_pair(a_dst, &tmap_a, bar, k0, m0);
                     tma_load_2d_pair(a_dst + 128 * 128, &tmap_a, bar, k0 + 128, m0);
@@ -264,45 +465,38 @@ __global__ void __launch_bounds__(kF8Threads, 1)
                     } else {
                         tma_load_2d_pair(b_dst, &tmap_b, bar, n0, k0);
                     }
-                    if (++stage == kF8Stages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
                 }
             }
-            // every stage this CTA filled is released by the MMAs before the CTA may exit
-            for (int i = 0; ok && i < kF8Stages; ++i) {
-                if (!mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns, kErrWaitTail, stage)) break;
-                if (++stage == kF8Stages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
-            }
+            // the MMAs' signals to this CTA's barriers have all arrived before the CTA may exit
+            for (int i = 0; ok && i < kF8Stages; ++i, r.next())
+                ok = mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitTail, r.at);
         }
     } else if (warp == 1) {
         auto mma_loop = [&](auto b_k_tag) {
             constexpr bool B_K = decltype(b_k_tag)::value;
             constexpr uint32_t kIdesc = idesc_mxf8(256, 256, !B_K);
-            int stage = 0, slot = 0, it = 0;
-            uint32_t phase = 0, sf_phase = 0, set = 0;
-            for (int t = cluster_id; t < tiles; t += num_clusters, ++it) {
-                // the tile before has left the columns the two accumulators share (and, before that, this one's)
+            Ring r(kF8Stages), sf(kF8SfSlots);
+            int it = 0;
+            uint32_t set = 0;
+            for (int u = cluster_id; u < units; u += num_clusters, ++it) {
+                const Work w = work_unit(p.work, u, part);
+                // the unit before has left the columns the two accumulators share (and, before that, this one's)
                 if (!mbar_wait(tempty_bar, static_cast<uint32_t>(it & 1) ^ 1u, p.timeout_ns, kErrWaitMma, 100)) return;
                 tc_fence_after();
                 const uint32_t d = tmem + ((it & 1) ? kF8Acc1 : 0);
-                for (int st = 0; st < p.num_st; ++st) {
-                    if (!mbar_wait(full_bar(stage), phase, p.timeout_ns, kErrWaitMma, stage)) return;
+                for (int st = w.st0; st < w.st1; ++st) {
+                    if (!mbar_wait(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) return;
                     const uint32_t sfa = tmem + kF8SfCol + set * 16, sfb = sfa + 4;
                     if ((st & 1) == 0) {
-                        if (!mbar_wait(sf_full_bar(slot), sf_phase, p.timeout_ns, kErrWaitMma, 200 + slot)) return;
+                        if (!mbar_wait(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) return;
                         tc_fence_after();
-                        const uint32_t src = smem_u32(sSf + slot * kF8SfBytes);
+                        const uint32_t src = smem_u32(sSf + sf.at * kF8SfBytes);
                         tmem_copy_scales_pair(sfa, smem_desc_rows16(src));
                         tmem_copy_scales_pair(sfb, smem_desc_rows16(src + 512));
                         tmem_copy_scales_pair(sfb + 4, smem_desc_rows16(src + 1024));
                     }
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(sA + stage * kF8ABytes), b_addr = smem_u32(sB + stage * kF8BBytes);
+                    const uint32_t a_addr = smem_u32(sA + r.at * kF8ABytes), b_addr = smem_u32(sB + r.at * kF8BBytes);
                     const int kk_end = min(8, (p.K - st * 256 + 31) / 32);
                     const uint32_t id0 = static_cast<uint32_t>(st & 1) * 2;  // scale bytes of this stage's two k-blocks
                     const uint32_t idesc = kIdesc | (id0 << 4) | (id0 << 29);
@@ -312,120 +506,88 @@ __global__ void __launch_bounds__(kF8Threads, 1)
                         const uint64_t a = smem_desc_sw128(a_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024);
                         const uint64_t b = B_K ? smem_desc_sw128(b_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024)
                                                : smem_desc_sw128(b_addr + kk * 32 * 128, 256 * 128, 1024);
-                        umma_mxf8_pair(d, a, b, idesc + (kk >> 2) * ((1u << 4) | (1u << 29)), sfa, sfb, (st | kk) != 0);
+                        umma_mxf8_pair(d, a, b, idesc + (kk >> 2) * ((1u << 4) | (1u << 29)), sfa, sfb, st != w.st0 || kk != 0);
                     }
-                    umma_commit<2>(empty_bar(stage));
-                    umma_commit<2>(mapa_shared(empty_bar(stage), 1));
-                    if (++stage == kF8Stages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
-                    if ((st & 1) || st + 1 == p.num_st) {
-                        umma_commit<2>(sf_empty_bar(slot));
-                        umma_commit<2>(mapa_shared(sf_empty_bar(slot), 1));
+                    umma_commit<2>(mapa_shared(empty_bar(r.at), lead));
+                    umma_commit<2>(mapa_shared(empty_bar(r.at), lead | 1u));
+                    r.next();
+                    if ((st & 1) || st + 1 == w.st1) {
+                        umma_commit<2>(mapa_shared(sf_empty_bar(sf.at), lead));
+                        umma_commit<2>(mapa_shared(sf_empty_bar(sf.at), lead | 1u));
                         set ^= 1u;
-                        if (++slot == kF8SfSlots) {
-                            slot = 0;
-                            sf_phase ^= 1u;
-                        }
+                        sf.next();
                     }
                 }
-                umma_commit<2>(tfull_bar(it & 1));
-                umma_commit<2>(mapa_shared(tfull_bar(it & 1), 1));
+                umma_commit<2>(mapa_shared(tfull_bar(it & 1), lead));
+                umma_commit<2>(mapa_shared(tfull_bar(it & 1), lead | 1u));
             }
         };
-        if (rank == 0 && lane == 0) {
+        if (half == 0 && lane == 0) {
             if (p.b_k)
                 mma_loop(std::true_type{});
             else
                 mma_loop(std::false_type{});
         }
     } else if (warp == 6) {
-        int slot = 0;
-        uint32_t phase = 0;
+        Ring sf(kF8SfSlots);
         const int num_kb = (p.K + 127) / 128;
         bool ok = true;
-        for (int t = cluster_id; ok && t < tiles; t += num_clusters) {
-            int tm, tn;
-            f8_tile_coords(t, p.tiles_m, p.tiles_n, p.raster_group, tm, tn);
-            const int m0 = tm * 256 + static_cast<int>(rank) * 128 + lane, n0 = tn * 256 + lane;
-            for (int kb = 0; kb < num_kb; kb += 4) {
-                uint4 a, b0, b1;
-                a.x = p.sa.word(m0, kb, num_kb);
-                a.y = p.sa.word(m0 + 32, kb, num_kb);
-                a.z = p.sa.word(m0 + 64, kb, num_kb);
-                a.w = p.sa.word(m0 + 96, kb, num_kb);
-                b0.x = p.sb.word(n0, kb, num_kb);
-                b0.y = p.sb.word(n0 + 32, kb, num_kb);
-                b0.z = p.sb.word(n0 + 64, kb, num_kb);
-                b0.w = p.sb.word(n0 + 96, kb, num_kb);
-                b1.x = p.sb.word(n0 + 128, kb, num_kb);
-                b1.y = p.sb.word(n0 + 160, kb, num_kb);
-                b1.z = p.sb.word(n0 + 192, kb, num_kb);
-                b1.w = p.sb.word(n0 + 224, kb, num_kb);
-                if (!mbar_wait(sf_empty_bar(slot), phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + slot)) {
+        for (int u = cluster_id; ok && u < units; u += num_clusters) {
+            const Work w = work_unit(p.work, u, part);
+            const int m0 = w.tm * 256 + half * 128 + lane, n0 = w.tn * 256 + lane;
+            for (int kb = w.st0 * 2; kb < min(num_kb, w.st1 * 2); kb += 4, sf.next()) {
+                uint32_t s[12];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] = p.sa.word(m0 + 32 * i, kb, num_kb);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[4 + i] = p.sb.word(n0 + 32 * i, kb, num_kb);
+                if (!mbar_wait(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at)) {
                     ok = false;
                     break;
                 }
-                uint4* dst = reinterpret_cast<uint4*>(sSf + slot * kF8SfBytes) + lane;
-                dst[0] = a;
-                dst[32] = b0;
-                dst[64] = b1;
+                uint4* dst = reinterpret_cast<uint4*>(sSf + sf.at * kF8SfBytes) + lane;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) dst[32 * i] = make_uint4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_pair(mapa_shared(sf_full_bar(slot), 0));
-                if (++slot == kF8SfSlots) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
+                if (lane == 0) mbar_arrive_pair(mapa_shared(sf_full_bar(sf.at), lead));
             }
             ok = __all_sync(0xffffffffu, ok);
         }
-        // the MMAs' signals to this CTA's barriers have all arrived before the CTA may exit
-        for (int i = 0; ok && i < kF8SfSlots; ++i) {
-            if (!mbar_wait(sf_empty_bar(slot), phase ^ 1u, p.timeout_ns, kErrWaitTail, 200 + slot)) break;
-            if (++slot == kF8SfSlots) {
-                slot = 0;
-                phase ^= 1u;
-            }
-        }
-    } else {
-        const int q = warp & 3;  // the lane quarter this warp may read
-        const BoxOut out{&tmap_c, p.C, p.ldc, p.M, p.N, p.c_tma};
-        uint8_t* stg = epi + q * kF8EpiWarpBytes;
-        uint32_t turn = 0;
+        // as above
+        for (int i = 0; ok && i < kF8SfSlots; ++i, sf.next())
+            ok = mbar_wait(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitTail, 200 + sf.at);
+    }
+
+    const bool epilogue = warp >= 2 && warp < 6;
+    const int q = warp & 3;  // the lane quarter an epilogue warp may read
+    const BoxOut out{&tmap_c, p.C, p.ldc, p.M, p.N, p.c_tma, 0};
+    uint8_t* stg = epi + q * kF8EpiWarpBytes;
+    float4* sums = reinterpret_cast<float4*>(sA);  // of a shared tile: its stages have all been read by then
+    uint32_t turn = 0;
+    if (epilogue) {
         int it = 0;
-        for (int t = cluster_id; t < tiles; t += num_clusters, ++it) {
+        for (int u = cluster_id; u < units; u += num_clusters, ++it) {
+            const Work w = work_unit(p.work, u, part);
             const int acc = it & 1;
             if (!mbar_wait(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, p.timeout_ns, kErrWaitEpilogue, acc)) break;
             tc_fence_after();
-            int tm, tn;
-            f8_tile_coords(t, p.tiles_m, p.tiles_n, p.raster_group, tm, tn);
-            const int row0 = tm * 256 + static_cast<int>(rank) * 128 + q * 32;
-            const uint32_t base = tmem + (acc ? kF8Acc1 : 0) + (static_cast<uint32_t>(q * 32) << 16);
-#pragma unroll 1
-            for (int j = 0; j < 8; ++j) {
-                // the shared columns first: the last 32 of accumulator 0, the first 32 of accumulator 1
-                const int c = (acc ? j : (j + 7) & 7) * 32;
-                uint32_t r[32];
-                tmem_ld_32x32b_x32(base + static_cast<uint32_t>(c), r);
-                tmem_ld_wait();
-                if (j == 0) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar, 0));
-                }
-                const int col = tn * 256 + c;
-                if (col >= p.N) continue;
-                float f[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
-                store_box<OUT>(out, stg, row0, lane, col, f, turn);
-            }
+            // the shared columns first: the last 32 of accumulator 0, the first 32 of accumulator 1
+            finish_unit<OUT, 2>(p.work, w, out, stg, p.work.pairs > 1 ? sums : nullptr, tmem + (acc ? kF8Acc1 : 0), acc ? 0 : 7, half, q, lane,
+                                turn, p.timeout_ns, [&] {
+                                    tc_fence_before();
+                                    __syncwarp();
+                                    if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar, lead));
+                                });
             tc_fence_before();
         }
-        if (p.c_tma && lane == 0) bulk_wait_group_all();
     }
+    if (p.work.pairs > 1) {
+        __syncthreads();
+        cluster_sync_all();
+        if (epilogue) finish_shared<OUT, 2>(p.work, work_unit(p.work, cluster_id, part), out, stg, sums, part, half, q, lane, turn);
+    }
+    if (epilogue && p.c_tma && lane == 0) bulk_wait_group_all();
 
     tc_fence_before();
     __syncthreads();
