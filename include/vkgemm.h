@@ -259,8 +259,7 @@ int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* args);
 
 /* C[m x n] = A * op(B) of 8-bit operands, fp32 accumulation, C in fp16, bf16 or fp32.  A is m x k.  With trans_b B is
  * stored n x k (a layer's weights in its forward pass); without, k x n (the same weights in the input's gradient),
- * which needs VK_FP8_TILE scales.  With a workspace (vk_gemm_fp8_workspace bytes, 16-byte aligned; it belongs to the call
- * until it has run) the tiles of a partial last wave are shared out over the whole GPU; without one (NULL) they are not. */
+ * which needs VK_FP8_TILE scales. */
 typedef struct vk_gemm_fp8_args {
     const void* A;
     const void* B;
@@ -273,17 +272,14 @@ typedef struct vk_gemm_fp8_args {
     int32_t a_scaling, b_scaling; /* vk_fp8_scaling */
     int32_t trans_b;
     int32_t dtype;                /* vk_dtype of C */
-    void* workspace;              /* may be NULL */
-    size_t workspace_bytes;
     void* stream;
 } vk_gemm_fp8_args;
-int vk_gemm_fp8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
 int vk_gemm_fp8(const vk_gemm_fp8_args* args);
 
 /* dW[n x k] = dY^T * X (accumulate = 1: dW += it): a layer's weight gradient from its output's gradient dY[tokens x n]
  * in 16 bits and its input X[tokens x k] as the forward pass kept it, in 8 bits with VK_FP8_ROW scales.  X's values are
  * used in dY's type: bf16 holds each of them exactly; fp16 rounds what lies below its smallest normal number and
- * holds what lies above its largest at that.  fp32 accumulation; dW in fp16, bf16 or fp32.  The workspace is as in vk_gemm_fp8. */
+ * holds what lies above its largest at that.  fp32 accumulation; dW in fp16, bf16 or fp32. */
 typedef struct vk_wgrad_fp8_args {
     const void* dY;
     const void* X;
@@ -294,11 +290,8 @@ typedef struct vk_wgrad_fp8_args {
     int32_t dtype;     /* of dY: VK_DTYPE_F16 or VK_DTYPE_BF16 */
     int32_t out_dtype; /* vk_dtype of dW */
     int32_t accumulate;
-    void* workspace;   /* may be NULL */
-    size_t workspace_bytes;
     void* stream;
 } vk_wgrad_fp8_args;
-int vk_wgrad_fp8_workspace(int64_t tokens, int64_t n, int64_t k, size_t* bytes);
 int vk_wgrad_fp8(const vk_wgrad_fp8_args* args);
 
 /* Multi-GPU row-block sharding (no counterpart in the reference, which is single-GPU,

@@ -157,63 +157,25 @@ int prepare_kernel(Kernel fn, int id, int smem, int threads, int clusters[4])
     return VK_OK;
 }
 
-// Workspace of a product whose last tiles are cut into slices: counters, then fp32 sums of at most one slice per pair.
-constexpr int kMaxPairs = 74;
-constexpr size_t kCounterBytes = 8192;
-constexpr size_t kSliceBytes = 2 * 128 * 256 * sizeof(float);
-
-int grains_of(const TileWork& w) { return (w.stages + w.grain - 1) / w.grain; }
-
-// Shares the tiles out.  Fewer tiles than clusters of several pairs: as many pairs to a tile as can all run at once.
-// Otherwise the tiles of a partial last wave are cut into up to 4 slices (more would have more sums to join than the whole
-// tiles after them hide), none shorter than `least` grains.
-void plan_work(TileWork& w, const int clusters[4], int least, void* workspace, int* launch)
+// Shares the tiles out.  Fewer tiles than clusters of several pairs: as many pairs to a tile as can all run at once, each
+// with at least `least` grains of k.  Otherwise the tiles of a last wave that at most half of the pairs would have are
+// halved.
+int plan_work(TileWork& w, const int clusters[4], int least)
 {
     const long long tiles = static_cast<long long>(w.tiles_m) * w.tiles_n;
-    const int grains = grains_of(w), pairs = clusters[0] < kMaxPairs ? clusters[0] : kMaxPairs;
+    const int grains = (w.stages + w.grain - 1) / w.grain;
     w.raster_group = 8;
-    w.pairs = w.split = 1;
-    w.tail = 0;
-    w.ws = nullptr;
-    w.counters = nullptr;
+    w.pairs = 1;
+    w.halved = 0;
     for (int s = 4; s >= 2; --s)
         if (tiles <= clusters[s - 1] && grains >= s * least) {
             w.pairs = s;
-            *launch = static_cast<int>(tiles);
-            return;
+            return static_cast<int>(tiles);
         }
-    const long long rest = tiles % pairs;
-    if (workspace != nullptr && rest > 0) {
-        long long s = pairs / rest;
-        if (s > 4) s = 4;
-        if (s > grains / least) s = grains / least;
-        if (s >= 2) {
-            w.tail = static_cast<int>(rest);
-            w.split = static_cast<int>(s);
-            w.counters = static_cast<int*>(workspace);
-            w.ws = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-        }
-    }
+    const long long rest = tiles % clusters[0];
+    if (2 * rest <= clusters[0]) w.halved = static_cast<int>(rest);
     const int units = work_units(w);
-    *launch = units < pairs ? units : pairs;
-}
-
-int clear_counters(const TileWork& w, cudaStream_t stream)
-{
-    if (w.tail > 0) F8_CUDA_TRY(cudaMemsetAsync(w.counters, 0, static_cast<size_t>(w.tail) * 16 * sizeof(int), stream));
-    return VK_OK;
-}
-
-int check_workspace(const char* name, const void* p, size_t bytes, size_t need)
-{
-    if (p != nullptr && (bytes < need || !aligned(p, 16)))
-        return set_error(VK_ERR_INVALID_ARGUMENT, "%s: a workspace has %zu bytes and is 16-byte aligned (%s_workspace), or is NULL", name, need, name);
-    return VK_OK;
-}
-
-size_t product_workspace(int64_t m, int64_t n, int64_t k)
-{
-    return m > 0 && n > 0 && k > 0 ? kCounterBytes + kMaxPairs * kSliceBytes : 0;
+    return units < clusters[0] ? units : clusters[0];
 }
 
 template <typename Kernel, typename... Args>
@@ -452,37 +414,13 @@ static int launch_simt(const LA& la, const LB& lb, const F8Output& out, int64_t 
     return launched();
 }
 
-extern "C" int vk_gemm_fp8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes)
-{
-    static const char* const name = "vk_gemm_fp8_workspace";
-    if (bytes == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: bytes is NULL", name);
-    if (m < 0 || m > kMaxDim) return bad_size(name, "m", m);
-    if (n < 0 || n > kMaxDim) return bad_size(name, "n", n);
-    if (k < 0 || k > kMaxDim) return bad_size(name, "k", k);
-    *bytes = product_workspace(m, n, k);
-    return VK_OK;
-}
-
-extern "C" int vk_wgrad_fp8_workspace(int64_t tokens, int64_t n, int64_t k, size_t* bytes)
-{
-    static const char* const name = "vk_wgrad_fp8_workspace";
-    if (bytes == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: bytes is NULL", name);
-    if (tokens < 0 || tokens > kMaxDim) return bad_size(name, "tokens", tokens);
-    if (n < 0 || n > kMaxDim) return bad_size(name, "n", n);
-    if (k < 0 || k > kMaxDim) return bad_size(name, "k", k);
-    *bytes = product_workspace(n, k, tokens);
-    return VK_OK;
-}
-
 template <int OUT>
-static int launch_gemm(F8GemmParams p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, void* workspace, cudaStream_t stream)
+static int launch_gemm(F8GemmParams p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, cudaStream_t stream)
 {
-    int fit[4], clusters = 0;
-    int rc = prepare_kernel(gemm_fp8_kernel<OUT>, OUT, kF8SmemBytes, kF8Threads, fit);
+    int fit[4];
+    const int rc = prepare_kernel(gemm_fp8_kernel<OUT>, OUT, kF8SmemBytes, kF8Threads, fit);
     if (rc != VK_OK) return rc;
-    plan_work(p.work, fit, 2, workspace, &clusters);
-    rc = clear_counters(p.work, stream);
-    if (rc != VK_OK) return rc;
+    const int clusters = plan_work(p.work, fit, 2);
     return launch_clusters(gemm_fp8_kernel<OUT>, clusters, 2 * p.work.pairs, kF8Threads, kF8SmemBytes, stream, ta, tb, tc, p);
 }
 
@@ -522,8 +460,6 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     if (rc == VK_OK) rc = ld_of(name, "ld_a_scale", a->ld_a_scale, kb, &ldas);
     if (rc == VK_OK) rc = ld_of(name, "ld_b_scale", a->ld_b_scale, (b_row + 127) / 128, &ldbs);
     if (rc != VK_OK) return rc;
-    rc = check_workspace(name, a->workspace, a->workspace_bytes, product_workspace(a->m, a->n, a->k));
-    if (rc != VK_OK) return rc;
     if (a->m == 0 || a->n == 0) return VK_OK;
     if (a->C == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: C is NULL", name);
     if (a->k > 0 && (a->A == nullptr || a->B == nullptr || a->a_scale == nullptr || a->b_scale == nullptr))
@@ -551,13 +487,13 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
         CUtensorMap ta, tb, tc;
         rc = make_map(&ta, a->A, a->m, a->k, lda, 1, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc == VK_OK)
-            rc = a->trans_b ? make_map(&tb, a->B, a->n, a->k, ldb, 1, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B)
+            rc = a->trans_b ? make_map(&tb, a->B, a->n, a->k, ldb, 1, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B)
                             : make_map(&tb, a->B, a->k, a->n, ldb, 1, 128, 256, CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc == VK_OK) rc = make_out_map(&tc, a->C, a->m, a->n, ldc, a->dtype, &p.c_tma);
         if (rc != VK_OK) return rc;
-        return a->dtype == VK_DTYPE_F16   ? launch_gemm<VK_DTYPE_F16>(p, ta, tb, tc, a->workspace, stream)
-               : a->dtype == VK_DTYPE_F32 ? launch_gemm<VK_DTYPE_F32>(p, ta, tb, tc, a->workspace, stream)
-                                          : launch_gemm<VK_DTYPE_BF16>(p, ta, tb, tc, a->workspace, stream);
+        return a->dtype == VK_DTYPE_F16   ? launch_gemm<VK_DTYPE_F16>(p, ta, tb, tc, stream)
+               : a->dtype == VK_DTYPE_F32 ? launch_gemm<VK_DTYPE_F32>(p, ta, tb, tc, stream)
+                                          : launch_gemm<VK_DTYPE_BF16>(p, ta, tb, tc, stream);
     }
     const int tile_a = a->a_scaling == VK_FP8_TILE ? 7 : 0, tile_b = a->b_scaling == VK_FP8_TILE ? 7 : 0;
     const F8Operand fa{static_cast<const uint8_t*>(a->A), static_cast<const uint8_t*>(a->a_scale), lda, 1, ldas, 1, tile_a, 7};
@@ -573,16 +509,14 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
 }
 
 template <typename T, int OUT>
-static int launch_wgrad(WgradParams p, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, void* workspace, cudaStream_t stream)
+static int launch_wgrad(WgradParams p, const CUtensorMap& ta, const CUtensorMap& tc, cudaStream_t stream)
 {
     constexpr int kId = 3 + 3 * (std::is_same_v<T, __half> ? 0 : 1) + OUT;
-    int fit[4], clusters = 0;
-    int rc = prepare_kernel(wgrad_fp8_kernel<T, OUT>, kId, kWgSmemBytes, kWgThreads, fit);
+    int fit[4];
+    const int rc = prepare_kernel(wgrad_fp8_kernel<T, OUT>, kId, kWgSmemBytes, kWgThreads, fit);
     if (rc != VK_OK) return rc;
-    plan_work(p.work, fit, 4, workspace, &clusters);
-    rc = clear_counters(p.work, stream);
-    if (rc != VK_OK) return rc;
-    return launch_clusters(wgrad_fp8_kernel<T, OUT>, clusters, 2 * p.work.pairs, kWgThreads, kWgSmemBytes, stream, ta, tb, tc, p);
+    const int clusters = plan_work(p.work, fit, 4);
+    return launch_clusters(wgrad_fp8_kernel<T, OUT>, clusters, 2 * p.work.pairs, kWgThreads, kWgSmemBytes, stream, ta, tc, p);
 }
 
 extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
@@ -603,8 +537,6 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
     if (rc == VK_OK) rc = ld_of(name, "ld_x_scale", a->ld_x_scale, (a->k + 127) / 128, &ldxs);
     if (rc == VK_OK) rc = ld_of(name, "lddw", a->lddw, a->k, &lddw);
     if (rc != VK_OK) return rc;
-    rc = check_workspace(name, a->workspace, a->workspace_bytes, product_workspace(a->n, a->k, a->tokens));
-    if (rc != VK_OK) return rc;
     if (a->n == 0 || a->k == 0) return VK_OK;
     if (a->dW == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: dW is NULL", name);
     if (a->tokens > 0 && (a->dY == nullptr || a->X == nullptr || a->x_scale == nullptr))
@@ -623,22 +555,23 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
         p.work.tiles_n = static_cast<int>((a->k + 255) / 256);
         p.work.stages = static_cast<int>((a->tokens + kWgBK - 1) / kWgBK);
         p.work.grain = 1;
+        p.X = static_cast<const uint8_t*>(a->X);
+        p.ldx = ldx;
         p.scale = static_cast<const uint8_t*>(a->x_scale);
         p.lds = ldxs;
         p.C = a->dW;
         p.ldc = lddw;
         p.accumulate = a->accumulate;
         p.timeout_ns = wait_timeout_ns();
-        CUtensorMap ta, tb, tc;
+        CUtensorMap ta, tc;
         rc = make_map(&ta, a->dY, a->tokens, a->n, lddy, 2, 64, kWgBK, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc == VK_OK) rc = make_map(&tb, a->X, a->tokens, a->k, ldx, 1, 128, kWgXK, CU_TENSOR_MAP_SWIZZLE_NONE);
         if (rc == VK_OK) rc = make_out_map(&tc, a->dW, a->n, a->k, lddw, a->out_dtype, &p.c_tma);
         if (rc != VK_OK) return rc;
         return for_type(a->dtype, [&](auto t) {
             using T = std::conditional_t<std::is_same_v<decltype(t), __half>, __half, __nv_bfloat16>;
-            return a->out_dtype == VK_DTYPE_F16   ? launch_wgrad<T, VK_DTYPE_F16>(p, ta, tb, tc, a->workspace, stream)
-                   : a->out_dtype == VK_DTYPE_F32 ? launch_wgrad<T, VK_DTYPE_F32>(p, ta, tb, tc, a->workspace, stream)
-                                                  : launch_wgrad<T, VK_DTYPE_BF16>(p, ta, tb, tc, a->workspace, stream);
+            return a->out_dtype == VK_DTYPE_F16   ? launch_wgrad<T, VK_DTYPE_F16>(p, ta, tc, stream)
+                   : a->out_dtype == VK_DTYPE_F32 ? launch_wgrad<T, VK_DTYPE_F32>(p, ta, tc, stream)
+                                                  : launch_wgrad<T, VK_DTYPE_BF16>(p, ta, tc, stream);
         });
     }
     const F8Operand fx{static_cast<const uint8_t*>(a->X), static_cast<const uint8_t*>(a->x_scale), 1, ldx, 1, ldxs, 7, 0};

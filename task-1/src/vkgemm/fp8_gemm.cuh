@@ -16,12 +16,11 @@
 // accumulator begins at column 224: the two share 32 columns, which the epilogue reads first; the next tile's MMAs start
 // once it has.  Columns 480..511 hold two sets of scales (4 columns for A's 128 rows, 8 for B's 256), each for 512 of k.
 //
-// How tiles are handed out (TileWork): pairs walk over whole tiles.  The tiles of a partial last wave are cut along k into
-// slices, numbered first, so that joining them overlaps the whole tiles that follow: each (slice, CTA, epilogue warp)
-// counts its arrival; all but the last to arrive write their fp32 sums to the workspace and count that too, and the last
-// adds all slices' sums in slice order, whoever it is, so a result never depends on timing.  It waits (bounded) only for
-// CTAs that have arrived.  When there are fewer tiles than pairs, a cluster of 2 to 4 pairs shares one tile instead: each
-// pair sums its share of k, leaves it in its own shared memory, and adds its part of the columns from all of them.
+// How tiles are handed out (TileWork): pairs walk over whole tiles; when the last wave would leave half of them or more
+// without one, its tiles are cut into column halves.  (Cutting them along k, with the partial sums joined through
+// global memory, was built and measured first: writing the sums took 5 us and adding them 10, which held up the next
+// tile by more than the shorter wave gave.)  When there are fewer tiles than pairs, a cluster of 2 to 4 pairs shares one
+// tile: each pair sums its share of k, leaves it in its own shared memory, and adds its part of the columns from all.
 //
 // Scales in shared memory and tensor memory: row r's word (4 k-blocks) of a unit of 128 rows sits at byte
 // (r % 32) * 16 + (r / 32) * 4; tcgen05.cp.32x128b.warpx4 makes that lane r % 32, column r / 32, in all four lane quarters.
@@ -57,41 +56,28 @@ struct ScaleSource {
 // How the 256 x 256 tiles of an output are shared out over clusters.
 struct TileWork {
     int tiles_m, tiles_n, raster_group;
-    int stages;          // k-stages of a tile
-    int grain;           // stages that a slice's boundaries are multiples of
-    int pairs;           // pairs of CTAs that share each tile through their cluster's shared memory (1: none)
-    int tail, split;     // the last `tail` tiles are cut into `split` slices each, joined through the workspace
-    float* ws;           // [tail tile][slice][CTA of the pair][epilogue warp][32 rows x 256 columns] fp32
-    int* counters;       // [tail tile][CTA of the pair][epilogue warp][arrived, written], zero at the launch
+    int stages;  // k-stages of a tile
+    int grain;   // stages that a share of k begins at multiples of
+    int pairs;   // pairs of CTAs that share each tile through their cluster's shared memory (1: none)
+    int halved;  // the last `halved` tiles are two units of 128 columns each
 };
 
-// A pair's next piece of work: stages [st0, st1) of a tile.
+// A pair's next piece of work: stages [st0, st1) of `cols` columns from column n0 of tile row tm.
 struct Work {
-    int tm, tn, st0, st1;
-    int slice;           // of a tail tile, -1 for a whole one
-    int index;           // of the tail tile
+    int tm, n0, cols, st0, st1;
 };
 
-__host__ __device__ __forceinline__ int work_units(const TileWork& w)
-{
-    return w.tiles_m * w.tiles_n + w.tail * (w.split - 1);
-}
+__host__ __device__ __forceinline__ int work_units(const TileWork& w) { return w.tiles_m * w.tiles_n + w.halved; }
 
 // Unit u; `part`: which of w.pairs this pair is.
 __host__ __device__ __forceinline__ Work work_unit(const TileWork& w, int u, int part)
 {
     Work r;
-    int t = u - w.tail * w.split, cut = w.pairs, piece = part;
-    r.slice = r.index = -1;
-    if (t < 0) {
-        r.index = u / w.split;
-        r.slice = piece = u - r.index * w.split;
-        cut = w.split;
-        t = w.tiles_m * w.tiles_n - w.tail + r.index;
-    }
+    const int whole = w.tiles_m * w.tiles_n - w.halved;
+    const int t = u < whole ? u : whole + (u - whole) / 2;
     const int grains = (w.stages + w.grain - 1) / w.grain;
-    r.st0 = static_cast<int>(static_cast<long long>(grains) * piece / cut) * w.grain;
-    r.st1 = static_cast<int>(static_cast<long long>(grains) * (piece + 1) / cut) * w.grain;
+    r.st0 = static_cast<int>(static_cast<long long>(grains) * part / w.pairs) * w.grain;
+    r.st1 = static_cast<int>(static_cast<long long>(grains) * (part + 1) / w.pairs) * w.grain;
     if (r.st1 > w.stages) r.st1 = w.stages;
     const int per_group = w.raster_group * w.tiles_n;
     const int g = t / per_group;
@@ -99,7 +85,8 @@ __host__ __device__ __forceinline__ Work work_unit(const TileWork& w, int u, int
     const int rows = w.tiles_m - first_m < w.raster_group ? w.tiles_m - first_m : w.raster_group;
     const int in = t - g * per_group;
     r.tm = first_m + in % rows;
-    r.tn = in / rows;
+    r.n0 = in / rows * 256 + (u < whole ? 0 : (u - whole) % 2 * 128);
+    r.cols = u < whole ? 256 : 128;
     return r;
 }
 
@@ -184,8 +171,8 @@ struct BoxOut {
     int accumulate;          // C += the results
 };
 
-// Results col .. col + 31 of this lane's row (row0 + lane).  BUFS boxes of staging take turns; `turn` counts them.
-template <int OUT, int BUFS>
+// Results col .. col + 31 of this lane's row (row0 + lane).  Two boxes of staging take turns; `turn` counts them.
+template <int OUT>
 __device__ __forceinline__ void store_box(const BoxOut& o, uint8_t* stg, int row0, int lane, int col, float (&f)[32], uint32_t& turn)
 {
     using T = std::conditional_t<OUT == 0, __half, std::conditional_t<OUT == 1, float, __nv_bfloat16>>;
@@ -205,8 +192,8 @@ __device__ __forceinline__ void store_box(const BoxOut& o, uint8_t* stg, int row
 #pragma unroll
         for (int h = 0; h < 32 / kCols; ++h) {
             if (col + h * kCols >= o.N) break;
-            uint8_t* box = stg + (turn % BUFS) * 2048;
-            if (lane == 0) bulk_wait_group_read<BUFS - 1>();
+            uint8_t* box = stg + (turn & 1u) * 2048;
+            if (lane == 0) bulk_wait_group_read<1>();
             __syncwarp();
             uint4* to = reinterpret_cast<uint4*>(box + lane * 64);
 #pragma unroll
@@ -253,101 +240,42 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr)
     return v;
 }
 
-// An epilogue warp's way with one unit's accumulator: columns acc .. acc + 255 of its lane quarter, read in chunks of 32
-// beginning with chunk `first`; `early()` is called once that one has been read.  part: where a pair that shares its
-// tile leaves its sums (null otherwise).
-template <int OUT, int BUFS, typename Early>
-__device__ __forceinline__ void finish_unit(const TileWork& w, const Work& u, const BoxOut& out, uint8_t* stg, float4* part, uint32_t acc,
-                                            int first, int half, int q, int lane, uint32_t& turn, unsigned long long timeout_ns,
-                                            const Early& early)
+// An epilogue warp's way with one unit's accumulator, from column acc of its lane quarter, in chunks of 32 columns
+// beginning with chunk `first`; `early()` is called once that one has been read.  sums: where a pair that shares its
+// tile leaves what it has (null otherwise).
+template <int OUT, typename Early>
+__device__ __forceinline__ void finish_unit(const Work& u, const BoxOut& out, uint8_t* stg, float4* sums, uint32_t acc, int first, int half,
+                                            int q, int lane, uint32_t& turn, const Early& early)
 {
     const int row0 = u.tm * 256 + half * 128 + q * 32;
     const uint32_t base = acc + (static_cast<uint32_t>(q * 32) << 16);
-    float f[32];
-    if (u.slice < 0) {
+    const int chunks = u.cols / 32;
 #pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-            const int ch = (j + first) & 7;
-            tmem_chunk(base + static_cast<uint32_t>(ch * 32), f);
-            if (j == 0) early();
-            const int col = u.tn * 256 + ch * 32;
-            if (part != nullptr) {
-                float4* to = part + ch * 8 * 128 + q * 32 + lane;
+    for (int j = 0; j < chunks; ++j) {
+        const int ch = (j + first) & (chunks - 1);
+        float f[32];
+        tmem_chunk(base + static_cast<uint32_t>(ch * 32), f);
+        if (j == 0) early();
+        const int col = u.n0 + ch * 32;
+        if (sums != nullptr) {
+            float4* to = sums + ch * 8 * 128 + q * 32 + lane;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) to[i * 128] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-            } else if (col < out.N) {
-                store_box<OUT, BUFS>(out, stg, row0, lane, col, f, turn);
-            }
+            for (int i = 0; i < 8; ++i) to[i * 128] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+        } else if (col < out.N) {
+            store_box<OUT>(out, stg, row0, lane, col, f, turn);
         }
-        return;
-    }
-    constexpr long long kWarp = 32 * 256;
-    int* ctr = w.counters + ((u.index * 2 + half) * 4 + q) * 2;
-    auto sums_of = [&](int slice) {
-        return reinterpret_cast<float4*>(w.ws + ((static_cast<long long>(u.index * w.split + slice) * 2 + half) * 4 + q) * kWarp) + lane;
-    };
-    int arrived = 0;
-    if (lane == 0) arrived = atomicAdd(&ctr[0], 1);
-    arrived = __shfl_sync(0xffffffffu, arrived, 0);
-    if (arrived < w.split - 1) {
-        float4* mine = sums_of(u.slice);
-#pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-            const int ch = (j + first) & 7;
-            tmem_chunk(base + static_cast<uint32_t>(ch * 32), f);
-            if (j == 0) early();
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                __stcg(mine + (ch * 8 + i) * 32, make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]));
-        }
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) atomicAdd(&ctr[1], 1);
-        return;
-    }
-    float own[32];
-    tmem_chunk(base + static_cast<uint32_t>(first * 32), own);
-    early();
-    int ok = 1;
-    if (lane == 0) ok = wait_count_at_least(&ctr[1], w.split - 1, timeout_ns, kErrWaitEpilogue, 300 + q);
-    ok = __shfl_sync(0xffffffffu, ok, 0);
-    __threadfence();
-#pragma unroll 1
-    for (int j = 0; j < 8; ++j) {
-        const int ch = (j + first) & 7;
-        if (j > 0) tmem_chunk(base + static_cast<uint32_t>(ch * 32), own);
-        const int col = u.tn * 256 + ch * 32;
-        if (!ok || col >= out.N) continue;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = 0.f;
-#pragma unroll 1
-        for (int s = 0; s < w.split; ++s) {
-            float4 v[8];
-            const float4* from = sums_of(s) + ch * 8 * 32;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = s == u.slice ? make_float4(own[4 * i], own[4 * i + 1], own[4 * i + 2], own[4 * i + 3]) : __ldcg(from + i * 32);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                f[4 * i] += v[i].x;
-                f[4 * i + 1] += v[i].y;
-                f[4 * i + 2] += v[i].z;
-                f[4 * i + 3] += v[i].w;
-            }
-        }
-        store_box<OUT, BUFS>(out, stg, row0, lane, col, f, turn);
     }
 }
 
 // The columns of a shared tile that fall to pair `part`, added from all pairs' shared memory.
-template <int OUT, int BUFS>
+template <int OUT>
 __device__ __forceinline__ void finish_shared(const TileWork& w, const Work& u, const BoxOut& out, uint8_t* stg, const float4* sums,
                                               int part, int half, int q, int lane, uint32_t& turn)
 {
     const int row0 = u.tm * 256 + half * 128 + q * 32;
 #pragma unroll 1
     for (int ch = 8 * part / w.pairs; ch < 8 * (part + 1) / w.pairs; ++ch) {
-        const int col = u.tn * 256 + ch * 32;
+        const int col = u.n0 + ch * 32;
         if (col >= out.N) break;
         const uint32_t at = smem_u32(sums + ch * 8 * 128 + q * 32 + lane);
         float f[32];
@@ -365,7 +293,7 @@ __device__ __forceinline__ void finish_shared(const TileWork& w, const Work& u, 
                 f[4 * i + 3] += v.w;
             }
         }
-        store_box<OUT, BUFS>(out, stg, row0, lane, col, f, turn);
+        store_box<OUT>(out, stg, row0, lane, col, f, turn);
     }
 }
 
@@ -407,8 +335,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_ctarank();
-    const uint32_t lead = rank & ~1u;  // the pair's leader
+    const uint32_t rank = blockIdx.x % (2 * p.work.pairs);  // in the cluster
+    const uint32_t lead = rank & ~1u;                       // the pair's leader
     const int half = static_cast<int>(rank & 1u), part = static_cast<int>(rank >> 1);
     const int cluster_id = blockIdx.x / (2 * p.work.pairs);
     const int num_clusters = gridDim.x / (2 * p.work.pairs);
@@ -447,22 +375,27 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             bool ok = true;
             for (int u = cluster_id; ok && u < units; u += num_clusters) {
                 const Work w = work_unit(p.work, u, part);
-                const int m0 = w.tm * 256 + half * 128, n0 = w.tn * 256 + half * 128;
+                const int m0 = w.tm * 256 + half * 128, n0 = w.n0 + half * (w.cols / 2);
+                const int b_boxes = w.cols / 128;  // of 64 rows of a B stored n x k
+                const uint32_t bytes = kF8ABytes + (p.b_k ? w.cols / 2 * 256 : kF8BBytes);
                 for (int st = w.st0; st < w.st1; ++st, r.next()) {
                     if (!mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitProducer, r.at)) {
                         ok = false;
                         break;
                     }
-                    if (half == 0) mbar_arrive_expect_tx(full_bar(r.at), 2 * kF8StageBytes);
+                    if (half == 0) mbar_arrive_expect_tx(full_bar(r.at), 2 * bytes);
                     const uint32_t bar = mapa_shared(full_bar(r.at), lead);
                     const uint32_t a_dst = smem_u32(sA + r.at * kF8ABytes), b_dst = smem_u32(sB + r.at * kF8BBytes);
                     const int k0 = st * 256;
                     tma_load_2d_pair(a_dst, &tmap_a, bar, k0, m0);
                     tma_load_2d_pair(a_dst + 128 * 128, &tmap_a, bar, k0 + 128, m0);
                     if (p.b_k) {
-                        tma_load_2d_pair(b_dst, &tmap_b, bar, k0, n0);
-                        tma_load_2d_pair(b_dst + 128 * 128, &tmap_b, bar, k0 + 128, n0);
+                        for (int i = 0; i < b_boxes; ++i) {
+                            tma_load_2d_pair(b_dst + i * 64 * 128, &tmap_b, bar, k0, n0 + 64 * i);
+                            tma_load_2d_pair(b_dst + (128 + i * 64) * 128, &tmap_b, bar, k0 + 128, n0 + 64 * i);
+                        }
                     } else {
+                        // 128 columns whatever their number in use: the width of a swizzled row
                         tma_load_2d_pair(b_dst, &tmap_b, bar, n0, k0);
                     }
                 }
@@ -472,57 +405,64 @@ __global__ void __launch_bounds__(kF8Threads, 1)
                 ok = mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitTail, r.at);
         }
     } else if (warp == 1) {
+        // The whole warp walks through the loop and one lane issues: what the instructions take is then the same in every
+        // lane and stays in uniform registers.  With one lane in the loop, issuing the eight MMAs of a stage took longer
+        // than running them (1422 clocks a stage instead of 1024).
         auto mma_loop = [&](auto b_k_tag) {
             constexpr bool B_K = decltype(b_k_tag)::value;
-            constexpr uint32_t kIdesc = idesc_mxf8(256, 256, !B_K);
+            constexpr uint32_t kIdesc = idesc_mxf8(256, 256, !B_K), kIdescHalf = idesc_mxf8(256, 128, !B_K);
+            const bool one = elect_one();
+            const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t a_desc = smem_desc_sw128(smem_u32(sA), 16, 1024);
+            const uint64_t b_desc = B_K ? smem_desc_sw128(smem_u32(sB), 16, 1024) : smem_desc_sw128(smem_u32(sB), 256 * 128, 1024);
+            const uint64_t sf_desc = smem_desc_rows16(smem_u32(sSf));
             Ring r(kF8Stages), sf(kF8SfSlots);
             int it = 0;
             uint32_t set = 0;
             for (int u = cluster_id; u < units; u += num_clusters, ++it) {
                 const Work w = work_unit(p.work, u, part);
                 // the unit before has left the columns the two accumulators share (and, before that, this one's)
-                if (!mbar_wait(tempty_bar, static_cast<uint32_t>(it & 1) ^ 1u, p.timeout_ns, kErrWaitMma, 100)) return;
-                tc_fence_after();
-                const uint32_t d = tmem + ((it & 1) ? kF8Acc1 : 0);
+                if (!mbar_wait_warp(tempty_bar, static_cast<uint32_t>(it & 1) ^ 1u, p.timeout_ns, kErrWaitMma, 100)) return;
+                const uint32_t d = base + ((it & 1) ? kF8Acc1 : 0);
                 for (int st = w.st0; st < w.st1; ++st) {
-                    if (!mbar_wait(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) return;
-                    const uint32_t sfa = tmem + kF8SfCol + set * 16, sfb = sfa + 4;
-                    if ((st & 1) == 0) {
-                        if (!mbar_wait(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) return;
-                        tc_fence_after();
-                        const uint32_t src = smem_u32(sSf + sf.at * kF8SfBytes);
-                        tmem_copy_scales_pair(sfa, smem_desc_rows16(src));
-                        tmem_copy_scales_pair(sfb, smem_desc_rows16(src + 512));
-                        tmem_copy_scales_pair(sfb + 4, smem_desc_rows16(src + 1024));
-                    }
+                    const uint32_t sfa = base + kF8SfCol + set * 16, sfb = sfa + 4;
+                    if ((st & 1) == 0 && !mbar_wait_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) return;
+                    if (!mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) return;
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(sA + r.at * kF8ABytes), b_addr = smem_u32(sB + r.at * kF8BBytes);
-                    const int kk_end = min(8, (p.K - st * 256 + 31) / 32);
-                    const uint32_t id0 = static_cast<uint32_t>(st & 1) * 2;  // scale bytes of this stage's two k-blocks
-                    const uint32_t idesc = kIdesc | (id0 << 4) | (id0 << 29);
+                    const bool last = (st & 1) || st + 1 == w.st1;  // of its set of scales
+                    if (one) {
+                        if ((st & 1) == 0) {
+                            const uint64_t src = sf_desc + static_cast<uint32_t>(sf.at) * (kF8SfBytes >> 4);
+                            tmem_copy_scales_pair(sfa, src);
+                            tmem_copy_scales_pair(sfb, src + (512 >> 4));
+                            tmem_copy_scales_pair(sfb + 4, src + (1024 >> 4));
+                        }
+                        const uint64_t a = a_desc + static_cast<uint32_t>(r.at) * (kF8ABytes >> 4);
+                        const uint64_t b = b_desc + static_cast<uint32_t>(r.at) * (kF8BBytes >> 4);
+                        const int kk_end = min(8, (p.K - st * 256 + 31) / 32);
+                        const uint32_t id0 = static_cast<uint32_t>(st & 1) * 2;  // scale bytes of this stage's two k-blocks
+                        const uint32_t idesc = (w.cols == 256 ? kIdesc : kIdescHalf) | (id0 << 4) | (id0 << 29);
 #pragma unroll
-                    for (int kk = 0; kk < 8; ++kk) {
-                        if (kk >= kk_end) break;
-                        const uint64_t a = smem_desc_sw128(a_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024);
-                        const uint64_t b = B_K ? smem_desc_sw128(b_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024)
-                                               : smem_desc_sw128(b_addr + kk * 32 * 128, 256 * 128, 1024);
-                        umma_mxf8_pair(d, a, b, idesc + (kk >> 2) * ((1u << 4) | (1u << 29)), sfa, sfb, st != w.st0 || kk != 0);
+                        for (int kk = 0; kk < 8; ++kk) {
+                            if (kk >= kk_end) break;
+                            umma_mxf8_pair(d, a + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4),
+                                           b + ((B_K ? (kk >> 2) * (128 * 128) + (kk & 3) * 32 : kk * 32 * 128) >> 4),
+                                           idesc + (kk >> 2) * ((1u << 4) | (1u << 29)), sfa, sfb, st != w.st0 || kk != 0);
+                        }
+                        umma_commit_pair(empty_bar(r.at), lead);
+                        if (last) umma_commit_pair(sf_empty_bar(sf.at), lead);
+                        if (st + 1 == w.st1) umma_commit_pair(tfull_bar(it & 1), lead);
                     }
-                    umma_commit<2>(mapa_shared(empty_bar(r.at), lead));
-                    umma_commit<2>(mapa_shared(empty_bar(r.at), lead | 1u));
+                    __syncwarp();
                     r.next();
-                    if ((st & 1) || st + 1 == w.st1) {
-                        umma_commit<2>(mapa_shared(sf_empty_bar(sf.at), lead));
-                        umma_commit<2>(mapa_shared(sf_empty_bar(sf.at), lead | 1u));
+                    if (last) {
                         set ^= 1u;
                         sf.next();
                     }
                 }
-                umma_commit<2>(mapa_shared(tfull_bar(it & 1), lead));
-                umma_commit<2>(mapa_shared(tfull_bar(it & 1), lead | 1u));
             }
         };
-        if (half == 0 && lane == 0) {
+        if (half == 0) {
             if (p.b_k)
                 mma_loop(std::true_type{});
             else
@@ -534,7 +474,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         bool ok = true;
         for (int u = cluster_id; ok && u < units; u += num_clusters) {
             const Work w = work_unit(p.work, u, part);
-            const int m0 = w.tm * 256 + half * 128 + lane, n0 = w.tn * 256 + lane;
+            const int m0 = w.tm * 256 + half * 128 + lane, n0 = w.n0 + lane;
             for (int kb = w.st0 * 2; kb < min(num_kb, w.st1 * 2); kb += 4, sf.next()) {
                 uint32_t s[12];
 #pragma unroll
@@ -573,19 +513,18 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             if (!mbar_wait(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, p.timeout_ns, kErrWaitEpilogue, acc)) break;
             tc_fence_after();
             // the shared columns first: the last 32 of accumulator 0, the first 32 of accumulator 1
-            finish_unit<OUT, 2>(p.work, w, out, stg, p.work.pairs > 1 ? sums : nullptr, tmem + (acc ? kF8Acc1 : 0), acc ? 0 : 7, half, q, lane,
-                                turn, p.timeout_ns, [&] {
-                                    tc_fence_before();
-                                    __syncwarp();
-                                    if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar, lead));
-                                });
+            finish_unit<OUT>(w, out, stg, p.work.pairs > 1 ? sums : nullptr, tmem + (acc ? kF8Acc1 : 0), acc ? 0 : 7, half, q, lane, turn, [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_pair(mapa_shared(tempty_bar, lead));
+            });
             tc_fence_before();
         }
     }
     if (p.work.pairs > 1) {
         __syncthreads();
         cluster_sync_all();
-        if (epilogue) finish_shared<OUT, 2>(p.work, work_unit(p.work, cluster_id, part), out, stg, sums, part, half, q, lane, turn);
+        if (epilogue) finish_shared<OUT>(p.work, work_unit(p.work, cluster_id, part), out, stg, sums, part, half, q, lane, turn);
     }
     if (epilogue && p.c_tma && lane == 0) bulk_wait_group_all();
 

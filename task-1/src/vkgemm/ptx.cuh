@@ -374,6 +374,32 @@ __device__ __forceinline__ void umma_commit(uint32_t bar)
                      : "memory");
 }
 
+// The same on the barriers at this offset in both CTAs of a pair, whose even rank is `lead`.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint32_t lead)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"(static_cast<uint16_t>(3u << lead))
+                 : "memory");
+}
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
+// mbar_wait by a whole warp, with one answer.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, uint64_t timeout_ns, uint32_t code, uint32_t detail)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, timeout_ns, code, detail));
+}
+
 // 32 lanes x 32 consecutive 32-bit columns: thread i of the warp receives lane (base + i).
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32])
 {

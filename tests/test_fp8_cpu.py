@@ -97,22 +97,6 @@ def test_workspace_size():
     assert vk.lib.vk_rmsnorm_fp8_workspace(4, 8, None) == BAD
 
 
-@pytest.mark.parametrize("name", ["gemm_fp8", "wgrad_fp8"])
-def test_product_workspace(name):
-    """A workspace is optional; one that is too small or unaligned is refused."""
-    query = getattr(vk.lib, f"vk_{name}_workspace")
-    n = ctypes.c_size_t(0)
-    assert query(4, 8, 8, ctypes.byref(n)) == vk.VK_OK and n.value > 0
-    need = n.value
-    assert query(0, 8, 8, ctypes.byref(n)) == vk.VK_OK and n.value == 0
-    assert query(-1, 8, 8, ctypes.byref(n)) == BAD
-    assert query(4, 1 << 31, 8, ctypes.byref(n)) == UNSUPPORTED
-    assert query(4, 8, 8, None) == BAD
-    for bad in (dict(workspace=P, workspace_bytes=need - 1), dict(workspace=P + 8, workspace_bytes=need)):
-        assert _call(name, **{**_good(name), **bad}) == BAD
-        assert "workspace" in vk.last_error()
-
-
 def test_cpu_tensors_are_refused():
     x = torch.zeros(4, 128, dtype=torch.bfloat16)
     w = torch.zeros(128, dtype=torch.bfloat16)

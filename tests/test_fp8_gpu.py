@@ -326,6 +326,14 @@ def test_gemm(vk, shape, layout, out):
     _check_product(c, av @ bv, av.abs() @ bv.abs(), k)
 
 
+# more tiles than the GPU has pairs of SMs: whole tiles only (6 x 13 = 78: halves of 4), a half-full wave (10 x 11: 36 halved),
+# most of a wave (12 x 12), a second wave of one tile (15 x 5), each with ragged edges
+@pytest.mark.parametrize("shape", [(1400, 3300, 300), (2500, 2700, 600), (3000, 2900, 1200), (3800, 1100, 2100)])
+@pytest.mark.parametrize("layout", ["nt_tile", "nt_row", "nn"])
+def test_gemm_waves(vk, shape, layout):
+    test_gemm(vk, shape, layout, BF16)
+
+
 @pytest.mark.parametrize("m", [4, 200])
 def test_gemm_tile_scales_of_a(vk, m):
     a, sa = _quantized((m, 1000), 32, True)
@@ -421,6 +429,12 @@ def test_wgrad(vk, shape, dtype, out):
     base = _rand((n, k), out or dtype, 42)
     acc = vk.wgrad_fp8(dy, x, sx, base.clone(), accumulate=True)
     _check_product(acc, d @ xv, d.abs() @ xv.abs(), t, base)
+
+
+@pytest.mark.parametrize("shape", [(300, 1400, 3300), (600, 2504, 2700), (1200, 3000, 2900), (1100, 3800, 1100)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_wgrad_waves(vk, shape, dtype):
+    test_wgrad(vk, shape, dtype, None)
 
 
 @pytest.mark.parametrize("lead,tail", [(1, 2), (16, 16)])

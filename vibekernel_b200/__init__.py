@@ -44,7 +44,7 @@ EXPORTED = (
     "vk_copy_async", "vk_debug_schedule", "vk_gemm_peers", "vk_gemm_mc", "vk_mc_supported", "vk_mc_alloc",
     "vk_mc_free", "vk_mc_create", "vk_mc_import", "vk_mc_attach", "vk_mc_detach", "vk_debug_watchdog",
     "vk_quantize_fp8", "vk_rmsnorm_fp8", "vk_rmsnorm_fp8_workspace", "vk_rmsnorm_fp8_backward", "vk_gemm_fp8",
-    "vk_wgrad_fp8", "vk_gemm_fp8_workspace", "vk_wgrad_fp8_workspace",
+    "vk_wgrad_fp8",
 )
 
 
@@ -119,8 +119,7 @@ class GemmFp8Args(ctypes.Structure):
     _fields_ = [
         ("A", _P), ("B", _P), ("a_scale", _P), ("b_scale", _P), ("C", _P), ("m", _I64), ("n", _I64), ("k", _I64),
         ("lda", _I64), ("ldb", _I64), ("ldc", _I64), ("ld_a_scale", _I64), ("ld_b_scale", _I64), ("a_scaling", _I32),
-        ("b_scaling", _I32), ("trans_b", _I32), ("dtype", _I32), ("workspace", _P), ("workspace_bytes", ctypes.c_size_t),
-        ("stream", _P),
+        ("b_scaling", _I32), ("trans_b", _I32), ("dtype", _I32), ("stream", _P),
     ]
 
 
@@ -128,7 +127,7 @@ class WgradFp8Args(ctypes.Structure):
     _fields_ = [
         ("dY", _P), ("X", _P), ("x_scale", _P), ("dW", _P), ("tokens", _I64), ("n", _I64), ("k", _I64), ("lddy", _I64),
         ("ldx", _I64), ("ld_x_scale", _I64), ("lddw", _I64), ("dtype", _I32), ("out_dtype", _I32), ("accumulate", _I32),
-        ("workspace", _P), ("workspace_bytes", ctypes.c_size_t), ("stream", _P),
+        ("stream", _P),
     ]
 
 
@@ -213,10 +212,6 @@ def _load() -> ctypes.CDLL:
                        ("rmsnorm_fp8_backward", RmsnormFp8BackwardArgs), ("wgrad_fp8", WgradFp8Args)):
         fn = getattr(lib, "vk_" + name)
         fn.argtypes = [ctypes.POINTER(args)]
-        fn.restype = ctypes.c_int
-    for name in ("gemm_fp8", "wgrad_fp8"):
-        fn = getattr(lib, f"vk_{name}_workspace")
-        fn.argtypes = [_I64, _I64, _I64, ctypes.POINTER(ctypes.c_size_t)]
         fn.restype = ctypes.c_int
     lib.vk_rmsnorm_fp8_workspace.argtypes = [_I64, _I64, ctypes.POINTER(ctypes.c_size_t)]
     lib.vk_rmsnorm_fp8_workspace.restype = ctypes.c_int
@@ -750,6 +745,8 @@ def rmsnorm_fp8_backward(dy, h, weight, rstd, *, dres=None, dx=None, dweight=Non
     if dres is not None:
         a.ld_dres = _matrix(dres, "dres", (rows, cols), (dy.dtype,), dev)
         a.dres = dres.data_ptr()
+    need = ctypes.c_size_t(0)
+    check(lib.vk_rmsnorm_fp8_workspace(rows, cols, ctypes.byref(need)))
     with _On(dev, stream) as handle:
         if dx is None:
             dx = torch.empty((rows, cols), dtype=dy.dtype, device=dev)
@@ -757,21 +754,14 @@ def rmsnorm_fp8_backward(dy, h, weight, rstd, *, dres=None, dx=None, dweight=Non
             dweight = torch.empty((cols,), dtype=torch.float32, device=dev)
         a.lddx = _matrix(dx, "dx", (rows, cols), (dy.dtype,), dev)
         _vector(dweight, "dweight", cols, torch.float32, dev)
-        work = _workspace(lib.vk_rmsnorm_fp8_workspace, rows, cols, device=dev)
+        # from torch's allocator for this stream, so that a captured graph keeps it
+        work = torch.empty((need.value,), dtype=torch.uint8, device=dev)
         a.dY, a.H, a.weight, a.rstd = dy.data_ptr(), h.data_ptr(), weight.data_ptr(), rstd.data_ptr()
-        a.dX, a.dweight, a.workspace, a.workspace_bytes = dx.data_ptr(), dweight.data_ptr(), work.data_ptr(), work.numel()
+        a.dX, a.dweight, a.workspace, a.workspace_bytes = dx.data_ptr(), dweight.data_ptr(), work.data_ptr(), need.value
         a.rows, a.cols = rows, cols
         a.stream = handle
         check(lib.vk_rmsnorm_fp8_backward(ctypes.byref(a)))
     return dx, dweight
-
-
-def _workspace(query, *sizes, device):
-    """A call's own workspace: from torch's allocator for the current stream, so that captured graphs keep it."""
-    import torch
-    need = ctypes.c_size_t(0)
-    check(query(*sizes, ctypes.byref(need)))
-    return torch.empty((need.value,), dtype=torch.uint8, device=device)
 
 
 def _scaling(scale, rows: int, cols: int, what: str, device):
@@ -819,8 +809,6 @@ def gemm_fp8(A, a_scale, B, b_scale, C=None, *, trans_b: bool = False, out_dtype
         a.A, a.B, a.a_scale, a.b_scale, a.C = A.data_ptr(), B.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), C.data_ptr()
         a.m, a.n, a.k = m, n, k
         a.trans_b = int(bool(trans_b))
-        work = _workspace(lib.vk_gemm_fp8_workspace, m, n, k, device=dev)
-        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
         a.stream = handle
         check(lib.vk_gemm_fp8(ctypes.byref(a)))
     return C
@@ -858,8 +846,6 @@ def wgrad_fp8(dY, X, x_scale, dW=None, *, accumulate: bool = False, out_dtype=No
         a.dY, a.X, a.x_scale, a.dW = dY.data_ptr(), X.data_ptr(), x_scale.data_ptr(), dW.data_ptr()
         a.tokens, a.n, a.k = tokens, n, k
         a.accumulate = int(bool(accumulate))
-        work = _workspace(lib.vk_wgrad_fp8_workspace, tokens, n, k, device=dev)
-        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
         a.stream = handle
         check(lib.vk_wgrad_fp8(ctypes.byref(a)))
     return dW
