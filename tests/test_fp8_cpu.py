@@ -126,6 +126,18 @@ def test_structures_match_the_header(tmp_path):
     assert got == want
 
 
+def test_packed_arguments_match_the_structures():
+    """The Python calls pack their arguments with struct formats: the same size and offsets as the structures."""
+    import struct
+    for name, fmt in vk._FP8_STRUCTS.items():
+        cls = {"quantize_fp8": vk.QuantizeFp8Args, "rmsnorm_fp8": vk.RmsnormFp8Args, "gemm_fp8": vk.GemmFp8Args,
+               "rmsnorm_fp8_backward": vk.RmsnormFp8BackwardArgs, "wgrad_fp8": vk.WgradFp8Args}[name]
+        assert struct.calcsize(fmt) == ctypes.sizeof(cls), name
+        fields = [f for f, _ in cls._fields_]
+        got = cls.from_buffer_copy(struct.pack(fmt, *range(1, len(fields) + 1)))
+        assert [getattr(got, f) for f in fields] == list(range(1, len(fields) + 1)), name
+
+
 def test_oracle_form_agrees_with_torch():
     codes = torch.arange(256, dtype=torch.uint8)
     np.testing.assert_array_equal(fp8.E4M3, codes.view(torch.float8_e4m3fn).double().numpy())

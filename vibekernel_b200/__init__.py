@@ -582,72 +582,95 @@ def row_blocks(m: int, parts: int):
 # ------------------------------------------------------------------------------------------
 # 8-bit linear layer
 # ------------------------------------------------------------------------------------------
-def _fp8_types():
-    import torch
-    return {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32, "q": torch.float8_e4m3fn,
-            "scale": torch.float8_e8m0fnu}
+class _Fp8:
+    """What the calls below need of torch, looked up once: a small call's time is mostly the host's."""
 
+    def __init__(self):
+        import struct
 
-def _dtype_code(t, *, f32: bool, what: str) -> int:
-    import torch
-    code = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32 if f32 else None}.get(t)
-    if code is None:
-        raise TypeError(f"{what} must be float16{', bfloat16 or float32' if f32 else ' or bfloat16'}, not {t}")
-    return code
-
-
-def _matrix(t, what: str, shape=None, dtypes=None, device=None) -> int:
-    """Checks a row-major CUDA matrix and returns its row pitch in elements."""
-    if not t.is_cuda:
-        raise ValueError(f"{what} must be a CUDA tensor (no CPU fallback)")
-    if t.dim() != 2 or not _unit_col(t):
-        raise ValueError(f"{what} must be 2-D with unit column stride")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what} must be {tuple(shape)}, not {tuple(t.shape)}")
-    if dtypes is not None and t.dtype not in dtypes:
-        raise TypeError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{what} is on {t.device}, not on {device}")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{what} must not have overlapping rows")
-    return max(_row_pitch(t), 1)
-
-
-def _vector(t, what: str, n: int, dtype, device) -> None:
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or t.device != device:
-        raise ValueError(f"{what} must be a contiguous {dtype} vector of length {n} on {device}")
-
-
-class _On:
-    """The device of a call's tensors made current, and the stream it runs on: allocations inside belong to that stream."""
-
-    def __init__(self, device, stream):
         import torch
-        self.device = device
-        self.guards = []
-        if torch.cuda.current_device() != device.index:
-            self.guards.append(torch.cuda.device(device))
+        self.torch = torch
+        self.empty = torch.empty
+        self.codes16 = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+        self.codes = {**self.codes16, torch.float32: DTYPE_F32}
+        self.f16, self.f32, self.u8 = torch.float16, torch.float32, torch.uint8
+        self.q, self.scale = torch.float8_e4m3fn, torch.float8_e8m0fnu
+        self.current_device = torch.cuda.current_device
+        self.raw_stream = torch._C._cuda_getCurrentRawStream
+        # the argument structures of include/vkgemm.h, packed in one call each
+        for name, fmt in _FP8_STRUCTS.items():
+            fn = lib["vk_" + name]
+            fn.argtypes = [ctypes.c_char_p]
+            fn.restype = ctypes.c_int
+            setattr(self, name, (fn, struct.Struct(fmt).pack))
+
+
+_FP8_STRUCTS = {"quantize_fp8": "3P5q2iP", "rmsnorm_fp8": "7P7qfiP", "rmsnorm_fp8_backward": "8PN6qiP", "gemm_fp8": "5P8q4iP",
+                "wgrad_fp8": "4P7q3iP"}
+_fp8_cache = None
+
+
+def _fp8():
+    global _fp8_cache
+    if _fp8_cache is None:
+        _fp8_cache = _Fp8()
+    return _fp8_cache
+
+
+def _elsewhere(F, t, stream):
+    """Guards for a call on another device than the current one or on a given stream (allocations inside belong to that
+    stream); None when there is nothing to do."""
+    index = t.get_device()
+    if stream is None and (index < 0 or index == F.current_device()):
+        return None
+    import contextlib
+    guard = contextlib.ExitStack()
+    if index >= 0:
+        guard.enter_context(F.torch.cuda.device(index))
         if stream is not None:
             if not hasattr(stream, "cuda_stream"):
-                stream = torch.cuda.ExternalStream(int(stream), device=device) if int(stream) else torch.cuda.default_stream(device)
-            self.guards.append(torch.cuda.stream(stream))
-
-    def __enter__(self):
-        import torch
-        for g in self.guards:
-            g.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream or None
-
-    def __exit__(self, *exc):
-        for g in reversed(self.guards):
-            g.__exit__(*exc)
+                stream = F.torch.cuda.ExternalStream(int(stream), device=t.device) if int(stream) else F.torch.cuda.default_stream(t.device)
+            guard.enter_context(F.torch.cuda.stream(stream))
+    return guard
 
 
-def _empty_fp8(rows: int, cols: int, device):
+def _matrix(t, what: str, device: int | None = None, dtype=None, shape=None):
+    """Checks a row-major CUDA matrix; returns (rows, columns, row pitch in elements)."""
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{what} must be a CUDA tensor (no CPU fallback)")
+    if device is not None and index != device:
+        raise ValueError(f"{what} is on cuda:{index}, not on cuda:{device}")
+    if dtype is not None and t.dtype is not dtype:
+        raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be 2-D with unit column stride")
+    rows, cols = t.shape
+    pitch, unit = t.stride()
+    if unit != 1 and cols > 1:
+        raise ValueError(f"{what} must be 2-D with unit column stride")
+    if shape is not None and (rows, cols) != shape:
+        raise ValueError(f"{what} must be {shape}, not {(rows, cols)}")
+    if rows > 1:
+        if pitch < cols:
+            raise ValueError(f"{what} must not have overlapping rows")
+    else:
+        pitch = cols
+    return rows, cols, pitch or 1
+
+
+def _vector(t, what: str, device: int, dtype, n: int) -> int:
+    """Checks a contiguous vector; returns its address."""
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or t.get_device() != device:
+        raise ValueError(f"{what} must be a contiguous {dtype} vector of length {n} on cuda:{device}")
+    return t.data_ptr()
+
+
+def _new_q(F, rows: int, cols: int, device):
     """A new 8-bit matrix whose rows start at 16-byte boundaries (what the tensor-core kernels' loads need)."""
-    import torch
-    q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)
-    return q if q.shape[1] == cols else q[:, :cols]
+    pitch = (cols + 15) // 16 * 16
+    q = F.empty((rows, pitch), dtype=F.q, device=device)
+    return q if pitch == cols else q[:, :cols]
 
 
 def quantize_fp8(x, *, tile: bool = False, q=None, scale=None, stream=None):
@@ -660,25 +683,31 @@ def quantize_fp8(x, *, tile: bool = False, q=None, scale=None, stream=None):
     same form serves the product with W^T and the one with W).  The value of an element is q * scale; a block with an
     infinity or a NaN becomes NaN.  Asynchronous on ``stream`` (default: torch's current stream).
     """
-    import torch
-    T = _fp8_types()
-    a = QuantizeFp8Args()
-    a.dtype = _dtype_code(x.dtype, f32=True, what="x")
-    a.ldx = _matrix(x, "x")
-    rows, cols = x.shape
+    F = _fp8()
+    guard = _elsewhere(F, x, stream)
+    if guard is not None:
+        with guard:
+            return quantize_fp8(x, tile=tile, q=q, scale=scale)
+    code = F.codes.get(x.dtype)
+    if code is None:
+        raise TypeError(f"x must be float16, bfloat16 or float32, not {x.dtype}")
+    rows, cols, ldx = _matrix(x, "x")
+    device = x.device
+    index = device.index
     s_shape = ((rows + 127) // 128 if tile else rows, (cols + 127) // 128)
-    with _On(x.device, stream) as handle:
-        if q is None:
-            q = _empty_fp8(rows, cols, x.device)
-        if scale is None:
-            scale = torch.empty(s_shape, dtype=T["scale"], device=x.device)
-        a.ldq = _matrix(q, "q", (rows, cols), (T["q"],), x.device)
-        a.ld_scale = _matrix(scale, "scale", s_shape, (T["scale"],), x.device)
-        a.X, a.Q, a.scale = x.data_ptr(), q.data_ptr(), scale.data_ptr()
-        a.rows, a.cols = rows, cols
-        a.scaling = FP8_TILE if tile else FP8_ROW
-        a.stream = handle
-        check(lib.vk_quantize_fp8(ctypes.byref(a)))
+    if q is None:
+        q = _new_q(F, rows, cols, device)
+        ldq = (cols + 15) // 16 * 16
+    else:
+        ldq = _matrix(q, "q", index, F.q, (rows, cols))[2]
+    if scale is None:
+        scale = F.empty(s_shape, dtype=F.scale, device=device)
+        lds = s_shape[1]
+    else:
+        lds = _matrix(scale, "scale", index, F.scale, s_shape)[2]
+    fn, pack = F.quantize_fp8
+    check(fn(pack(x.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, cols, ldx, ldq, lds, code, FP8_TILE if tile else FP8_ROW,
+                  F.raw_stream(index))))
     return q, scale
 
 
@@ -690,39 +719,51 @@ def rmsnorm_fp8(x, weight, *, residual=None, eps: float = 1e-6, q=None, scale=No
     [rows, cols], float16 or bfloat16, weight a vector of the same type.  ``h`` may be x or residual itself (in place).
     Outputs that are not given are allocated.
     """
-    import torch
-    T = _fp8_types()
-    a = RmsnormFp8Args()
-    a.dtype = _dtype_code(x.dtype, f32=False, what="x")
-    a.ldx = _matrix(x, "x")
-    rows, cols = x.shape
-    dev = x.device
-    _vector(weight, "weight", cols, x.dtype, dev)
-    s_shape = (rows, (cols + 127) // 128)
-    with _On(dev, stream) as handle:
-        if residual is not None:
-            a.ld_residual = _matrix(residual, "residual", (rows, cols), (x.dtype,), dev)
-            if h is None:
-                h = torch.empty((rows, cols), dtype=x.dtype, device=dev)
-            a.ldh = _matrix(h, "h", (rows, cols), (x.dtype,), dev)
-            a.residual, a.H = residual.data_ptr(), h.data_ptr()
-        elif h is not None:
-            raise ValueError("h is given with a residual only (without one it is x)")
+    F = _fp8()
+    guard = _elsewhere(F, x, stream)
+    if guard is not None:
+        with guard:
+            return rmsnorm_fp8(x, weight, residual=residual, eps=eps, q=q, scale=scale, h=h, rstd=rstd)
+    dtype = x.dtype
+    code = F.codes16.get(dtype)
+    if code is None:
+        raise TypeError(f"x must be float16 or bfloat16, not {dtype}")
+    rows, cols, ldx = _matrix(x, "x")
+    device = x.device
+    index = device.index
+    w_ptr = _vector(weight, "weight", index, dtype, cols)
+    blocks = (cols + 127) // 128
+    r_ptr = h_ptr = ldr = ldh = 0
+    if residual is not None:
+        ldr = _matrix(residual, "residual", index, dtype, (rows, cols))[2]
+        if h is None:
+            h = F.empty((rows, cols), dtype=dtype, device=device)
+            ldh = cols
         else:
-            h = x
-        if q is None:
-            q = _empty_fp8(rows, cols, dev)
-        if scale is None:
-            scale = torch.empty(s_shape, dtype=T["scale"], device=dev)
-        if rstd is None:
-            rstd = torch.empty((rows,), dtype=torch.float32, device=dev)
-        a.ldq = _matrix(q, "q", (rows, cols), (T["q"],), dev)
-        a.ld_scale = _matrix(scale, "scale", s_shape, (T["scale"],), dev)
-        _vector(rstd, "rstd", rows, torch.float32, dev)
-        a.X, a.weight, a.Q, a.scale, a.rstd = x.data_ptr(), weight.data_ptr(), q.data_ptr(), scale.data_ptr(), rstd.data_ptr()
-        a.rows, a.cols, a.eps = rows, cols, eps
-        a.stream = handle
-        check(lib.vk_rmsnorm_fp8(ctypes.byref(a)))
+            ldh = _matrix(h, "h", index, dtype, (rows, cols))[2]
+        r_ptr, h_ptr = residual.data_ptr(), h.data_ptr()
+    elif h is not None:
+        raise ValueError("h is given with a residual only (without one it is x)")
+    else:
+        h = x
+    if q is None:
+        q = _new_q(F, rows, cols, device)
+        ldq = (cols + 15) // 16 * 16
+    else:
+        ldq = _matrix(q, "q", index, F.q, (rows, cols))[2]
+    if scale is None:
+        scale = F.empty((rows, blocks), dtype=F.scale, device=device)
+        lds = blocks
+    else:
+        lds = _matrix(scale, "scale", index, F.scale, (rows, blocks))[2]
+    if rstd is None:
+        rstd = F.empty((rows,), dtype=F.f32, device=device)
+        rstd_ptr = rstd.data_ptr()
+    else:
+        rstd_ptr = _vector(rstd, "rstd", index, F.f32, rows)
+    fn, pack = F.rmsnorm_fp8
+    check(fn(pack(x.data_ptr(), r_ptr, w_ptr, q.data_ptr(), scale.data_ptr(), h_ptr, rstd_ptr, rows, cols, ldx, ldr, ldq, lds, ldh,
+                  eps, code, F.raw_stream(index))))
     return q, scale, h, rstd
 
 
@@ -733,47 +774,55 @@ def rmsnorm_fp8_backward(dy, h, weight, rstd, *, dres=None, dx=None, dweight=Non
     what the forward pass returned, dres (optional) is the gradient that reaches h from elsewhere.  dx, in dy's type,
     is the gradient of x and of the residual alike and may be dy or dres itself; dweight is float32.
     """
-    import torch
-    a = RmsnormFp8BackwardArgs()
-    a.dtype = _dtype_code(dy.dtype, f32=False, what="dy")
-    a.lddy = _matrix(dy, "dy")
-    rows, cols = dy.shape
-    dev = dy.device
-    a.ldh = _matrix(h, "h", (rows, cols), (dy.dtype,), dev)
-    _vector(weight, "weight", cols, dy.dtype, dev)
-    _vector(rstd, "rstd", rows, torch.float32, dev)
+    F = _fp8()
+    guard = _elsewhere(F, dy, stream)
+    if guard is not None:
+        with guard:
+            return rmsnorm_fp8_backward(dy, h, weight, rstd, dres=dres, dx=dx, dweight=dweight)
+    dtype = dy.dtype
+    code = F.codes16.get(dtype)
+    if code is None:
+        raise TypeError(f"dy must be float16 or bfloat16, not {dtype}")
+    rows, cols, lddy = _matrix(dy, "dy")
+    device = dy.device
+    index = device.index
+    ldh = _matrix(h, "h", index, dtype, (rows, cols))[2]
+    w_ptr = _vector(weight, "weight", index, dtype, cols)
+    rstd_ptr = _vector(rstd, "rstd", index, F.f32, rows)
+    dres_ptr = ldr = 0
     if dres is not None:
-        a.ld_dres = _matrix(dres, "dres", (rows, cols), (dy.dtype,), dev)
-        a.dres = dres.data_ptr()
+        ldr = _matrix(dres, "dres", index, dtype, (rows, cols))[2]
+        dres_ptr = dres.data_ptr()
+    if dx is None:
+        dx = F.empty((rows, cols), dtype=dtype, device=device)
+        lddx = cols
+    else:
+        lddx = _matrix(dx, "dx", index, dtype, (rows, cols))[2]
+    if dweight is None:
+        dweight = F.empty((cols,), dtype=F.f32, device=device)
+        dw_ptr = dweight.data_ptr()
+    else:
+        dw_ptr = _vector(dweight, "dweight", index, F.f32, cols)
     need = ctypes.c_size_t(0)
     check(lib.vk_rmsnorm_fp8_workspace(rows, cols, ctypes.byref(need)))
-    with _On(dev, stream) as handle:
-        if dx is None:
-            dx = torch.empty((rows, cols), dtype=dy.dtype, device=dev)
-        if dweight is None:
-            dweight = torch.empty((cols,), dtype=torch.float32, device=dev)
-        a.lddx = _matrix(dx, "dx", (rows, cols), (dy.dtype,), dev)
-        _vector(dweight, "dweight", cols, torch.float32, dev)
-        # from torch's allocator for this stream, so that a captured graph keeps it
-        work = torch.empty((need.value,), dtype=torch.uint8, device=dev)
-        a.dY, a.H, a.weight, a.rstd = dy.data_ptr(), h.data_ptr(), weight.data_ptr(), rstd.data_ptr()
-        a.dX, a.dweight, a.workspace, a.workspace_bytes = dx.data_ptr(), dweight.data_ptr(), work.data_ptr(), need.value
-        a.rows, a.cols = rows, cols
-        a.stream = handle
-        check(lib.vk_rmsnorm_fp8_backward(ctypes.byref(a)))
+    # from torch's allocator for this stream, so that a captured graph keeps it
+    work = F.empty((need.value,), dtype=F.u8, device=device)
+    fn, pack = F.rmsnorm_fp8_backward
+    check(fn(pack(dy.data_ptr(), h.data_ptr(), w_ptr, rstd_ptr, dres_ptr, dx.data_ptr(), dw_ptr, work.data_ptr(), need.value, rows, cols,
+                  lddy, ldh, ldr, lddx, code, F.raw_stream(index))))
     return dx, dweight
 
 
-def _scaling(scale, rows: int, cols: int, what: str, device):
+def _scaling(F, scale, rows: int, cols: int, what: str, device: int):
     """(vk_fp8_scaling, pitch) of the scales of a [rows, cols] matrix, told by their shape."""
-    T = _fp8_types()
+    s_rows, s_cols, pitch = _matrix(scale, what, device, F.scale)
     blocks = (cols + 127) // 128
-    ld = _matrix(scale, what, None, (T["scale"],), device)
-    if tuple(scale.shape) == (rows, blocks):
-        return FP8_ROW, ld
-    if tuple(scale.shape) == ((rows + 127) // 128, blocks):
-        return FP8_TILE, ld
-    raise ValueError(f"{what} must be {(rows, blocks)} or {((rows + 127) // 128, blocks)}, not {tuple(scale.shape)}")
+    if s_cols == blocks:
+        if s_rows == rows:
+            return FP8_ROW, pitch
+        if s_rows == (rows + 127) // 128:
+            return FP8_TILE, pitch
+    raise ValueError(f"{what} must be {(rows, blocks)} or {((rows + 127) // 128, blocks)}, not {(s_rows, s_cols)}")
 
 
 def gemm_fp8(A, a_scale, B, b_scale, C=None, *, trans_b: bool = False, out_dtype=None, stream=None):
@@ -784,33 +833,35 @@ def gemm_fp8(A, a_scale, B, b_scale, C=None, *, trans_b: bool = False, out_dtype
     is stored [k, n] needs tile scales.  C is [m, n] in ``out_dtype`` (default float16; bfloat16 and float32 too).
     Operands whose rows start at 16-byte boundaries run on the tensor cores; any others on a slow kernel.
     """
-    import torch
-    T = _fp8_types()
-    a = GemmFp8Args()
-    a.lda = _matrix(A, "A", None, (T["q"],))
-    dev = A.device
-    a.ldb = _matrix(B, "B", None, (T["q"],), dev)
-    m, k = A.shape
-    n, kb = (B.shape[0], B.shape[1]) if trans_b else (B.shape[1], B.shape[0])
+    F = _fp8()
+    guard = _elsewhere(F, A, stream)
+    if guard is not None:
+        with guard:
+            return gemm_fp8(A, a_scale, B, b_scale, C, trans_b=trans_b, out_dtype=out_dtype)
+    m, k, lda = _matrix(A, "A", None, F.q)
+    device = A.device
+    index = device.index
+    b_rows, b_cols, ldb = _matrix(B, "B", index, F.q)
+    n, kb = (b_rows, b_cols) if trans_b else (b_cols, b_rows)
     if kb != k:
-        raise ValueError(f"A is {tuple(A.shape)} and B is {tuple(B.shape)} with trans_b={bool(trans_b)}")
-    a.a_scaling, a.ld_a_scale = _scaling(a_scale, m, k, "a_scale", dev)
-    a.b_scaling, a.ld_b_scale = _scaling(b_scale, B.shape[0], B.shape[1], "b_scale", dev)
-    if not trans_b and B.shape[0] == 1:
-        a.b_scaling = FP8_TILE  # one row: both forms are the same scales
-    if C is not None:
-        out_dtype = out_dtype or C.dtype
-    out_dtype = out_dtype or torch.float16
-    a.dtype = _dtype_code(out_dtype, f32=True, what="out_dtype")
-    with _On(dev, stream) as handle:
-        if C is None:
-            C = torch.empty((m, n), dtype=out_dtype, device=dev)
-        a.ldc = _matrix(C, "C", (m, n), (out_dtype,), dev)
-        a.A, a.B, a.a_scale, a.b_scale, a.C = A.data_ptr(), B.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), C.data_ptr()
-        a.m, a.n, a.k = m, n, k
-        a.trans_b = int(bool(trans_b))
-        a.stream = handle
-        check(lib.vk_gemm_fp8(ctypes.byref(a)))
+        raise ValueError(f"A is {(m, k)} and B is {(b_rows, b_cols)} with trans_b={bool(trans_b)}")
+    a_scaling, ldas = _scaling(F, a_scale, m, k, "a_scale", index)
+    b_scaling, ldbs = _scaling(F, b_scale, b_rows, b_cols, "b_scale", index)
+    if not trans_b and b_rows == 1:
+        b_scaling = FP8_TILE  # one row: both forms are the same scales
+    if out_dtype is None:
+        out_dtype = F.f16 if C is None else C.dtype
+    code = F.codes.get(out_dtype)
+    if code is None:
+        raise TypeError(f"out_dtype must be float16, bfloat16 or float32, not {out_dtype}")
+    if C is None:
+        C = F.empty((m, n), dtype=out_dtype, device=device)
+        ldc = n
+    else:
+        ldc = _matrix(C, "C", index, out_dtype, (m, n))[2]
+    fn, pack = F.gemm_fp8
+    check(fn(pack(A.data_ptr(), B.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), C.data_ptr(), m, n, k, lda, ldb, ldc, ldas, ldbs,
+                  a_scaling, b_scaling, 1 if trans_b else 0, code, F.raw_stream(index))))
     return C
 
 
@@ -821,31 +872,34 @@ def wgrad_fp8(dY, X, x_scale, dW=None, *, accumulate: bool = False, out_dtype=No
     (:func:`quantize_fp8`, or the output of :func:`rmsnorm_fp8`).  dW is [n, k] in ``out_dtype`` (default dY's type;
     float32 too), fp32 accumulation.  X's values enter the product in dY's type (exact in bfloat16).
     """
-    import torch
-    T = _fp8_types()
-    a = WgradFp8Args()
-    a.dtype = _dtype_code(dY.dtype, f32=False, what="dY")
-    a.lddy = _matrix(dY, "dY")
-    dev = dY.device
-    tokens, n = dY.shape
-    a.ldx = _matrix(X, "X", None, (T["q"],), dev)
-    if X.shape[0] != tokens:
-        raise ValueError(f"dY is {tuple(dY.shape)} and X is {tuple(X.shape)}")
-    k = X.shape[1]
-    a.ld_x_scale = _matrix(x_scale, "x_scale", (tokens, (k + 127) // 128), (T["scale"],), dev)
+    F = _fp8()
+    guard = _elsewhere(F, dY, stream)
+    if guard is not None:
+        with guard:
+            return wgrad_fp8(dY, X, x_scale, dW, accumulate=accumulate, out_dtype=out_dtype)
+    code = F.codes16.get(dY.dtype)
+    if code is None:
+        raise TypeError(f"dY must be float16 or bfloat16, not {dY.dtype}")
+    tokens, n, lddy = _matrix(dY, "dY")
+    device = dY.device
+    index = device.index
+    x_rows, k, ldx = _matrix(X, "X", index, F.q)
+    if x_rows != tokens:
+        raise ValueError(f"dY is {(tokens, n)} and X is {(x_rows, k)}")
+    ldxs = _matrix(x_scale, "x_scale", index, F.scale, (tokens, (k + 127) // 128))[2]
     if accumulate and dW is None:
         raise ValueError("accumulate needs dW")
-    if dW is not None:
-        out_dtype = out_dtype or dW.dtype
-    out_dtype = out_dtype or dY.dtype
-    a.out_dtype = _dtype_code(out_dtype, f32=True, what="out_dtype")
-    with _On(dev, stream) as handle:
-        if dW is None:
-            dW = torch.empty((n, k), dtype=out_dtype, device=dev)
-        a.lddw = _matrix(dW, "dW", (n, k), (out_dtype,), dev)
-        a.dY, a.X, a.x_scale, a.dW = dY.data_ptr(), X.data_ptr(), x_scale.data_ptr(), dW.data_ptr()
-        a.tokens, a.n, a.k = tokens, n, k
-        a.accumulate = int(bool(accumulate))
-        a.stream = handle
-        check(lib.vk_wgrad_fp8(ctypes.byref(a)))
+    if out_dtype is None:
+        out_dtype = dY.dtype if dW is None else dW.dtype
+    out_code = F.codes.get(out_dtype)
+    if out_code is None:
+        raise TypeError(f"out_dtype must be float16, bfloat16 or float32, not {out_dtype}")
+    if dW is None:
+        dW = F.empty((n, k), dtype=out_dtype, device=device)
+        lddw = k
+    else:
+        lddw = _matrix(dW, "dW", index, out_dtype, (n, k))[2]
+    fn, pack = F.wgrad_fp8
+    check(fn(pack(dY.data_ptr(), X.data_ptr(), x_scale.data_ptr(), dW.data_ptr(), tokens, n, k, lddy, ldx, ldxs, lddw, code, out_code,
+                  1 if accumulate else 0, F.raw_stream(index))))
     return dW
