@@ -244,20 +244,33 @@ extern "C" int vk_quantize_fp8(const vk_quantize_fp8_args* a)
     p.rows = a->rows;
     p.cols = static_cast<int>(a->cols);
     p.blocks = static_cast<int>(blocks);
-    p.vec_x = rows_at(a->X, p.ldx, bytes_of(a->dtype), 16);
-    p.vec_q = rows_at(a->Q, p.ldq, 1, 8);
+    const bool vec = rows_at(a->X, p.ldx, bytes_of(a->dtype), 16) && rows_at(a->Q, p.ldq, 1, 8) && a->cols % 8 == 0;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     if (a->scaling == VK_FP8_TILE) {
         const int64_t tiles = (a->rows + 127) / 128 * blocks;
         if (tiles > kMaxDim) return set_error(VK_ERR_UNSUPPORTED, "%s: too many tiles", name);
+        const unsigned grid = static_cast<unsigned>(tiles);
         return for_type(a->dtype, [&](auto t) {
-            quantize_tiles_kernel<decltype(t)><<<static_cast<unsigned>(tiles), 256, 0, stream>>>(p);
+            if (vec)
+                quantize_tiles_kernel<decltype(t), true><<<grid, 256, 0, stream>>>(p);
+            else
+                quantize_tiles_kernel<decltype(t), false><<<grid, 256, 0, stream>>>(p);
             return launched();
         });
     }
-    const int64_t need = (a->rows * blocks + 15) / 16, most = 148 * 32;
+    const int64_t need = (a->rows * blocks + 15) / 16;
     return for_type(a->dtype, [&](auto t) {
-        quantize_rows_kernel<decltype(t)><<<static_cast<unsigned>(need < most ? need : most), 256, 0, stream>>>(p);
+        // four blocks at a time once there are enough for every SM
+        if (vec && need >= 148 * 4 * 4) {
+            const int64_t most = 148 * 8, wanted = (need + 3) / 4;
+            quantize_rows_kernel<decltype(t), true, 4><<<static_cast<unsigned>(wanted < most ? wanted : most), 256, 0, stream>>>(p);
+        } else {
+            const unsigned grid = static_cast<unsigned>(need < 148 * 32 ? need : 148 * 32);
+            if (vec)
+                quantize_rows_kernel<decltype(t), true, 1><<<grid, 256, 0, stream>>>(p);
+            else
+                quantize_rows_kernel<decltype(t), false, 1><<<grid, 256, 0, stream>>>(p);
+        }
         return launched();
     });
 }
@@ -265,20 +278,20 @@ extern "C" int vk_quantize_fp8(const vk_quantize_fp8_args* a)
 // ------------------------------------------------------------------------------------------
 // RMS norm
 // ------------------------------------------------------------------------------------------
-template <typename T>
+template <typename T, bool VEC>
 static int launch_norm(const NormParams& p, int64_t rows, cudaStream_t stream)
 {
     const unsigned grid = static_cast<unsigned>(rows);
-    if (p.cols <= 1024)
-        rmsnorm_fp8_kernel<T, 128, 1><<<grid, 128, 0, stream>>>(p);
-    else if (p.cols <= 2048)
-        rmsnorm_fp8_kernel<T, 256, 1><<<grid, 256, 0, stream>>>(p);
-    else if (p.cols <= 4096)
-        rmsnorm_fp8_kernel<T, 256, 2><<<grid, 256, 0, stream>>>(p);
-    else if (p.cols <= 8192)
-        rmsnorm_fp8_kernel<T, 512, 2><<<grid, 512, 0, stream>>>(p);
+    const int vectors = (p.cols + 127) / 128 * 16;  // of 8 columns, whole blocks
+    auto threads = [&](int nv) { return static_cast<unsigned>(((vectors + nv - 1) / nv + 31) / 32 * 32); };
+    if (vectors <= 256)
+        rmsnorm_fp8_kernel<T, 1, VEC><<<grid, threads(1), 0, stream>>>(p);
+    else if (vectors <= 512)
+        rmsnorm_fp8_kernel<T, 2, VEC><<<grid, threads(2), 0, stream>>>(p);
+    else if (vectors <= 1024)
+        rmsnorm_fp8_kernel<T, 4, VEC><<<grid, threads(4), 0, stream>>>(p);
     else
-        rmsnorm_fp8_kernel<T, 512, 0><<<grid, 512, 0, stream>>>(p);
+        rmsnorm_fp8_kernel<T, 0, VEC><<<grid, 512, 0, stream>>>(p);
     return launched();
 }
 
@@ -315,17 +328,17 @@ extern "C" int vk_rmsnorm_fp8(const vk_rmsnorm_fp8_args* a)
     p.rstd = a->rstd;
     p.cols = static_cast<int>(a->cols);
     p.eps = a->eps;
-    p.vec_x = rows_at(a->X, p.ldx, 2, 16);
-    p.vec_r = rows_at(a->residual, p.ldr, 2, 16);
-    p.vec_w = aligned(a->weight, 16);
-    p.vec_q = rows_at(a->Q, p.ldq, 1, 8);
-    p.vec_h = rows_at(a->H, p.ldh, 2, 16);
+    const bool vec = rows_at(a->X, p.ldx, 2, 16) && (a->residual == nullptr || (rows_at(a->residual, p.ldr, 2, 16) && rows_at(a->H, p.ldh, 2, 16))) &&
+                     aligned(a->weight, 16) && rows_at(a->Q, p.ldq, 1, 8) && a->cols % 8 == 0;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
-    return a->dtype == VK_DTYPE_F16 ? launch_norm<__half>(p, a->rows, stream) : launch_norm<__nv_bfloat16>(p, a->rows, stream);
+    return for_type(a->dtype, [&](auto t) {
+        using T = std::conditional_t<std::is_same_v<decltype(t), __half>, __half, __nv_bfloat16>;
+        return vec ? launch_norm<T, true>(p, a->rows, stream) : launch_norm<T, false>(p, a->rows, stream);
+    });
 }
 
-// CTAs of the backward pass, each with a row of fp32 partial sums in the workspace: two per SM of B200.
-static int64_t norm_backward_parts(int64_t rows) { return rows < 296 ? rows : 296; }
+// CTAs of the backward pass, each with a row of fp32 partial sums in the workspace: one per SM of B200.
+static int64_t norm_backward_parts(int64_t rows) { return rows < 148 ? rows : 148; }
 
 extern "C" int vk_rmsnorm_fp8_workspace(int64_t rows, int64_t cols, size_t* bytes)
 {
@@ -337,19 +350,20 @@ extern "C" int vk_rmsnorm_fp8_workspace(int64_t rows, int64_t cols, size_t* byte
     return VK_OK;
 }
 
-template <typename T>
-static int launch_norm_backward(const NormBackParams& p, unsigned grid, cudaStream_t stream)
+// Shared memory that the rows in flight may take.
+constexpr int kNormBackBytes = 200 * 1024;
+
+template <typename T, int NV>
+static int launch_norm_backward(NormBackParams p, int id, unsigned grid, cudaStream_t stream)
 {
-    if (p.cols <= 1024)
-        rmsnorm_fp8_backward_kernel<T, 128, 1><<<grid, 128, 0, stream>>>(p);
-    else if (p.cols <= 2048)
-        rmsnorm_fp8_backward_kernel<T, 256, 1><<<grid, 256, 0, stream>>>(p);
-    else if (p.cols <= 4096)
-        rmsnorm_fp8_backward_kernel<T, 512, 1><<<grid, 512, 0, stream>>>(p);
-    else if (p.cols <= 8192)
-        rmsnorm_fp8_backward_kernel<T, 512, 2><<<grid, 512, 0, stream>>>(p);
-    else
-        rmsnorm_fp8_backward_kernel<T, 512, 0><<<grid, 512, 0, stream>>>(p);
+    const int pitch = (p.cols * 2 + 127) / 128 * 128;
+    int clusters[4];
+    const int rc = prepare_kernel(rmsnorm_fp8_backward_kernel<T, NV>, id, kNormBackBytes, 512, clusters);
+    if (rc != VK_OK) return rc;
+    p.stages = kNormBackBytes / (3 * pitch);
+    if (p.stages > 8) p.stages = 8;
+    const unsigned threads = static_cast<unsigned>(((p.cols / 8 + NV - 1) / NV + 31) / 32 * 32);
+    rmsnorm_fp8_backward_kernel<T, NV><<<grid, threads, p.stages * 3 * pitch, stream>>>(p);
     return launched();
 }
 
@@ -387,14 +401,20 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
     p.part = static_cast<float*>(a->workspace);
     p.rows = a->rows;
     p.cols = static_cast<int>(a->cols);
-    p.vec_dy = rows_at(a->dY, p.lddy, 2, 16);
-    p.vec_h = rows_at(a->H, p.ldh, 2, 16);
-    p.vec_w = aligned(a->weight, 16);
-    p.vec_dres = rows_at(a->dres, p.lddres, 2, 16);
-    p.vec_dx = rows_at(a->dX, p.lddx, 2, 16);
+    p.stages = 0;
+    p.timeout_ns = wait_timeout_ns();
+    const bool vec = rows_at(a->dY, p.lddy, 2, 16) && rows_at(a->H, p.ldh, 2, 16) && aligned(a->weight, 16) &&
+                     (a->dres == nullptr || rows_at(a->dres, p.lddres, 2, 16)) && rows_at(a->dX, p.lddx, 2, 16) && a->cols % 8 == 0;
     if (a->rows > 0) {
-        rc = a->dtype == VK_DTYPE_F16 ? launch_norm_backward<__half>(p, static_cast<unsigned>(parts), stream)
-                                      : launch_norm_backward<__nv_bfloat16>(p, static_cast<unsigned>(parts), stream);
+        const unsigned grid = static_cast<unsigned>(parts);
+        rc = for_type(a->dtype, [&](auto t) {
+            using T = std::conditional_t<std::is_same_v<decltype(t), __half>, __half, __nv_bfloat16>;
+            constexpr int kId = 9 + (std::is_same_v<T, __half> ? 0 : 2);
+            if (vec && p.cols <= 512 * 8) return launch_norm_backward<T, 1>(p, kId, grid, stream);
+            if (vec && p.cols <= 512 * 16) return launch_norm_backward<T, 2>(p, kId + 1, grid, stream);
+            rmsnorm_fp8_backward_any_kernel<T><<<grid, 512, 0, stream>>>(p);
+            return launched();
+        });
         if (rc != VK_OK) return rc;
     }
     norm_weight_grad_kernel<<<static_cast<unsigned>((a->cols + 31) / 32), 256, 0, stream>>>(

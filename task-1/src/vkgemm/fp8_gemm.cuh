@@ -182,7 +182,7 @@ __device__ __forceinline__ void store_box(const BoxOut& o, uint8_t* stg, int row
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int n = o.N - col - 8 * j;
-            const Vec8<T> v = load8(c + (n > 0 ? 8 * j : 0), n, o.c_tma);
+            const Vec8<T> v = o.c_tma && n >= 8 ? load8<true>(c + 8 * j, n) : load8<false>(c + (n > 0 ? 8 * j : 0), n);
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[8 * j + i] += to_f32(v.v[i]);
         }

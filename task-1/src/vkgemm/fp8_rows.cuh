@@ -14,6 +14,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include "ptx.cuh"
+
 namespace vk {
 
 template <typename T>
@@ -40,16 +42,17 @@ struct alignas(16) Vec8 {
     T v[8];
 };
 
-// n elements (1..8; the rest become zeros); `vec`: the address is 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ Vec8<T> load8(const T* src, int n, bool vec)
+// n elements (the rest become zeros).  VEC: n is at least 8 or at most 0, and the address is 16-byte aligned; then the
+// load is one predicated instruction, and several stay in flight together.
+template <bool VEC, typename T>
+__device__ __forceinline__ Vec8<T> load8(const T* src, int n)
 {
     Vec8<T> r;
-    if (vec && n >= 8) {
+    if constexpr (VEC) {
         const uint4* s = reinterpret_cast<const uint4*>(src);
         uint4* d = reinterpret_cast<uint4*>(&r);
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) d[i] = s[i];
+        for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) d[i] = n > 0 ? s[i] : make_uint4(0, 0, 0, 0);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) r.v[i] = i < n ? src[i] : from_f32<T>(0.f);
@@ -57,10 +60,11 @@ __device__ __forceinline__ Vec8<T> load8(const T* src, int n, bool vec)
     return r;
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* dst, const Vec8<T>& r, int n, bool vec)
+template <bool VEC, typename T>
+__device__ __forceinline__ void store8(T* dst, const Vec8<T>& r, int n)
 {
-    if (vec && n >= 8) {
+    if constexpr (VEC) {
+        if (n <= 0) return;
         const uint4* s = reinterpret_cast<const uint4*>(&r);
         uint4* d = reinterpret_cast<uint4*>(dst);
 #pragma unroll
@@ -98,15 +102,16 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
     return lo | (hi << 16);
 }
 
-// Eight values of a block with this scale as e4m3 bytes; n of them are written.
-__device__ __forceinline__ void store_q8(uint8_t* dst, const float (&f)[8], uint32_t s, int n, bool vec)
+// Eight values of a block with this scale as e4m3 bytes; n of them are written.  VEC as above, and 8-byte alignment.
+template <bool VEC>
+__device__ __forceinline__ void store_q8(uint8_t* dst, const float (&f)[8], uint32_t s, int n)
 {
     const float inv = inverse_scale(s);
     uint2 w;
     w.x = pack_e4m3(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
     w.y = pack_e4m3(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
-    if (vec && n >= 8) {
-        *reinterpret_cast<uint2*>(dst) = w;
+    if constexpr (VEC) {
+        if (n > 0) *reinterpret_cast<uint2*>(dst) = w;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -138,12 +143,12 @@ struct QuantParams {
     uint8_t* q;
     uint8_t* scale;
     long long rows, ldx, ldq, lds;
-    int cols, blocks;      // blocks of 128 in a row
-    int vec_x, vec_q;      // rows start at 16-byte (x) / 8-byte (q) boundaries
+    int cols, blocks;  // blocks of 128 in a row
 };
 
-// Blocks of 128 of one row: 16 lanes hold one block, 8 values each, and walk over the blocks of the whole matrix.
-template <typename T>
+// Blocks of 128 of one row: 16 lanes hold one block, 8 values each; UNROLL blocks at a time, so that as many loads are in
+// flight, and on over the whole matrix.
+template <typename T, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
 {
     const int sub = threadIdx.x & 15;
@@ -156,40 +161,46 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
     int blk = static_cast<int>(first % p.blocks);
     const T* x = static_cast<const T*>(p.x);
     // a warp's two halves leave the loop together: the shuffles below need every lane
-    for (long long at = first & ~1ll; at < total; at += step) {
-        const bool live = row < p.rows;
-        const int c = blk * 128 + sub * 8;
-        const int n = live ? p.cols - c : 0;
-        float f[8];
-        if (n > 0) {
-            const Vec8<T> v = load8(x + row * p.ldx + c, n, p.vec_x);
+    for (long long at = first & ~1ll; at < total; at += step * UNROLL) {
+        Vec8<T> v[UNROLL];
+        long long rows[UNROLL];
+        int blks[UNROLL];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = to_f32(v.v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = 0.f;
+        for (int j = 0; j < UNROLL; ++j) {
+            rows[j] = row;
+            blks[j] = blk;
+            const int c = blk * 128 + sub * 8;
+            const int n = row < p.rows ? p.cols - c : 0;
+            v[j] = load8<VEC>(x + (n > 0 ? row * p.ldx + c : 0), n);
+            row += drow;
+            blk += dblk;
+            if (blk >= p.blocks) {
+                blk -= p.blocks;
+                ++row;
+            }
         }
-        const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
-        if (n > 0) store_q8(p.q + row * p.ldq + c, f, s, n, p.vec_q);
-        if (live && sub == 0) p.scale[row * p.lds + blk] = static_cast<uint8_t>(s);
-        row += drow;
-        blk += dblk;
-        if (blk >= p.blocks) {
-            blk -= p.blocks;
-            ++row;
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j) {
+            const int c = blks[j] * 128 + sub * 8;
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = to_f32(v[j].v[i]);
+            const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
+            if (rows[j] >= p.rows) continue;
+            store_q8<VEC>(p.q + rows[j] * p.ldq + c, f, s, p.cols - c);
+            if (sub == 0) p.scale[rows[j] * p.lds + blks[j]] = static_cast<uint8_t>(s);
         }
     }
 }
 
 // One 128 x 128 tile per CTA, held in registers between its maximum and its rounding: 16 lanes per row, 16 rows at a time.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p)
 {
     __shared__ uint32_t tops[8];
     const long long tr = blockIdx.x / p.blocks;
     const int blk = static_cast<int>(blockIdx.x % p.blocks);
     const int c = blk * 128 + (threadIdx.x & 15) * 8;
-    const int n = p.cols - c;
     const long long row0 = tr * 128 + (threadIdx.x >> 4);
     const T* x = static_cast<const T*>(p.x);
     Vec8<T> v[8];
@@ -197,8 +208,8 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const long long row = row0 + 16 * j;
-        const bool in = n > 0 && row < p.rows;
-        v[j] = load8(x + (in ? row * p.ldx + c : 0), in ? n : 0, p.vec_x);
+        const int n = row < p.rows ? p.cols - c : 0;
+        v[j] = load8<VEC>(x + (n > 0 ? row * p.ldx + c : 0), n);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -214,11 +225,11 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const long long row = row0 + 16 * j;
-        if (n <= 0 || row >= p.rows) continue;
+        if (row >= p.rows) break;
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = to_f32(v[j].v[i]);
-        store_q8(p.q + row * p.ldq + c, f, s, n, p.vec_q);
+        store_q8<VEC>(p.q + row * p.ldq + c, f, s, p.cols - c);
     }
 }
 
@@ -226,7 +237,6 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p
 // RMS norm
 // ------------------------------------------------------------------------------------------
 // Sum over the CTA's threads, the same on all of them.  `slots` alternates between calls (one barrier each).
-template <int THREADS>
 __device__ __forceinline__ float cta_sum(float v, float* slots)
 {
 #pragma unroll
@@ -234,8 +244,7 @@ __device__ __forceinline__ float cta_sum(float v, float* slots)
     if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
     __syncthreads();
     float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) t += slots[w];
+    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) t += slots[w];
     return t;
 }
 
@@ -250,32 +259,39 @@ struct NormParams {
     long long ldx, ldr, ldq, lds, ldh;
     int cols;
     float eps;
-    int vec_x, vec_r, vec_w, vec_q, vec_h;
 };
 
-// One row per CTA; thread t holds the vectors of 8 at t, t + THREADS, ... (NV of them; NV = 0: any number, read again
-// from h for the second pass).  THREADS is a multiple of 16, so the 16 lanes of an aligned group hold one block.
-template <typename T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS) rmsnorm_fp8_kernel(const NormParams p)
+// One row per CTA; thread t holds the vectors of 8 at t, t + blockDim.x, ... (NV of them; NV = 0: any number, read again
+// from h for the second pass).  blockDim.x is a multiple of 32, so the 16 lanes of an aligned group hold one block.
+// VEC: rows and weight are aligned for 16-byte accesses (q: 8) and cols is a multiple of 8.
+template <typename T, int NV, bool VEC>
+__global__ void __launch_bounds__(NV == 0 ? 512 : 256) rmsnorm_fp8_kernel(const NormParams p)
 {
-    __shared__ float slots[THREADS / 32];
+    __shared__ float slots[16];
     constexpr int kHeld = NV > 0 ? NV : 1;
+    const int threads = blockDim.x;
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
     const T* w = static_cast<const T*>(p.weight);
     T* h = p.residual ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
-    const int vectors = (p.cols + 127) / 128 * 16;  // whole blocks
-    const int nv = NV > 0 ? NV : (vectors + THREADS - 1) / THREADS;
+    const int nv = NV > 0 ? NV : ((p.cols + 127) / 128 * 16 + threads - 1) / threads;
 
-    Vec8<T> held[kHeld], res[kHeld];
+    Vec8<T> held[kHeld], res[kHeld], gain[kHeld];
     float sq = 0.f;
-    auto first_pass = [&](Vec8<T>& a, const Vec8<T>& b, int c) {
-        const int n = p.cols - c;
-        if (r != nullptr && n > 0) {
+    auto load = [&](int j, int slot) {
+        const int c = (threadIdx.x + j * threads) * 8;
+        const int n = p.cols - c, o = n > 0 ? c : 0;
+        held[slot] = load8<VEC>(x + o, n);
+        if (r != nullptr) res[slot] = load8<VEC>(r + o, n);
+    };
+    auto first_pass = [&](int j, int slot) {
+        const int c = (threadIdx.x + j * threads) * 8;
+        Vec8<T>& a = held[slot];
+        if (r != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a.v[i] = from_f32<T>(to_f32(a.v[i]) + to_f32(b.v[i]));
-            store8(h + c, a, n, p.vec_h);
+            for (int i = 0; i < 8; ++i) a.v[i] = from_f32<T>(to_f32(a.v[i]) + to_f32(res[slot].v[i]));
+            store8<VEC>(h + c, a, p.cols - c);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -283,52 +299,47 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_fp8_kernel(const NormParams p
             sq = fmaf(f, f, sq);
         }
     };
-    if constexpr (NV > 0) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = (threadIdx.x + j * THREADS) * 8;
-            const int n = max(p.cols - c, 0);
-            held[j] = load8(x + (n ? c : 0), n, p.vec_x);
-            if (r != nullptr) res[j] = load8(r + (n ? c : 0), n, p.vec_r);
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) first_pass(held[j], res[j], (threadIdx.x + j * THREADS) * 8);
-    } else {
-        for (int j = 0; j < nv; ++j) {
-            const int c = (threadIdx.x + j * THREADS) * 8;
-            const int n = max(p.cols - c, 0);
-            held[0] = load8(x + (n ? c : 0), n, p.vec_x);
-            if (r != nullptr) res[0] = load8(r + (n ? c : 0), n, p.vec_r);
-            first_pass(held[0], res[0], c);
-        }
-    }
-    const float total = cta_sum<THREADS>(sq, slots);
-    const float rstd = 1.0f / sqrtf(total / static_cast<float>(p.cols) + p.eps);
-    if (threadIdx.x == 0) p.rstd[row] = rstd;
-
-    auto second_pass = [&](const Vec8<T>& a, int c) {
-        const int n = max(p.cols - c, 0);
-        const Vec8<T> g = load8(w + (n ? c : 0), n, p.vec_w);
+    auto load_gain = [&](int j, int slot) {
+        const int c = (threadIdx.x + j * threads) * 8;
+        gain[slot] = load8<VEC>(w + (c < p.cols ? c : 0), p.cols - c);
+    };
+    auto second_pass = [&](int j, int slot, float rstd) {
+        const int c = (threadIdx.x + j * threads) * 8;
         float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f32(a.v[i]) * rstd * to_f32(g.v[i]);
+        for (int i = 0; i < 8; ++i) f[i] = to_f32(held[slot].v[i]) * rstd * to_f32(gain[slot].v[i]);
         const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
-        if (n > 0) {
-            store_q8(p.q + row * p.ldq + c, f, s, n, p.vec_q);
+        if (c < p.cols) {
+            store_q8<VEC>(p.q + row * p.ldq + c, f, s, p.cols - c);
             if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + c / 128] = static_cast<uint8_t>(s);
         }
     };
     if constexpr (NV > 0) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) second_pass(held[j], (threadIdx.x + j * THREADS) * 8);
+        for (int j = 0; j < NV; ++j) load(j, j);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) load_gain(j, j);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) first_pass(j, j);
+    } else {
+        for (int j = 0; j < nv; ++j) {
+            load(j, 0);
+            first_pass(j, 0);
+        }
+    }
+    const float total = cta_sum(sq, slots);
+    const float rstd = 1.0f / sqrtf(total / static_cast<float>(p.cols) + p.eps);
+    if (threadIdx.x == 0) p.rstd[row] = rstd;
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) second_pass(j, j, rstd);
     } else {
         const T* src = r != nullptr ? h : x;  // this thread's own writes
-        const bool vec = r != nullptr ? p.vec_h : p.vec_x;
         for (int j = 0; j < nv; ++j) {
-            const int c = (threadIdx.x + j * THREADS) * 8;
-            const int n = max(p.cols - c, 0);
-            held[0] = load8(src + (n ? c : 0), n, vec);
-            second_pass(held[0], c);
+            const int c = (threadIdx.x + j * threads) * 8;
+            held[0] = load8<VEC>(src + (c < p.cols ? c : 0), p.cols - c);
+            load_gain(j, 0);
+            second_pass(j, 0, rstd);
         }
     }
 }
@@ -343,30 +354,20 @@ struct NormBackParams {
     float* part;       // [gridDim.x][cols] fp32: each CTA's share of dweight
     long long rows, lddy, ldh, lddres, lddx;
     int cols;
-    int vec_dy, vec_h, vec_w, vec_dres, vec_dx;
+    int stages;        // rows in flight (rmsnorm_fp8_backward_kernel)
+    unsigned long long timeout_ns;
 };
 
 // dx = rstd * (g - xhat * mean(g * xhat)) + dres with g = dy * weight, xhat = h * rstd; dweight = sum over rows of
-// dy * xhat.  CTAs walk over the rows; a thread keeps its columns' share of dweight in registers (NV > 0) or in its
-// CTA's row of `part` (NV = 0, any number of columns; each element belongs to one thread).
-template <typename T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS) rmsnorm_fp8_backward_kernel(const NormBackParams p)
+// dy * xhat.  CTAs walk over the rows.  Here, any alignment and any number of columns: a thread adds its columns' share
+// of dweight in its CTA's row of `part` (each element belongs to one thread), and reads a row twice.
+template <typename T>
+__global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const NormBackParams p)
 {
-    __shared__ float slots[2][THREADS / 32];
-    constexpr int kHeld = NV > 0 ? NV : 1;
+    __shared__ float slots[2][16];
     const T* w = static_cast<const T*>(p.weight);
     float* part = p.part + static_cast<long long>(blockIdx.x) * p.cols;
-    const int nv = NV > 0 ? NV : ((p.cols + 7) / 8 + THREADS - 1) / THREADS;
-    float acc[kHeld][8];
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[j][i] = 0.f;
-    if constexpr (NV == 0) {
-        for (int j = 0; j < nv; ++j)
-            for (int i = 0, c = (threadIdx.x + j * THREADS) * 8; i < 8; ++i)
-                if (c + i < p.cols) part[c + i] = 0.f;
-    }
+    for (int c = threadIdx.x; c < p.cols; c += blockDim.x) part[c] = 0.f;
     int turn = 0;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
@@ -374,72 +375,109 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_fp8_backward_kernel(const Nor
         const T* dres = p.dres ? static_cast<const T*>(p.dres) + row * p.lddres : nullptr;
         T* dx = static_cast<T*>(p.dx) + row * p.lddx;
         const float rstd = p.rstd[row];
-        Vec8<T> a[kHeld], b[kHeld], d[kHeld];
         float dot = 0.f;
-        auto load = [&](int j, int slot) {
-            const int c = (threadIdx.x + j * THREADS) * 8;
-            const int n = max(p.cols - c, 0), o = n ? c : 0;
-            a[slot] = load8(dy + o, n, p.vec_dy);
-            b[slot] = load8(h + o, n, p.vec_h);
-            if (dres != nullptr) d[slot] = load8(dres + o, n, p.vec_dres);
-        };
-        auto first_pass = [&](int j, int slot) {
-            const int c = (threadIdx.x + j * THREADS) * 8;
-            const int n = max(p.cols - c, 0);
-            const Vec8<T> g = load8(w + (n ? c : 0), n, p.vec_w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                dot = fmaf(to_f32(a[slot].v[i]) * to_f32(g.v[i]), to_f32(b[slot].v[i]) * rstd, dot);
-        };
-        if constexpr (NV > 0) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) load(j, j);
-#pragma unroll
-            for (int j = 0; j < NV; ++j) first_pass(j, j);
-        } else {
-            for (int j = 0; j < nv; ++j) {
-                load(j, 0);
-                first_pass(j, 0);
-            }
-        }
-        const float mean = cta_sum<THREADS>(dot, slots[turn]) / static_cast<float>(p.cols);
-        auto second_pass = [&](int j, int slot) {
-            const int c = (threadIdx.x + j * THREADS) * 8;
-            const int n = p.cols - c;
-            if (n <= 0) return;
-            const Vec8<T> g = load8(w + c, n, p.vec_w);
-            Vec8<T> o;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float dyf = to_f32(a[slot].v[i]), xhat = to_f32(b[slot].v[i]) * rstd;
-                float t = rstd * (dyf * to_f32(g.v[i]) - xhat * mean);
-                if (dres != nullptr) t += to_f32(d[slot].v[i]);
-                o.v[i] = from_f32<T>(t);
-                if constexpr (NV > 0)
-                    acc[slot][i] = fmaf(dyf, xhat, acc[slot][i]);
-                else if (i < n)
-                    part[c + i] = fmaf(dyf, xhat, part[c + i]);
-            }
-            store8(dx + c, o, n, p.vec_dx);
-        };
-        if constexpr (NV > 0) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) second_pass(j, j);
-        } else {
-            for (int j = 0; j < nv; ++j) {
-                load(j, 0);
-                second_pass(j, 0);
-            }
+        for (int c = threadIdx.x; c < p.cols; c += blockDim.x) dot = fmaf(to_f32(dy[c]) * to_f32(w[c]), to_f32(h[c]) * rstd, dot);
+        const float mean = cta_sum(dot, slots[turn]) / static_cast<float>(p.cols);
+        for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
+            const float dyf = to_f32(dy[c]), xhat = to_f32(h[c]) * rstd;
+            float t = rstd * (dyf * to_f32(w[c]) - xhat * mean);
+            if (dres != nullptr) t += to_f32(dres[c]);
+            dx[c] = from_f32<T>(t);
+            part[c] = fmaf(dyf, xhat, part[c]);
         }
     }
-    if constexpr (NV > 0) {
+}
+
+// The same for aligned rows of at most 512 * 8 * NV columns, a multiple of 8.  One CTA per SM; rows arrive ahead in
+// shared memory (one bulk copy per tensor and row, p.stages rows deep), so that memory stays busy through the two passes
+// and the barrier of each row; dweight's share stays in registers.
+template <typename T, int NV>
+__global__ void __launch_bounds__(512, 1) rmsnorm_fp8_backward_kernel(const NormBackParams p)
+{
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float slots[2][16];
+    __shared__ __align__(8) uint64_t bars[8];
+    const int threads = blockDim.x;
+    const uint32_t row_bytes = static_cast<uint32_t>(p.cols) * 2, pitch = (row_bytes + 127u) & ~127u;
+    const int tensors = p.dres ? 3 : 2;
+    auto issue = [&](long long row, int stage) {
+        const uint32_t bar = smem_u32(&bars[stage]), dst = smem_u32(smem) + static_cast<uint32_t>(stage) * 3 * pitch;
+        mbar_arrive_expect_tx(bar, row_bytes * tensors);
+        bulk_load(dst, static_cast<const T*>(p.dy) + row * p.lddy, row_bytes, bar);
+        bulk_load(dst + pitch, static_cast<const T*>(p.h) + row * p.ldh, row_bytes, bar);
+        if (p.dres) bulk_load(dst + 2 * pitch, static_cast<const T*>(p.dres) + row * p.lddres, row_bytes, bar);
+    };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) mbar_init(smem_u32(&bars[s]), 1);
+        fence_mbar_init();
+        fence_proxy_async_smem();
+        for (int s = 0; s < p.stages; ++s)
+            if (blockIdx.x + static_cast<long long>(s) * gridDim.x < p.rows) issue(blockIdx.x + static_cast<long long>(s) * gridDim.x, s);
+    }
+    const T* w = static_cast<const T*>(p.weight);
+    Vec8<T> gain[NV];
+    float acc[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (threadIdx.x + j * threads) * 8;
+        gain[j] = load8<true>(w + (c < p.cols ? c : 0), p.cols - c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[j][i] = 0.f;
+    }
+    __syncthreads();
+    int stage = 0, turn = 0;
+    uint32_t phase = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        const float rstd = p.rstd[row];
+        if (!mbar_wait(smem_u32(&bars[stage]), phase, p.timeout_ns, kErrWaitProducer, stage)) break;
+        const uint8_t* base = smem + static_cast<size_t>(stage) * 3 * pitch;
+        Vec8<T> a[NV], b[NV], d[NV];
+        float dot = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (threadIdx.x + j * threads) * 8;
+            const int n = p.cols - c, o = n > 0 ? c * 2 : 0;
+            a[j] = load8<true>(reinterpret_cast<const T*>(base + o), n);
+            b[j] = load8<true>(reinterpret_cast<const T*>(base + pitch + o), n);
+            if (p.dres) d[j] = load8<true>(reinterpret_cast<const T*>(base + 2 * pitch + o), n);
+        }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
+            for (int i = 0; i < 8; ++i)
+                dot = fmaf(to_f32(a[j].v[i]) * to_f32(gain[j].v[i]), to_f32(b[j].v[i]) * rstd, dot);
+        fence_proxy_async_smem();  // this thread has read its part of the stage
+        const float mean = cta_sum(dot, slots[turn]) / static_cast<float>(p.cols);
+        const long long ahead = row + static_cast<long long>(p.stages) * gridDim.x;
+        if (threadIdx.x == 0 && ahead < p.rows) issue(ahead, stage);
+        T* dx = static_cast<T*>(p.dx) + row * p.lddx;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (threadIdx.x + j * threads) * 8;
+            Vec8<T> o;
+#pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int c = (threadIdx.x + j * THREADS) * 8 + i;
-                if (c < p.cols) part[c] = acc[j][i];
+                const float dyf = to_f32(a[j].v[i]), xhat = to_f32(b[j].v[i]) * rstd;
+                float t = rstd * (dyf * to_f32(gain[j].v[i]) - xhat * mean);
+                if (p.dres) t += to_f32(d[j].v[i]);
+                o.v[i] = from_f32<T>(t);
+                acc[j][i] = fmaf(dyf, xhat, acc[j][i]);
             }
+            store8<true>(dx + c, o, p.cols - c);
+        }
+        if (++stage == p.stages) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
+    float* part = p.part + static_cast<long long>(blockIdx.x) * p.cols;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (threadIdx.x + j * threads) * 8;
+        if (c >= p.cols) continue;
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)
+            *reinterpret_cast<float4*>(part + c + i) = make_float4(acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]);
     }
 }
 
