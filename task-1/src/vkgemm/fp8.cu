@@ -258,19 +258,14 @@ extern "C" int vk_quantize_fp8(const vk_quantize_fp8_args* a)
             return launched();
         });
     }
-    const int64_t need = (a->rows * blocks + 15) / 16;
+    const int64_t ctas = (a->rows * ((blocks + 3) / 4) + 15) / 16;
+    if (ctas > kMaxDim) return set_error(VK_ERR_UNSUPPORTED, "%s: too many blocks", name);
+    const unsigned grid = static_cast<unsigned>(ctas);
     return for_type(a->dtype, [&](auto t) {
-        // four blocks at a time once there are enough for every SM
-        if (vec && need >= 148 * 4 * 4) {
-            const int64_t most = 148 * 8, wanted = (need + 3) / 4;
-            quantize_rows_kernel<decltype(t), true, 4><<<static_cast<unsigned>(wanted < most ? wanted : most), 256, 0, stream>>>(p);
-        } else {
-            const unsigned grid = static_cast<unsigned>(need < 148 * 32 ? need : 148 * 32);
-            if (vec)
-                quantize_rows_kernel<decltype(t), true, 1><<<grid, 256, 0, stream>>>(p);
-            else
-                quantize_rows_kernel<decltype(t), false, 1><<<grid, 256, 0, stream>>>(p);
-        }
+        if (vec)
+            quantize_rows_kernel<decltype(t), true><<<grid, 256, 0, stream>>>(p);
+        else
+            quantize_rows_kernel<decltype(t), false><<<grid, 256, 0, stream>>>(p);
         return launched();
     });
 }
@@ -283,15 +278,16 @@ static int launch_norm(const NormParams& p, int64_t rows, cudaStream_t stream)
 {
     const unsigned grid = static_cast<unsigned>(rows);
     const int vectors = (p.cols + 127) / 128 * 16;  // of 8 columns, whole blocks
-    auto threads = [&](int nv) { return static_cast<unsigned>(((vectors + nv - 1) / nv + 31) / 32 * 32); };
-    if (vectors <= 256)
-        rmsnorm_fp8_kernel<T, 1, VEC><<<grid, threads(1), 0, stream>>>(p);
-    else if (vectors <= 512)
-        rmsnorm_fp8_kernel<T, 2, VEC><<<grid, threads(2), 0, stream>>>(p);
-    else if (vectors <= 1024)
-        rmsnorm_fp8_kernel<T, 4, VEC><<<grid, threads(4), 0, stream>>>(p);
+    if (vectors > 1024) {
+        rmsnorm_fp8_long_kernel<T, VEC><<<grid, 512, 0, stream>>>(p);
+        return launched();
+    }
+    const int nv = vectors > 256 ? 2 : 1;
+    const int threads = ((vectors + nv - 1) / nv + 31) / 32 * 32;
+    if (nv == 1)
+        rmsnorm_fp8_kernel<T, 1, VEC><<<grid, threads, 0, stream>>>(p);
     else
-        rmsnorm_fp8_kernel<T, 0, VEC><<<grid, 512, 0, stream>>>(p);
+        rmsnorm_fp8_kernel<T, 2, VEC><<<grid, threads, 0, stream>>>(p);
     return launched();
 }
 
@@ -337,8 +333,24 @@ extern "C" int vk_rmsnorm_fp8(const vk_rmsnorm_fp8_args* a)
     });
 }
 
-// CTAs of the backward pass, each with a row of fp32 partial sums in the workspace: one per SM of B200.
-static int64_t norm_backward_parts(int64_t rows) { return rows < 148 ? rows : 148; }
+// How the backward pass is laid out: threads of a CTA with nv vectors of 8 columns each (nv = 0: the kernel for any number
+// of columns), and CTAs, each with a row of fp32 partial sums in the workspace.  Narrow rows need several CTAs on an SM
+// to keep memory busy; a CTA has four rows at least, so that the partial sums stay few.
+struct NormBackPlan {
+    int nv, threads, per_sm;
+    int64_t parts;
+};
+
+static NormBackPlan norm_backward_plan(int64_t rows, int64_t cols)
+{
+    NormBackPlan plan;
+    plan.nv = cols <= 512 * 8 ? 1 : cols <= 512 * 16 ? 2 : 0;
+    plan.threads = plan.nv ? static_cast<int>(((cols + 7) / 8 + plan.nv - 1) / plan.nv + 31) / 32 * 32 : 512;
+    plan.per_sm = plan.nv != 1 ? 1 : plan.threads <= 128 ? 8 : plan.threads <= 256 ? 4 : 2;
+    const int64_t most = 148 * plan.per_sm, wanted = (rows + 3) / 4;
+    plan.parts = wanted < 148 ? (rows < 148 ? rows : 148) : wanted < most ? wanted : most;
+    return plan;
+}
 
 extern "C" int vk_rmsnorm_fp8_workspace(int64_t rows, int64_t cols, size_t* bytes)
 {
@@ -346,24 +358,23 @@ extern "C" int vk_rmsnorm_fp8_workspace(int64_t rows, int64_t cols, size_t* byte
     if (bytes == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: bytes is NULL", name);
     if (rows < 0 || rows > kMaxDim) return bad_size(name, "rows", rows);
     if (cols < 1 || cols > kMaxDim) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: cols = %lld is out of range", name, (long long)cols);
-    *bytes = static_cast<size_t>(norm_backward_parts(rows)) * static_cast<size_t>(cols) * sizeof(float);
+    *bytes = static_cast<size_t>(norm_backward_plan(rows, cols).parts) * static_cast<size_t>(cols) * sizeof(float);
     return VK_OK;
 }
 
-// Shared memory that the rows in flight may take.
-constexpr int kNormBackBytes = 200 * 1024;
+// Shared memory per SM that the rows in flight may take.
+constexpr int kNormBackBytes = 208 * 1024;
 
 template <typename T, int NV>
-static int launch_norm_backward(NormBackParams p, int id, unsigned grid, cudaStream_t stream)
+static int launch_norm_backward(NormBackParams p, int id, const NormBackPlan& plan, cudaStream_t stream)
 {
     const int pitch = (p.cols * 2 + 127) / 128 * 128;
     int clusters[4];
-    const int rc = prepare_kernel(rmsnorm_fp8_backward_kernel<T, NV>, id, kNormBackBytes, 512, clusters);
+    const int rc = prepare_kernel(rmsnorm_fp8_backward_kernel<T, NV>, id, kNormBackBytes / (NV == 1 ? 2 : 1), 512, clusters);
     if (rc != VK_OK) return rc;
-    p.stages = kNormBackBytes / (3 * pitch);
+    p.stages = kNormBackBytes / plan.per_sm / (3 * pitch);
     if (p.stages > 8) p.stages = 8;
-    const unsigned threads = static_cast<unsigned>(((p.cols / 8 + NV - 1) / NV + 31) / 32 * 32);
-    rmsnorm_fp8_backward_kernel<T, NV><<<grid, threads, p.stages * 3 * pitch, stream>>>(p);
+    rmsnorm_fp8_backward_kernel<T, NV><<<static_cast<unsigned>(plan.parts), plan.threads, p.stages * 3 * pitch, stream>>>(p);
     return launched();
 }
 
@@ -391,7 +402,7 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
     rc = use_device();
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
-    const int64_t parts = norm_backward_parts(a->rows);
+    const NormBackPlan plan = norm_backward_plan(a->rows, a->cols);
     p.dy = a->dY;
     p.h = a->H;
     p.weight = a->weight;
@@ -406,19 +417,18 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
     const bool vec = rows_at(a->dY, p.lddy, 2, 16) && rows_at(a->H, p.ldh, 2, 16) && aligned(a->weight, 16) &&
                      (a->dres == nullptr || rows_at(a->dres, p.lddres, 2, 16)) && rows_at(a->dX, p.lddx, 2, 16) && a->cols % 8 == 0;
     if (a->rows > 0) {
-        const unsigned grid = static_cast<unsigned>(parts);
         rc = for_type(a->dtype, [&](auto t) {
             using T = std::conditional_t<std::is_same_v<decltype(t), __half>, __half, __nv_bfloat16>;
             constexpr int kId = 9 + (std::is_same_v<T, __half> ? 0 : 2);
-            if (vec && p.cols <= 512 * 8) return launch_norm_backward<T, 1>(p, kId, grid, stream);
-            if (vec && p.cols <= 512 * 16) return launch_norm_backward<T, 2>(p, kId + 1, grid, stream);
-            rmsnorm_fp8_backward_any_kernel<T><<<grid, 512, 0, stream>>>(p);
+            if (vec && plan.nv == 1) return launch_norm_backward<T, 1>(p, kId, plan, stream);
+            if (vec && plan.nv == 2) return launch_norm_backward<T, 2>(p, kId + 1, plan, stream);
+            rmsnorm_fp8_backward_any_kernel<T><<<static_cast<unsigned>(plan.parts), 512, 0, stream>>>(p);
             return launched();
         });
         if (rc != VK_OK) return rc;
     }
-    norm_weight_grad_kernel<<<static_cast<unsigned>((a->cols + 31) / 32), 256, 0, stream>>>(
-        p.part, static_cast<int>(parts), p.cols, a->dweight);
+    norm_weight_grad_kernel<<<static_cast<unsigned>((a->cols + 31) / 32), 1024, 0, stream>>>(
+        p.part, static_cast<int>(plan.parts), p.cols, a->dweight);
     return launched();
 }
 

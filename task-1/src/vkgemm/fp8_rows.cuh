@@ -127,6 +127,19 @@ __device__ __forceinline__ uint32_t top_of(const float (&f)[8])
     return t;
 }
 
+// The same of eight stored values.  16-bit ones are compared two at a time, as integers that order like the numbers.
+__device__ __forceinline__ uint32_t top_of(const Vec8<float>& v) { return top_of(v.v); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const Vec8<T>& v)
+{
+    const uint4 w = *reinterpret_cast<const uint4*>(&v);
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    const uint32_t t = __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs), __vmaxu2(w.z & kAbs, w.w & kAbs));
+    const uint16_t top = static_cast<uint16_t>(max(t & 0xffffu, t >> 16));
+    return abs_bits(to_f32(*reinterpret_cast<const T*>(&top)));
+}
+
 // The largest value over the 16 lanes that share a block of 128.
 __device__ __forceinline__ uint32_t top_of_16_lanes(uint32_t t)
 {
@@ -146,49 +159,41 @@ struct QuantParams {
     int cols, blocks;  // blocks of 128 in a row
 };
 
-// Blocks of 128 of one row: 16 lanes hold one block, 8 values each; UNROLL blocks at a time, so that as many loads are in
-// flight, and on over the whole matrix.
-template <typename T, bool VEC, int UNROLL>
+// Rows: 16 lanes hold one block, 8 values each, and have four neighbouring blocks of a row, so that four loads are in
+// flight and the four scales leave in one store.  16 such quads to a CTA.  (Blocks one by one, a grid apart: 8192 x 8192
+// bf16 45 us.)
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
 {
     const int sub = threadIdx.x & 15;
-    const long long step = static_cast<long long>(gridDim.x) * 16;
-    const long long first = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-    const long long total = p.rows * p.blocks;
-    const long long drow = step / p.blocks;
-    const int dblk = static_cast<int>(step % p.blocks);
-    long long row = first / p.blocks;
-    int blk = static_cast<int>(first % p.blocks);
-    const T* x = static_cast<const T*>(p.x);
-    // a warp's two halves leave the loop together: the shuffles below need every lane
-    for (long long at = first & ~1ll; at < total; at += step * UNROLL) {
-        Vec8<T> v[UNROLL];
-        long long rows[UNROLL];
-        int blks[UNROLL];
+    const int quads = (p.blocks + 3) / 4;
+    const long long item = static_cast<long long>(blockIdx.x) * 16;
+    const unsigned in = static_cast<unsigned>(item % quads) + (threadIdx.x >> 4);
+    const long long row = item / quads + in / quads;
+    const int blk = static_cast<int>(in % quads) * 4;
+    const int c = blk * 128 + sub * 8;
+    const int left = row < p.rows ? p.cols - c : 0;
+    const T* x = static_cast<const T*>(p.x) + (left > 0 ? row * p.ldx + c : 0);
+    Vec8<T> v[4];
 #pragma unroll
-        for (int j = 0; j < UNROLL; ++j) {
-            rows[j] = row;
-            blks[j] = blk;
-            const int c = blk * 128 + sub * 8;
-            const int n = row < p.rows ? p.cols - c : 0;
-            v[j] = load8<VEC>(x + (n > 0 ? row * p.ldx + c : 0), n);
-            row += drow;
-            blk += dblk;
-            if (blk >= p.blocks) {
-                blk -= p.blocks;
-                ++row;
-            }
-        }
+    for (int j = 0; j < 4; ++j) v[j] = load8<VEC>(x + (left > 128 * j ? 128 * j : 0), left - 128 * j);
+    uint32_t scales = 0;
 #pragma unroll
-        for (int j = 0; j < UNROLL; ++j) {
-            const int c = blks[j] * 128 + sub * 8;
-            float f[8];
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t s = block_scale(top_of_16_lanes(top_of(v[j])));
+        scales |= s << (8 * j);
+        if (left <= 128 * j) continue;
+        float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = to_f32(v[j].v[i]);
-            const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
-            if (rows[j] >= p.rows) continue;
-            store_q8<VEC>(p.q + rows[j] * p.ldq + c, f, s, p.cols - c);
-            if (sub == 0) p.scale[rows[j] * p.lds + blks[j]] = static_cast<uint8_t>(s);
+        for (int i = 0; i < 8; ++i) f[i] = to_f32(v[j].v[i]);
+        store_q8<VEC>(p.q + row * p.ldq + c + 128 * j, f, s, left - 128 * j);
+    }
+    if (sub == 0 && left > 0) {
+        uint8_t* out = p.scale + row * p.lds + blk;
+        if (blk + 4 <= p.blocks && (reinterpret_cast<uintptr_t>(out) & 3) == 0) {
+            *reinterpret_cast<uint32_t*>(out) = scales;
+        } else {
+            for (int j = 0; j < 4 && blk + j < p.blocks; ++j) out[j] = static_cast<uint8_t>(scales >> (8 * j));
         }
     }
 }
@@ -212,9 +217,7 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p
         v[j] = load8<VEC>(x + (n > 0 ? row * p.ldx + c : 0), n);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, abs_bits(to_f32(v[j].v[i])));
+    for (int j = 0; j < 8; ++j) top = max(top, top_of(v[j]));
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
@@ -261,85 +264,104 @@ struct NormParams {
     float eps;
 };
 
-// One row per CTA; thread t holds the vectors of 8 at t, t + blockDim.x, ... (NV of them; NV = 0: any number, read again
-// from h for the second pass).  blockDim.x is a multiple of 32, so the 16 lanes of an aligned group hold one block.
-// VEC: rows and weight are aligned for 16-byte accesses (q: 8) and cols is a multiple of 8.
+// One row per CTA; a thread holds the vectors of 8 at t, t + blockDim.x, ... (NV of them).  blockDim.x is a multiple of
+// 32, so the 16 lanes of an aligned group hold one block.  VEC: rows and weight are aligned for 16-byte accesses (q: 8)
+// and cols is a multiple of 8.  (CTAs that walk over the rows with the next one on its way take the registers of two
+// rows: 8192 x 8192 bf16 with a residual 150 us, against 92 like this.)
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(NV == 0 ? 512 : 256) rmsnorm_fp8_kernel(const NormParams p)
+__global__ void __launch_bounds__(NV == 1 ? 256 : 512) rmsnorm_fp8_kernel(const NormParams p)
 {
     __shared__ float slots[16];
-    constexpr int kHeld = NV > 0 ? NV : 1;
     const int threads = blockDim.x;
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
+    const T* r = static_cast<const T*>(p.residual) + row * p.ldr;
     const T* w = static_cast<const T*>(p.weight);
-    T* h = p.residual ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
-    const int nv = NV > 0 ? NV : ((p.cols + 127) / 128 * 16 + threads - 1) / threads;
-
-    Vec8<T> held[kHeld], res[kHeld], gain[kHeld];
-    float sq = 0.f;
-    auto load = [&](int j, int slot) {
-        const int c = (threadIdx.x + j * threads) * 8;
-        const int n = p.cols - c, o = n > 0 ? c : 0;
-        held[slot] = load8<VEC>(x + o, n);
-        if (r != nullptr) res[slot] = load8<VEC>(r + o, n);
-    };
-    auto first_pass = [&](int j, int slot) {
-        const int c = (threadIdx.x + j * threads) * 8;
-        Vec8<T>& a = held[slot];
-        if (r != nullptr) {
+    Vec8<T> held[NV], res[NV], gain[NV];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a.v[i] = from_f32<T>(to_f32(a.v[i]) + to_f32(res[slot].v[i]));
-            store8<VEC>(h + c, a, p.cols - c);
+    for (int j = 0; j < NV; ++j) {
+        const int c = (threadIdx.x + j * threads) * 8, n = p.cols - c, o = n > 0 ? c : 0;
+        held[j] = load8<VEC>(x + o, n);
+        if (p.residual != nullptr) res[j] = load8<VEC>(r + o, n);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (threadIdx.x + j * threads) * 8;
+        gain[j] = load8<VEC>(w + (c < p.cols ? c : 0), p.cols - c);
+    }
+    float sq = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (threadIdx.x + j * threads) * 8;
+        if (p.residual != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) held[j].v[i] = from_f32<T>(to_f32(held[j].v[i]) + to_f32(res[j].v[i]));
+            store8<VEC>(static_cast<T*>(p.h) + row * p.ldh + c, held[j], p.cols - c);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = to_f32(held[j].v[i]);
+            sq = fmaf(f, f, sq);
+        }
+    }
+    const float total = cta_sum(sq, slots);
+    const float rstd = 1.0f / sqrtf(total / static_cast<float>(p.cols) + p.eps);
+    if (threadIdx.x == 0) p.rstd[row] = rstd;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = (threadIdx.x + j * threads) * 8;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f32(held[j].v[i]) * rstd * to_f32(gain[j].v[i]);
+        const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
+        if (c < p.cols) {
+            store_q8<VEC>(p.q + row * p.ldq + c, f, s, p.cols - c);
+            if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + c / 128] = static_cast<uint8_t>(s);
+        }
+    }
+}
+
+// The same for any number of columns: h (or x) is read again for the second pass.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(512) rmsnorm_fp8_long_kernel(const NormParams p)
+{
+    __shared__ float slots[16];
+    const long long row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* r = static_cast<const T*>(p.residual) + row * p.ldr;
+    const T* w = static_cast<const T*>(p.weight);
+    T* h = static_cast<T*>(p.h) + row * p.ldh;
+    const int nv = ((p.cols + 127) / 128 * 16 + 511) / 512;
+    float sq = 0.f;
+    for (int j = 0; j < nv; ++j) {
+        const int c = (threadIdx.x + j * 512) * 8, n = p.cols - c, o = n > 0 ? c : 0;
+        Vec8<T> a = load8<VEC>(x + o, n);
+        if (p.residual != nullptr) {
+            const Vec8<T> b = load8<VEC>(r + o, n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a.v[i] = from_f32<T>(to_f32(a.v[i]) + to_f32(b.v[i]));
+            store8<VEC>(h + c, a, n);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float f = to_f32(a.v[i]);
             sq = fmaf(f, f, sq);
         }
-    };
-    auto load_gain = [&](int j, int slot) {
-        const int c = (threadIdx.x + j * threads) * 8;
-        gain[slot] = load8<VEC>(w + (c < p.cols ? c : 0), p.cols - c);
-    };
-    auto second_pass = [&](int j, int slot, float rstd) {
-        const int c = (threadIdx.x + j * threads) * 8;
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f32(held[slot].v[i]) * rstd * to_f32(gain[slot].v[i]);
-        const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
-        if (c < p.cols) {
-            store_q8<VEC>(p.q + row * p.ldq + c, f, s, p.cols - c);
-            if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + c / 128] = static_cast<uint8_t>(s);
-        }
-    };
-    if constexpr (NV > 0) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) load(j, j);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) load_gain(j, j);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) first_pass(j, j);
-    } else {
-        for (int j = 0; j < nv; ++j) {
-            load(j, 0);
-            first_pass(j, 0);
-        }
     }
     const float total = cta_sum(sq, slots);
     const float rstd = 1.0f / sqrtf(total / static_cast<float>(p.cols) + p.eps);
     if (threadIdx.x == 0) p.rstd[row] = rstd;
-    if constexpr (NV > 0) {
+    const T* src = p.residual != nullptr ? h : x;  // this thread's own writes
+    for (int j = 0; j < nv; ++j) {
+        const int c = (threadIdx.x + j * 512) * 8, n = p.cols - c, o = n > 0 ? c : 0;
+        const Vec8<T> a = load8<VEC>(src + o, n), gain = load8<VEC>(w + o, n);
+        float f[8];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) second_pass(j, j, rstd);
-    } else {
-        const T* src = r != nullptr ? h : x;  // this thread's own writes
-        for (int j = 0; j < nv; ++j) {
-            const int c = (threadIdx.x + j * threads) * 8;
-            held[0] = load8<VEC>(src + (c < p.cols ? c : 0), p.cols - c);
-            load_gain(j, 0);
-            second_pass(j, 0, rstd);
+        for (int i = 0; i < 8; ++i) f[i] = to_f32(a.v[i]) * rstd * to_f32(gain.v[i]);
+        const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
+        if (n > 0) {
+            store_q8<VEC>(p.q + row * p.ldq + c, f, s, n);
+            if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + c / 128] = static_cast<uint8_t>(s);
         }
     }
 }
@@ -388,11 +410,11 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const Nor
     }
 }
 
-// The same for aligned rows of at most 512 * 8 * NV columns, a multiple of 8.  One CTA per SM; rows arrive ahead in
-// shared memory (one bulk copy per tensor and row, p.stages rows deep), so that memory stays busy through the two passes
-// and the barrier of each row; dweight's share stays in registers.
+// The same for aligned rows of at most 512 * 8 * NV columns, a multiple of 8.  Two CTAs or more per SM; rows arrive ahead
+// in shared memory (one bulk copy per tensor and row, p.stages rows deep), so that memory stays busy through the two
+// passes and the barrier of each row; dweight's share stays in registers.
 template <typename T, int NV>
-__global__ void __launch_bounds__(512, 1) rmsnorm_fp8_backward_kernel(const NormBackParams p)
+__global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_kernel(const NormBackParams p)
 {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float slots[2][16];
@@ -425,46 +447,44 @@ __global__ void __launch_bounds__(512, 1) rmsnorm_fp8_backward_kernel(const Norm
         for (int i = 0; i < 8; ++i) acc[j][i] = 0.f;
     }
     __syncthreads();
-    int stage = 0, turn = 0;
+    int stage = 0, before = p.stages - 1, turn = 0;
     uint32_t phase = 0;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const float rstd = p.rstd[row];
         if (!mbar_wait(smem_u32(&bars[stage]), phase, p.timeout_ns, kErrWaitProducer, stage)) break;
         const uint8_t* base = smem + static_cast<size_t>(stage) * 3 * pitch;
-        Vec8<T> a[NV], b[NV], d[NV];
+        Vec8<T> a[NV], b[NV];
         float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (threadIdx.x + j * threads) * 8;
-            const int n = p.cols - c, o = n > 0 ? c * 2 : 0;
+            const int c = (threadIdx.x + j * threads) * 8, n = p.cols - c, o = n > 0 ? c * 2 : 0;
             a[j] = load8<true>(reinterpret_cast<const T*>(base + o), n);
             b[j] = load8<true>(reinterpret_cast<const T*>(base + pitch + o), n);
-            if (p.dres) d[j] = load8<true>(reinterpret_cast<const T*>(base + 2 * pitch + o), n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dot = fmaf(to_f32(a[j].v[i]) * to_f32(gain[j].v[i]), to_f32(b[j].v[i]) * rstd, dot);
         }
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                dot = fmaf(to_f32(a[j].v[i]) * to_f32(gain[j].v[i]), to_f32(b[j].v[i]) * rstd, dot);
-        fence_proxy_async_smem();  // this thread has read its part of the stage
         const float mean = cta_sum(dot, slots[turn]) / static_cast<float>(p.cols);
-        const long long ahead = row + static_cast<long long>(p.stages) * gridDim.x;
-        if (threadIdx.x == 0 && ahead < p.rows) issue(ahead, stage);
+        // Behind this barrier no thread reads the row before any more: its stage is free.
+        const long long ahead = row + static_cast<long long>(p.stages - 1) * gridDim.x;
+        if (threadIdx.x == 0 && row != blockIdx.x && ahead < p.rows) issue(ahead, before);
         T* dx = static_cast<T*>(p.dx) + row * p.lddx;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (threadIdx.x + j * threads) * 8;
-            Vec8<T> o;
+            const int c = (threadIdx.x + j * threads) * 8, n = p.cols - c, o = n > 0 ? c * 2 : 0;
+            Vec8<T> d;
+            if (p.dres) d = load8<true>(reinterpret_cast<const T*>(base + 2 * pitch + o), n);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float dyf = to_f32(a[j].v[i]), xhat = to_f32(b[j].v[i]) * rstd;
                 float t = rstd * (dyf * to_f32(gain[j].v[i]) - xhat * mean);
-                if (p.dres) t += to_f32(d[j].v[i]);
-                o.v[i] = from_f32<T>(t);
+                if (p.dres) t += to_f32(d.v[i]);
+                d.v[i] = from_f32<T>(t);
                 acc[j][i] = fmaf(dyf, xhat, acc[j][i]);
             }
-            store8<true>(dx + c, o, p.cols - c);
+            store8<true>(dx + c, d, n);
         }
+        fence_proxy_async_smem();  // read before the stage is written again
+        before = stage;
         if (++stage == p.stages) {
             stage = 0;
             phase ^= 1u;
@@ -481,22 +501,23 @@ __global__ void __launch_bounds__(512, 1) rmsnorm_fp8_backward_kernel(const Norm
     }
 }
 
-// dweight[c] = sum of the `parts` rows of part, in row order: 32 columns x 8 groups of rows per CTA.
-__global__ void __launch_bounds__(256) norm_weight_grad_kernel(const float* part, int parts, int cols, float* dweight)
+// dweight[c] = sum of the `parts` rows of part: 32 columns x 32 groups of rows per CTA.
+__global__ void __launch_bounds__(1024) norm_weight_grad_kernel(const float* part, int parts, int cols, float* dweight)
 {
-    __shared__ float sums[8][33];
+    __shared__ float sums[32][33];
     const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float t = 0.f;
-    if (c < cols)
-        for (int r = group; r < parts; r += 8) t += part[static_cast<long long>(r) * cols + c];
+    if (c < cols) {
+#pragma unroll 4
+        for (int r = group; r < parts; r += 32) t += part[static_cast<long long>(r) * cols + c];
+    }
     sums[group][lane] = t;
     __syncthreads();
-    if (group == 0 && c < cols) {
+    t = sums[lane][group];  // column `group` of this CTA
 #pragma unroll
-        for (int g = 1; g < 8; ++g) t += sums[g][lane];
-        dweight[c] = t;
-    }
+    for (int d = 16; d >= 1; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+    if (lane == 0 && blockIdx.x * 32 + group < cols) dweight[blockIdx.x * 32 + group] = t;
 }
 
 }  // namespace vk

@@ -7,7 +7,7 @@ Tolerances, all from arithmetic (u = 2^-24, half a step of fp32; h(t) = eps/2, h
              (2^-4 of the value, 2^-10 of the scale below e4m3's normal numbers), and a scale one power of two off
              only where the block's largest value is within 104 u of the border
   backward   sums as above: 104 u of the sum of magnitudes, and one rounding to the output's type; dweight adds
-             rows/148 terms in one thread, and 19 + 8 partial sums
+             rows/148 terms in one thread, and 37 + 5 partial sums
   products   fp32 accumulation in any order: k u of the sum of magnitudes, and one rounding
 """
 import itertools
@@ -228,7 +228,7 @@ def _check_norm_back(dy, h, w, rstd, dres, dx, dw):
     tol = 104 * U * size + HALF[dy.dtype] * (1 + 2.0 ** -8) * want.abs() + TINY[dy.dtype]
     assert ((dx.double() - want).abs() <= tol).all()
     wsize = (a * xhat).abs().sum(dim=0)
-    depth = -(-rows // 148) + 19 + 8 + 4
+    depth = -(-rows // 148) + 37 + 5 + 4
     assert ((dw.double() - (a * xhat).sum(dim=0)).abs() <= depth * U * wsize).all()
     assert dw.dtype == F32 and dx.dtype == dy.dtype and n == dw.shape[0]
 
