@@ -324,6 +324,7 @@ extern "C" int vk_rmsnorm_fp8(const vk_rmsnorm_fp8_args* a)
     p.rstd = a->rstd;
     p.cols = static_cast<int>(a->cols);
     p.eps = a->eps;
+    p.inv_cols = 1.0f / static_cast<float>(a->cols);
     const bool vec = rows_at(a->X, p.ldx, 2, 16) && (a->residual == nullptr || (rows_at(a->residual, p.ldr, 2, 16) && rows_at(a->H, p.ldh, 2, 16))) &&
                      aligned(a->weight, 16) && rows_at(a->Q, p.ldq, 1, 8) && a->cols % 8 == 0;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
@@ -413,6 +414,7 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
     p.rows = a->rows;
     p.cols = static_cast<int>(a->cols);
     p.stages = 0;
+    p.inv_cols = 1.0f / static_cast<float>(a->cols);
     p.timeout_ns = wait_timeout_ns();
     const bool vec = rows_at(a->dY, p.lddy, 2, 16) && rows_at(a->H, p.ldh, 2, 16) && aligned(a->weight, 16) &&
                      (a->dres == nullptr || rows_at(a->dres, p.lddres, 2, 16)) && rows_at(a->dX, p.lddx, 2, 16) && a->cols % 8 == 0;

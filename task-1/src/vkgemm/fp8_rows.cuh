@@ -95,10 +95,10 @@ __device__ __forceinline__ float inverse_scale(uint32_t s)
     return s == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float((254u - s) << 23);
 }
 
-__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d)
+__device__ __forceinline__ uint32_t pack_e4m3(float2 a, float2 b)
 {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
 }
 
@@ -108,8 +108,8 @@ __device__ __forceinline__ void store_q8(uint8_t* dst, const float (&f)[8], uint
 {
     const float inv = inverse_scale(s);
     uint2 w;
-    w.x = pack_e4m3(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-    w.y = pack_e4m3(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+    w.x = pack_e4m3(__fmul2_rn(make_float2(f[0], f[1]), make_float2(inv, inv)), __fmul2_rn(make_float2(f[2], f[3]), make_float2(inv, inv)));
+    w.y = pack_e4m3(__fmul2_rn(make_float2(f[4], f[5]), make_float2(inv, inv)), __fmul2_rn(make_float2(f[6], f[7]), make_float2(inv, inv)));
     if constexpr (VEC) {
         if (n > 0) *reinterpret_cast<uint2*>(dst) = w;
     } else {
@@ -121,10 +121,10 @@ __device__ __forceinline__ void store_q8(uint8_t* dst, const float (&f)[8], uint
 
 __device__ __forceinline__ uint32_t top_of(const float (&f)[8])
 {
-    uint32_t t = 0;
+    float t = f[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t = max(t, abs_bits(f[i]));
-    return t;
+    for (int i = 1; i < 8; ++i) asm("max.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(t) : "f"(f[i]));
+    return abs_bits(t);
 }
 
 // The same of eight stored values.  16-bit ones are compared two at a time, as integers that order like the numbers.
@@ -146,6 +146,23 @@ __device__ __forceinline__ uint32_t top_of_16_lanes(uint32_t t)
 #pragma unroll
     for (int d = 8; d >= 1; d >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, d));
     return t;
+}
+
+// Scales of N (2 or 4) blocks of a row from block `blk`, of which the row has `blocks`; one store where it can be.
+template <int N>
+__device__ __forceinline__ void put_scales(uint8_t* row, int blk, int blocks, uint32_t scales)
+{
+    uint8_t* out = row + blk;
+    if (blk + N <= blocks && (reinterpret_cast<uintptr_t>(out) & (N - 1)) == 0) {
+        if constexpr (N == 4)
+            *reinterpret_cast<uint32_t*>(out) = scales;
+        else
+            *reinterpret_cast<uint16_t*>(out) = static_cast<uint16_t>(scales);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (blk + j < blocks) out[j] = static_cast<uint8_t>(scales >> (8 * j));
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -188,14 +205,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
         for (int i = 0; i < 8; ++i) f[i] = to_f32(v[j].v[i]);
         store_q8<VEC>(p.q + row * p.ldq + c + 128 * j, f, s, left - 128 * j);
     }
-    if (sub == 0 && left > 0) {
-        uint8_t* out = p.scale + row * p.lds + blk;
-        if (blk + 4 <= p.blocks && (reinterpret_cast<uintptr_t>(out) & 3) == 0) {
-            *reinterpret_cast<uint32_t*>(out) = scales;
-        } else {
-            for (int j = 0; j < 4 && blk + j < p.blocks; ++j) out[j] = static_cast<uint8_t>(scales >> (8 * j));
-        }
-    }
+    if (sub == 0 && left > 0) put_scales<4>(p.scale + row * p.lds, blk, p.blocks, scales);
 }
 
 // One 128 x 128 tile per CTA, held in registers between its maximum and its rounding: 16 lanes per row, 16 rows at a time.
@@ -239,16 +249,19 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p
 // ------------------------------------------------------------------------------------------
 // RMS norm
 // ------------------------------------------------------------------------------------------
-// Sum over the CTA's threads, the same on all of them.  `slots` alternates between calls (one barrier each).
+// Sum over the CTA's threads (16 warps at most), the same on all of them.
+// `slots` alternates between calls (one barrier each).
 __device__ __forceinline__ float cta_sum(float v, float* slots)
 {
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
     __syncthreads();
-    float t = 0.f;
-    for (int w = 0; w < static_cast<int>(blockDim.x) / 32; ++w) t += slots[w];
-    return t;
+    const int from = threadIdx.x & 15;
+    v = from < static_cast<int>(blockDim.x) / 32 ? slots[from] : 0.f;
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
 }
 
 struct NormParams {
@@ -261,18 +274,18 @@ struct NormParams {
     float* rstd;
     long long ldx, ldr, ldq, lds, ldh;
     int cols;
-    float eps;
+    float eps, inv_cols;  // 1 / cols
 };
 
-// One row per CTA; a thread holds the vectors of 8 at t, t + blockDim.x, ... (NV of them).  blockDim.x is a multiple of
-// 32, so the 16 lanes of an aligned group hold one block.  VEC: rows and weight are aligned for 16-byte accesses (q: 8)
-// and cols is a multiple of 8.  (CTAs that walk over the rows with the next one on its way take the registers of two
-// rows: 8192 x 8192 bf16 with a residual 150 us, against 92 like this.)
+// One row per CTA; a warp has 32 NV neighbouring vectors of 8, 2 NV blocks, and stores their scales at once (a byte at a
+// time costs memory more than the row's values do).  VEC: rows and weight are aligned for 16-byte accesses (q: 8) and
+// cols is a multiple of 8.  (CTAs that walk over the rows with the next one on its way take the registers of two rows:
+// 8192 x 8192 bf16 with a residual 150 us, against 92 without.)
 template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(NV == 1 ? 256 : 512) rmsnorm_fp8_kernel(const NormParams p)
 {
     __shared__ float slots[16];
-    const int threads = blockDim.x;
+    const int lane = threadIdx.x & 31, first = (threadIdx.x >> 5) * 32 * NV + lane;
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* r = static_cast<const T*>(p.residual) + row * p.ldr;
@@ -280,45 +293,50 @@ __global__ void __launch_bounds__(NV == 1 ? 256 : 512) rmsnorm_fp8_kernel(const 
     Vec8<T> held[NV], res[NV], gain[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (threadIdx.x + j * threads) * 8, n = p.cols - c, o = n > 0 ? c : 0;
+        const int c = (first + j * 32) * 8, n = p.cols - c, o = n > 0 ? c : 0;
         held[j] = load8<VEC>(x + o, n);
         if (p.residual != nullptr) res[j] = load8<VEC>(r + o, n);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (threadIdx.x + j * threads) * 8;
+        const int c = (first + j * 32) * 8;
         gain[j] = load8<VEC>(w + (c < p.cols ? c : 0), p.cols - c);
     }
-    float sq = 0.f;
+    float2 sq = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (threadIdx.x + j * threads) * 8;
+        const int c = (first + j * 32) * 8;
         if (p.residual != nullptr) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) held[j].v[i] = from_f32<T>(to_f32(held[j].v[i]) + to_f32(res[j].v[i]));
             store8<VEC>(static_cast<T*>(p.h) + row * p.ldh + c, held[j], p.cols - c);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float f = to_f32(held[j].v[i]);
-            sq = fmaf(f, f, sq);
+        for (int i = 0; i < 8; i += 2) {
+            const float2 f = make_float2(to_f32(held[j].v[i]), to_f32(held[j].v[i + 1]));
+            sq = __ffma2_rn(f, f, sq);
         }
     }
-    const float total = cta_sum(sq, slots);
-    const float rstd = 1.0f / sqrtf(total / static_cast<float>(p.cols) + p.eps);
+    const float total = cta_sum(sq.x + sq.y, slots);
+    const float rstd = __frsqrt_rn(fmaf(total, p.inv_cols, p.eps));
     if (threadIdx.x == 0) p.rstd[row] = rstd;
+    uint32_t scales = 0;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (threadIdx.x + j * threads) * 8;
+        const int c = (first + j * 32) * 8;
         float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f32(held[j].v[i]) * rstd * to_f32(gain[j].v[i]);
-        const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
-        if (c < p.cols) {
-            store_q8<VEC>(p.q + row * p.ldq + c, f, s, p.cols - c);
-            if ((threadIdx.x & 15) == 0) p.scale[row * p.lds + c / 128] = static_cast<uint8_t>(s);
+        for (int i = 0; i < 8; i += 2) {
+            const float2 xhat = __fmul2_rn(make_float2(to_f32(held[j].v[i]), to_f32(held[j].v[i + 1])), make_float2(rstd, rstd));
+            const float2 y = __fmul2_rn(xhat, make_float2(to_f32(gain[j].v[i]), to_f32(gain[j].v[i + 1])));
+            f[i] = y.x;
+            f[i + 1] = y.y;
         }
+        const uint32_t s = block_scale(top_of_16_lanes(top_of(f)));
+        store_q8<VEC>(p.q + row * p.ldq + c, f, s, p.cols - c);
+        scales |= (s | __shfl_down_sync(0xffffffffu, s, 16) << 8) << (16 * j);
     }
+    if (lane == 0) put_scales<2 * NV>(p.scale + row * p.lds, (threadIdx.x >> 5) * 2 * NV, (p.cols + 127) / 128, scales);
 }
 
 // The same for any number of columns: h (or x) is read again for the second pass.
@@ -349,7 +367,7 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_long_kernel(const NormParams 
         }
     }
     const float total = cta_sum(sq, slots);
-    const float rstd = 1.0f / sqrtf(total / static_cast<float>(p.cols) + p.eps);
+    const float rstd = __frsqrt_rn(fmaf(total, p.inv_cols, p.eps));
     if (threadIdx.x == 0) p.rstd[row] = rstd;
     const T* src = p.residual != nullptr ? h : x;  // this thread's own writes
     for (int j = 0; j < nv; ++j) {
@@ -376,6 +394,7 @@ struct NormBackParams {
     float* part;       // [gridDim.x][cols] fp32: each CTA's share of dweight
     long long rows, lddy, ldh, lddres, lddx;
     int cols;
+    float inv_cols;    // 1 / cols
     int stages;        // rows in flight (rmsnorm_fp8_backward_kernel)
     unsigned long long timeout_ns;
 };
@@ -399,7 +418,7 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const Nor
         const float rstd = p.rstd[row];
         float dot = 0.f;
         for (int c = threadIdx.x; c < p.cols; c += blockDim.x) dot = fmaf(to_f32(dy[c]) * to_f32(w[c]), to_f32(h[c]) * rstd, dot);
-        const float mean = cta_sum(dot, slots[turn]) / static_cast<float>(p.cols);
+        const float mean = cta_sum(dot, slots[turn]) * p.inv_cols;
         for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
             const float dyf = to_f32(dy[c]), xhat = to_f32(h[c]) * rstd;
             float t = rstd * (dyf * to_f32(w[c]) - xhat * mean);
@@ -463,7 +482,7 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_ker
 #pragma unroll
             for (int i = 0; i < 8; ++i) dot = fmaf(to_f32(a[j].v[i]) * to_f32(gain[j].v[i]), to_f32(b[j].v[i]) * rstd, dot);
         }
-        const float mean = cta_sum(dot, slots[turn]) / static_cast<float>(p.cols);
+        const float mean = cta_sum(dot, slots[turn]) * p.inv_cols;
         // Behind this barrier no thread reads the row before any more: its stage is free.
         const long long ahead = row + static_cast<long long>(p.stages - 1) * gridDim.x;
         if (threadIdx.x == 0 && row != blockIdx.x && ahead < p.rows) issue(ahead, before);
