@@ -12,6 +12,7 @@
 #include "fp8_gemm.cuh"
 #include "fp8_rows.cuh"
 #include "fp8_simt.cuh"
+#include "fp8_thin.cuh"
 #include "fp8_wgrad.cuh"
 #include "vk_internal.h"
 
@@ -121,9 +122,9 @@ int make_out_map(CUtensorMap* map, void* c, int64_t m, int64_t n, long long ldc,
     return make_map(map, c, m, n, ldc, esize, 64 / esize, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// Clusters of 1 to 4 pairs of each kernel that fit on each device (0: not asked yet; the kernel's shared-memory attribute
-// is set by then).
-constexpr int kKernels = 16, kDevices = 64;
+// Clusters of 2, 4, 6 and 8 CTAs of each kernel that fit on each device (0: not asked yet; the kernel's shared-memory
+// attribute is set by then).
+constexpr int kKernels = 32, kDevices = 64;
 std::atomic<int> g_clusters[kKernels][kDevices][4];
 
 template <typename Kernel>
@@ -456,6 +457,22 @@ static int launch_gemm(F8GemmParams p, const CUtensorMap& ta, const CUtensorMap&
     return launch_clusters(gemm_fp8_kernel<OUT>, clusters, 2 * p.work.pairs, kF8Threads, kF8SmemBytes, stream, ta, tb, tc, p);
 }
 
+template <int NPAD, int OUT>
+static int launch_thin(ThinParams p, const CUtensorMap& tb, const CUtensorMap& ta, cudaStream_t stream)
+{
+    using Cfg = ThinCfg<NPAD>;
+    constexpr int kId = 16 + 3 * (NPAD == 16 ? 0 : NPAD == 32 ? 1 : 2) + OUT;
+    int fit[4];
+    const int rc = prepare_kernel(gemm_fp8_thin_kernel<NPAD, OUT>, kId, Cfg::kSmemBytes, kThinThreads, fit);
+    if (rc != VK_OK) return rc;
+    // as many CTAs to a tile as can all run at once, with two k-blocks each at least
+    const int tiles = static_cast<int>((static_cast<int64_t>(p.N) + 127) / 128), num_kb = (p.K + 127) / 128;
+    p.slices = 1;
+    for (int i = 3; i >= 0 && p.slices == 1; --i)
+        if (tiles <= fit[i] && num_kb >= 4 * (i + 1)) p.slices = 2 * (i + 1);
+    return launch_clusters(gemm_fp8_thin_kernel<NPAD, OUT>, tiles, p.slices, kThinThreads, Cfg::kSmemBytes, stream, tb, ta, p);
+}
+
 // Scales as the tensor-core kernels read them: strides per output index (or tile) and per k-block.
 static ScaleSource scales(const void* p, long long ld, int64_t count, int scaling, bool along_row)
 {
@@ -500,6 +517,31 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     if (a->k > 0 && tma_ok(a->A, lda, 1) && tma_ok(a->B, ldb, 1)) {
+        if (a->trans_b && a->m <= 64) {
+            ThinParams p;
+            p.M = static_cast<int>(a->m);
+            p.N = static_cast<int>(a->n);
+            p.K = static_cast<int>(a->k);
+            p.sa = scales(a->a_scale, ldas, a->m, a->a_scaling, true);
+            p.sb = scales(a->b_scale, ldbs, a->n, a->b_scaling, true);
+            p.C = a->C;
+            p.ldc = ldc;
+            p.timeout_ns = wait_timeout_ns();
+            const int npad = a->m <= 16 ? 16 : a->m <= 32 ? 32 : 64;
+            CUtensorMap tb, ta;
+            rc = make_map(&tb, a->B, a->n, a->k, ldb, 1, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+            if (rc == VK_OK) rc = make_map(&ta, a->A, a->m, a->k, lda, 1, 128, npad, CU_TENSOR_MAP_SWIZZLE_128B);
+            if (rc != VK_OK) return rc;
+            auto launch = [&](auto out) {
+                constexpr int kOut = decltype(out)::value;
+                return npad == 16   ? launch_thin<16, kOut>(p, tb, ta, stream)
+                       : npad == 32 ? launch_thin<32, kOut>(p, tb, ta, stream)
+                                    : launch_thin<64, kOut>(p, tb, ta, stream);
+            };
+            return a->dtype == VK_DTYPE_F16   ? launch(std::integral_constant<int, VK_DTYPE_F16>())
+                   : a->dtype == VK_DTYPE_F32 ? launch(std::integral_constant<int, VK_DTYPE_F32>())
+                                              : launch(std::integral_constant<int, VK_DTYPE_BF16>());
+        }
         const int64_t tiles = (a->m + 255) / 256 * ((a->n + 255) / 256);
         if (tiles > kMaxDim) return set_error(VK_ERR_UNSUPPORTED, "%s: too many tiles", name);
         F8GemmParams p;

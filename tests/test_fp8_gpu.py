@@ -334,6 +334,15 @@ def test_gemm_waves(vk, shape, layout):
     test_gemm(vk, shape, layout, BF16)
 
 
+# few rows of A: clusters of every size, more tiles than SMs, more k than fits in flight
+@pytest.mark.parametrize("shape", [(1, 500, 4096), (16, 1500, 1600), (17, 2000, 5000), (40, 3000, 1000), (5, 4096, 4096), (64, 20000, 300),
+                                   (2, 300, 20000)])
+@pytest.mark.parametrize("layout", ["nt_tile", "nt_row"])
+def test_gemm_few_rows(vk, shape, layout):
+    test_gemm(vk, shape, layout, F16)
+    test_gemm(vk, shape, layout, F32)
+
+
 @pytest.mark.parametrize("m", [4, 200])
 def test_gemm_tile_scales_of_a(vk, m):
     a, sa = _quantized((m, 1000), 32, True)

@@ -21,7 +21,7 @@ CSRC = os.path.join(ROOT, "task-1", "src", "vkgemm")
 LIB = os.path.join(HERE, "libvkgemm.so")
 SOURCES = ["vkgemm.cu", "sharded.cu", "host_gemm.cu", "peer_ipc.cu", "nvls.cu", "fp8.cu"]
 DEPS = SOURCES + ["ptx.cuh", "tc_gemm.cuh", "simt_gemm.cuh", "vk_internal.h", "fp8_rows.cuh", "fp8_simt.cuh",
-                  "fp8_gemm.cuh", "fp8_wgrad.cuh"]
+                  "fp8_gemm.cuh", "fp8_thin.cuh", "fp8_wgrad.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
