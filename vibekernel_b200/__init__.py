@@ -13,6 +13,7 @@ missing, importing this package raises; if no B200 is present, every GPU call ra
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -590,7 +591,7 @@ class _Fp8:
 
         import torch
         self.torch = torch
-        self.empty = torch.empty
+        self.empty = torch.empty_strided
         self.codes16 = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
         self.codes = {**self.codes16, torch.float32: DTYPE_F32}
         self.f16, self.f32, self.u8 = torch.float16, torch.float32, torch.uint8
@@ -668,9 +669,14 @@ def _vector(t, what: str, device: int, dtype, n: int) -> int:
 
 def _new_q(F, rows: int, cols: int, device):
     """A new 8-bit matrix whose rows start at 16-byte boundaries (what the tensor-core kernels' loads need)."""
-    pitch = (cols + 15) // 16 * 16
-    q = F.empty((rows, pitch), dtype=F.q, device=device)
-    return q if pitch == cols else q[:, :cols]
+    return F.empty((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=F.q, device=device)
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(rows: int, cols: int) -> int:
+    need = ctypes.c_size_t(0)
+    check(lib.vk_rmsnorm_fp8_workspace(rows, cols, ctypes.byref(need)))
+    return need.value
 
 
 def quantize_fp8(x, *, tile: bool = False, q=None, scale=None, stream=None):
@@ -701,7 +707,7 @@ def quantize_fp8(x, *, tile: bool = False, q=None, scale=None, stream=None):
     else:
         ldq = _matrix(q, "q", index, F.q, (rows, cols))[2]
     if scale is None:
-        scale = F.empty(s_shape, dtype=F.scale, device=device)
+        scale = F.empty(s_shape, (s_shape[1], 1), dtype=F.scale, device=device)
         lds = s_shape[1]
     else:
         lds = _matrix(scale, "scale", index, F.scale, s_shape)[2]
@@ -737,7 +743,7 @@ def rmsnorm_fp8(x, weight, *, residual=None, eps: float = 1e-6, q=None, scale=No
     if residual is not None:
         ldr = _matrix(residual, "residual", index, dtype, (rows, cols))[2]
         if h is None:
-            h = F.empty((rows, cols), dtype=dtype, device=device)
+            h = F.empty((rows, cols), (cols, 1), dtype=dtype, device=device)
             ldh = cols
         else:
             ldh = _matrix(h, "h", index, dtype, (rows, cols))[2]
@@ -752,12 +758,12 @@ def rmsnorm_fp8(x, weight, *, residual=None, eps: float = 1e-6, q=None, scale=No
     else:
         ldq = _matrix(q, "q", index, F.q, (rows, cols))[2]
     if scale is None:
-        scale = F.empty((rows, blocks), dtype=F.scale, device=device)
+        scale = F.empty((rows, blocks), (blocks, 1), dtype=F.scale, device=device)
         lds = blocks
     else:
         lds = _matrix(scale, "scale", index, F.scale, (rows, blocks))[2]
     if rstd is None:
-        rstd = F.empty((rows,), dtype=F.f32, device=device)
+        rstd = F.empty((rows,), (1,), dtype=F.f32, device=device)
         rstd_ptr = rstd.data_ptr()
     else:
         rstd_ptr = _vector(rstd, "rstd", index, F.f32, rows)
@@ -794,21 +800,20 @@ def rmsnorm_fp8_backward(dy, h, weight, rstd, *, dres=None, dx=None, dweight=Non
         ldr = _matrix(dres, "dres", index, dtype, (rows, cols))[2]
         dres_ptr = dres.data_ptr()
     if dx is None:
-        dx = F.empty((rows, cols), dtype=dtype, device=device)
+        dx = F.empty((rows, cols), (cols, 1), dtype=dtype, device=device)
         lddx = cols
     else:
         lddx = _matrix(dx, "dx", index, dtype, (rows, cols))[2]
     if dweight is None:
-        dweight = F.empty((cols,), dtype=F.f32, device=device)
+        dweight = F.empty((cols,), (1,), dtype=F.f32, device=device)
         dw_ptr = dweight.data_ptr()
     else:
         dw_ptr = _vector(dweight, "dweight", index, F.f32, cols)
-    need = ctypes.c_size_t(0)
-    check(lib.vk_rmsnorm_fp8_workspace(rows, cols, ctypes.byref(need)))
+    need = _norm_workspace(rows, cols)
     # from torch's allocator for this stream, so that a captured graph keeps it
-    work = F.empty((need.value,), dtype=F.u8, device=device)
+    work = F.empty((need,), (1,), dtype=F.u8, device=device)
     fn, pack = F.rmsnorm_fp8_backward
-    check(fn(pack(dy.data_ptr(), h.data_ptr(), w_ptr, rstd_ptr, dres_ptr, dx.data_ptr(), dw_ptr, work.data_ptr(), need.value, rows, cols,
+    check(fn(pack(dy.data_ptr(), h.data_ptr(), w_ptr, rstd_ptr, dres_ptr, dx.data_ptr(), dw_ptr, work.data_ptr(), need, rows, cols,
                   lddy, ldh, ldr, lddx, code, F.raw_stream(index))))
     return dx, dweight
 
@@ -855,7 +860,7 @@ def gemm_fp8(A, a_scale, B, b_scale, C=None, *, trans_b: bool = False, out_dtype
     if code is None:
         raise TypeError(f"out_dtype must be float16, bfloat16 or float32, not {out_dtype}")
     if C is None:
-        C = F.empty((m, n), dtype=out_dtype, device=device)
+        C = F.empty((m, n), (n, 1), dtype=out_dtype, device=device)
         ldc = n
     else:
         ldc = _matrix(C, "C", index, out_dtype, (m, n))[2]
@@ -895,7 +900,7 @@ def wgrad_fp8(dY, X, x_scale, dW=None, *, accumulate: bool = False, out_dtype=No
     if out_code is None:
         raise TypeError(f"out_dtype must be float16, bfloat16 or float32, not {out_dtype}")
     if dW is None:
-        dW = F.empty((n, k), dtype=out_dtype, device=device)
+        dW = F.empty((n, k), (k, 1), dtype=out_dtype, device=device)
         lddw = k
     else:
         lddw = _matrix(dW, "dW", index, out_dtype, (n, k))[2]
