@@ -70,15 +70,18 @@ struct Work {
 __host__ __device__ __forceinline__ int work_units(const TileWork& w) { return w.tiles_m * w.tiles_n + w.halved; }
 
 // Unit u; `part`: which of w.pairs this pair is.
-__host__ __device__ __forceinline__ Work work_unit(const TileWork& w, int u, int part)
+__device__ __forceinline__ Work work_unit(const TileWork& w, int u, int part)
 {
     Work r;
     const int whole = w.tiles_m * w.tiles_n - w.halved;
     const int t = u < whole ? u : whole + (u - whole) / 2;
     const int grains = (w.stages + w.grain - 1) / w.grain;
-    r.st0 = static_cast<int>(static_cast<long long>(grains) * part / w.pairs) * w.grain;
-    r.st1 = static_cast<int>(static_cast<long long>(grains) * (part + 1) / w.pairs) * w.grain;
-    if (r.st1 > w.stages) r.st1 = w.stages;
+    r.st0 = 0;
+    r.st1 = w.stages;
+    if (w.pairs > 1) {
+        r.st0 = grains * part / w.pairs * w.grain;
+        r.st1 = min(w.stages, grains * (part + 1) / w.pairs * w.grain);
+    }
     const int per_group = w.raster_group * w.tiles_n;
     const int g = t / per_group;
     const int first_m = g * w.raster_group;
