@@ -445,12 +445,16 @@ __global__ void __launch_bounds__(kF8Threads, 1)
                         const int kk_end = min(8, (p.K - st * 256 + 31) / 32);
                         const uint32_t id0 = static_cast<uint32_t>(st & 1) * 2;  // scale bytes of this stage's two k-blocks
                         const uint32_t idesc = (w.cols == 256 ? kIdesc : kIdescHalf) | (id0 << 4) | (id0 << 29);
-#pragma unroll
-                        for (int kk = 0; kk < 8; ++kk) {
-                            if (kk >= kk_end) break;
+                        auto mma = [&](int kk) {
                             umma_mxf8_pair(d, a + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4),
                                            b + ((B_K ? (kk >> 2) * (128 * 128) + (kk & 3) * 32 : kk * 32 * 128) >> 4),
                                            idesc + (kk >> 2) * ((1u << 4) | (1u << 29)), sfa, sfb, st != w.st0 || kk != 0);
+                        };
+                        if (kk_end == 8) {
+#pragma unroll
+                            for (int kk = 0; kk < 8; ++kk) mma(kk);
+                        } else {
+                            for (int kk = 0; kk < kk_end; ++kk) mma(kk);
                         }
                         umma_commit_pair(empty_bar(r.at), lead);
                         if (last) umma_commit_pair(sf_empty_bar(sf.at), lead);

@@ -135,10 +135,12 @@ __global__ void __launch_bounds__(kThinThreads, 1)
                 const uint64_t a = desc + static_cast<uint32_t>(r.at) * (Cfg::kStageBytes >> 4), b = a + (128 * 128 >> 4);
                 const uint32_t idesc = kIdesc | (static_cast<uint32_t>(in) << 4) | (static_cast<uint32_t>(in) << 29);
                 const int kk_end = min(4, (p.K - kb * 128 + 31) / 32);
+                auto mma = [&](int kk) { umma_mxf8(base, a + (kk * 32 >> 4), b + (kk * 32 >> 4), idesc, sfa, sfb, kb != kb0 || kk != 0); };
+                if (kk_end == 4) {
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    if (kk >= kk_end) break;
-                    umma_mxf8(base, a + (kk * 32 >> 4), b + (kk * 32 >> 4), idesc, sfa, sfb, kb != kb0 || kk != 0);
+                    for (int kk = 0; kk < 4; ++kk) mma(kk);
+                } else {
+                    for (int kk = 0; kk < kk_end; ++kk) mma(kk);
                 }
                 umma_commit<1>(empty_bar(r.at));
                 if (last) umma_commit<1>(sf_empty_bar(sf.at));

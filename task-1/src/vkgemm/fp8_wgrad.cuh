@@ -38,7 +38,7 @@ struct WgradParams {
 constexpr int kWgStages = 3, kWgBK = 128;
 constexpr int kWgABytes = 128 * kWgBK * 2;
 constexpr int kWgBBytes = 128 * kWgBK * 2;
-constexpr int kWgBars = 3 * kWgStages + 4;
+constexpr int kWgBars = 2 * kWgStages + 4;
 constexpr int kWgSmemBytes = 1024 + kWgStages * (kWgABytes + kWgBBytes) + 4 * kF8EpiWarpBytes + kWgBars * 8 + 16;
 constexpr int kWgThreads = 192 + 128 * kWgStages;
 static_assert(kWgSmemBytes <= 232448, "shared memory per CTA");
@@ -88,11 +88,10 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kWgBars);
 
     const uint32_t bar0 = smem_u32(bars);
-    auto full_bar = [&](int s) { return bar0 + 8u * s; };                 // dY loaded
-    auto ready_bar = [&](int s) { return bar0 + 8u * (kWgStages + s); };  // X's values written
-    auto empty_bar = [&](int s) { return bar0 + 8u * (2 * kWgStages + s); };
-    auto tfull_bar = [&](int a) { return bar0 + 8u * (3 * kWgStages + a); };
-    auto tempty_bar = [&](int a) { return bar0 + 8u * (3 * kWgStages + 2 + a); };
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (kWgStages + s); };
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * kWgStages + a); };
+    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kWgStages + 2 + a); };
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -107,8 +106,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         prefetch_tmap(&tmap_a);
         if (p.c_tma) prefetch_tmap(&tmap_c);
         for (int s = 0; s < kWgStages; ++s) {
-            mbar_init(full_bar(s), 1);
-            mbar_init(ready_bar(s), 8);  // the stage's four conversion warps of both CTAs
+            mbar_init(full_bar(s), 9);  // dY's bytes, and the stage's four conversion warps of both CTAs
             mbar_init(empty_bar(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -170,20 +168,21 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 const uint32_t d = base + static_cast<uint32_t>(acc * 256);
                 const uint32_t idesc = w.cols == 256 ? kIdesc : kIdescHalf;
                 for (int st = w.st0; st < w.st1; ++st, r.next()) {
-                    if (!mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at) ||
-                        !mbar_wait_warp(ready_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, 200 + r.at)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at);
+                    if (!ok) break;
                     tc_fence_after();
                     if (one) {
                         const uint64_t a = a_desc + static_cast<uint32_t>(r.at) * (kWgABytes >> 4);
                         const uint64_t b = b_desc + static_cast<uint32_t>(r.at) * (kWgBBytes >> 4);
                         const int kk_end = min(kWgBK / 16, (p.K - st * kWgBK + 15) / 16);
-#pragma unroll
-                        for (int kk = 0; kk < kWgBK / 16; ++kk) {
-                            if (kk >= kk_end) break;
+                        auto mma = [&](int kk) {
                             umma_f16<2>(d, a + (kk * 16 * 128 >> 4), b + (kk * 16 * 128 >> 4), idesc, (st != w.st0 || kk != 0) ? 1u : 0u);
+                        };
+                        if (kk_end == kWgBK / 16) {
+#pragma unroll
+                            for (int kk = 0; kk < kWgBK / 16; ++kk) mma(kk);
+                        } else {
+                            for (int kk = 0; kk < kk_end; ++kk) mma(kk);
                         }
                         umma_commit_pair(empty_bar(r.at), lead);
                         if (st + 1 == w.st1) umma_commit_pair(tfull_bar(acc), lead);
@@ -265,7 +264,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                 convert(std::false_type{}, dst);
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive_pair(mapa_shared(ready_bar(group), lead));
+            if (lane == 0) mbar_arrive_pair(mapa_shared(full_bar(group), lead));
             phase ^= 1u;
             step(kWgStages);
             if (u < units) fetch();  // behind the fence, which would wait for the loads
