@@ -113,9 +113,11 @@ int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, lon
 
 bool tma_ok(const void* p, long long ld, int esize) { return rows_at(p, ld, esize, 16) && ld * esize < (1LL << 40); }
 
-int make_out_map(CUtensorMap* map, void* c, int64_t m, int64_t n, long long ldc, int dtype, int* c_tma)
+int make_out_map(CUtensorMap* map, void* c, int64_t m, int64_t n, long long ldc, int dtype, int* c_tma, int* c_width)
 {
     const int esize = static_cast<int>(bytes_of(dtype));
+    *c_width = 16;
+    while (*c_width > 1 && !rows_at(c, ldc, esize, *c_width)) *c_width /= 2;
     memset(map, 0, sizeof(*map));
     *c_tma = tma_ok(c, ldc, esize);
     if (!*c_tma) return VK_OK;
@@ -367,16 +369,20 @@ extern "C" int vk_rmsnorm_fp8_workspace(int64_t rows, int64_t cols, size_t* byte
 // Shared memory per SM that the rows in flight may take.
 constexpr int kNormBackBytes = 208 * 1024;
 
-template <typename T, int NV>
+template <typename T, int NV, bool VEC>
 static int launch_norm_backward(NormBackParams p, int id, const NormBackPlan& plan, cudaStream_t stream)
 {
+    if (!VEC) {
+        rmsnorm_fp8_backward_kernel<T, NV, VEC><<<static_cast<unsigned>(plan.parts), plan.threads, 0, stream>>>(p);
+        return launched();
+    }
     const int pitch = (p.cols * 2 + 127) / 128 * 128;
     int clusters[4];
-    const int rc = prepare_kernel(rmsnorm_fp8_backward_kernel<T, NV>, id, kNormBackBytes / (NV == 1 ? 2 : 1), 512, clusters);
+    const int rc = prepare_kernel(rmsnorm_fp8_backward_kernel<T, NV, VEC>, id, kNormBackBytes / (NV == 1 ? 2 : 1), 512, clusters);
     if (rc != VK_OK) return rc;
     p.stages = kNormBackBytes / plan.per_sm / (3 * pitch);
     if (p.stages > 8) p.stages = 8;
-    rmsnorm_fp8_backward_kernel<T, NV><<<static_cast<unsigned>(plan.parts), plan.threads, p.stages * 3 * pitch, stream>>>(p);
+    rmsnorm_fp8_backward_kernel<T, NV, VEC><<<static_cast<unsigned>(plan.parts), plan.threads, p.stages * 3 * pitch, stream>>>(p);
     return launched();
 }
 
@@ -423,8 +429,10 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
         rc = for_type(a->dtype, [&](auto t) {
             using T = std::conditional_t<std::is_same_v<decltype(t), __half>, __half, __nv_bfloat16>;
             constexpr int kId = 9 + (std::is_same_v<T, __half> ? 0 : 2);
-            if (vec && plan.nv == 1) return launch_norm_backward<T, 1>(p, kId, plan, stream);
-            if (vec && plan.nv == 2) return launch_norm_backward<T, 2>(p, kId + 1, plan, stream);
+            if (plan.nv == 1)
+                return vec ? launch_norm_backward<T, 1, true>(p, kId, plan, stream) : launch_norm_backward<T, 1, false>(p, 0, plan, stream);
+            if (plan.nv == 2)
+                return vec ? launch_norm_backward<T, 2, true>(p, kId + 1, plan, stream) : launch_norm_backward<T, 2, false>(p, 0, plan, stream);
             rmsnorm_fp8_backward_any_kernel<T><<<static_cast<unsigned>(plan.parts), 512, 0, stream>>>(p);
             return launched();
         });
@@ -563,7 +571,7 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
         if (rc == VK_OK)
             rc = a->trans_b ? make_map(&tb, a->B, a->n, a->k, ldb, 1, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B)
                             : make_map(&tb, a->B, a->k, a->n, ldb, 1, 128, 256, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc == VK_OK) rc = make_out_map(&tc, a->C, a->m, a->n, ldc, a->dtype, &p.c_tma);
+        if (rc == VK_OK) rc = make_out_map(&tc, a->C, a->m, a->n, ldc, a->dtype, &p.c_tma, &p.c_width);
         if (rc != VK_OK) return rc;
         return a->dtype == VK_DTYPE_F16   ? launch_gemm<VK_DTYPE_F16>(p, ta, tb, tc, stream)
                : a->dtype == VK_DTYPE_F32 ? launch_gemm<VK_DTYPE_F32>(p, ta, tb, tc, stream)
@@ -639,7 +647,7 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
         p.timeout_ns = wait_timeout_ns();
         CUtensorMap ta, tc;
         rc = make_map(&ta, a->dY, a->tokens, a->n, lddy, 2, 64, kWgBK, CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc == VK_OK) rc = make_out_map(&tc, a->dW, a->n, a->k, lddw, a->out_dtype, &p.c_tma);
+        if (rc == VK_OK) rc = make_out_map(&tc, a->dW, a->n, a->k, lddw, a->out_dtype, &p.c_tma, &p.c_width);
         if (rc != VK_OK) return rc;
         return for_type(a->dtype, [&](auto t) {
             using T = std::conditional_t<std::is_same_v<decltype(t), __half>, __half, __nv_bfloat16>;

@@ -100,7 +100,7 @@ struct F8GemmParams {
     int b_k;                       // B stored n x k
     void* C;
     long long ldc;
-    int c_tma;                     // C can take TMA stores
+    int c_tma, c_width;            // see BoxOut
     unsigned long long timeout_ns;
 };
 
@@ -110,7 +110,7 @@ constexpr int kF8BBytes = 128 * 256;
 constexpr int kF8StageBytes = kF8ABytes + kF8BBytes;
 constexpr int kF8SfSlots = 3;
 constexpr int kF8SfBytes = 512 + 1024;  // a slot: A's unit, B's two
-constexpr int kF8EpiWarpBytes = 4096;   // two boxes of 32 rows x 64 bytes
+constexpr int kF8EpiWarpBytes = 4096;   // two boxes of 32 rows x 64 bytes, or one with rows 80 bytes apart
 constexpr int kF8Bars = 2 * kF8Stages + 3 + 2 * kF8SfSlots;
 constexpr int kF8SmemBytes =
     1024 + kF8Stages * kF8StageBytes + 4 * kF8EpiWarpBytes + kF8SfSlots * kF8SfBytes + kF8Bars * 8 + 16;
@@ -172,45 +172,91 @@ struct BoxOut {
     int M, N;
     int c_tma;               // C can take TMA stores (and 16-byte accesses)
     int accumulate;          // C += the results
+    int width;               // bytes that divide C's address and the distance of its rows (1, 2, 4 or 8 without TMA stores)
 };
+
+// Results of one row that leave together: 64 bytes.
+struct Packed {
+    uint4 w[4];
+};
+
+// A C that cannot take TMA stores: a warp's 32 rows go through the staging buffer, 80 bytes apart, to runs of 64 bytes
+// per row from column col, in the widest stores W that C's alignment allows.  (Each lane its own row: 4001 x 3333 x 2999
+// bf16 167 us, against 47.)  Not inlined: its registers would be taken from the kernels' other roles.
+template <typename T, typename W>
+__device__ __noinline__ void put_rows(T* C, long long ldc, int rows, int cols, uint8_t* stg, int lane, Packed p)
+{
+    constexpr int kLanes = 64 / sizeof(W), kRows = 32 / kLanes, kCount = sizeof(W) / sizeof(T);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stg + lane * 80 + j * 16) = p.w[j];
+    __syncwarp();
+    const int at = lane % kLanes, first = at * kCount, count = min(kCount, cols - first);
+    const int left = rows - lane / kLanes;
+    const uint8_t* from = stg + lane / kLanes * 80 + at * sizeof(W);
+    T* to = C + lane / kLanes * ldc + first;
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 8 * kRows) {
+        W v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (r0 + i * kRows < 32) v[i] = *reinterpret_cast<const W*>(from + (r0 + i * kRows) * 80);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + i * kRows;
+            if (r >= 32 || r >= left) continue;
+            if (count == kCount) {
+                *reinterpret_cast<W*>(to + r * ldc) = v[i];
+            } else {
+                for (int e = 0; e < count; ++e) to[r * ldc + e] = reinterpret_cast<const T*>(from + r * 80)[e];
+            }
+        }
+    }
+}
 
 // Results col .. col + 31 of this lane's row (row0 + lane).  Two boxes of staging take turns; `turn` counts them.
 template <int OUT>
 __device__ __forceinline__ void store_box(const BoxOut& o, uint8_t* stg, int row0, int lane, int col, float (&f)[32], uint32_t& turn)
 {
     using T = std::conditional_t<OUT == 0, __half, std::conditional_t<OUT == 1, float, __nv_bfloat16>>;
+    constexpr int kCols = 64 / sizeof(T);  // of a box
     const int row = row0 + lane;
-    T* c = static_cast<T*>(o.C) + static_cast<long long>(row) * o.ldc + col;
     if (o.accumulate && row < o.M) {
+        const T* c = static_cast<const T*>(o.C) + static_cast<long long>(row) * o.ldc + col;
+        if (o.c_tma && col + 32 <= o.N) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = o.N - col - 8 * j;
-            const Vec8<T> v = o.c_tma && n >= 8 ? load8<true>(c + 8 * j, n) : load8<false>(c + (n > 0 ? 8 * j : 0), n);
+            for (int j = 0; j < 4; ++j) {
+                const Vec8<T> v = load8<true>(c, 8 * j, 32);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[8 * j + i] += to_f32(v.v[i]);
+                for (int i = 0; i < 8; ++i) f[8 * j + i] += to_f32(v.v[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (col + i < o.N) f[i] += to_f32(c[i]);
         }
     }
-    if (o.c_tma) {
-        constexpr int kCols = 64 / sizeof(T);  // of a box
 #pragma unroll
-        for (int h = 0; h < 32 / kCols; ++h) {
-            if (col + h * kCols >= o.N) break;
+    for (int h = 0; h < 32 / kCols; ++h) {
+        if (col + h * kCols >= o.N) break;
+        Packed p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (OUT == 1) {
+                const float* g = f + 16 * h + 4 * j;
+                p.w[j] = make_uint4(__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]), __float_as_uint(g[3]));
+            } else {
+                p.w[j] = make_uint4(pack16<OUT>(f[8 * j], f[8 * j + 1]), pack16<OUT>(f[8 * j + 2], f[8 * j + 3]),
+                                    pack16<OUT>(f[8 * j + 4], f[8 * j + 5]), pack16<OUT>(f[8 * j + 6], f[8 * j + 7]));
+            }
+        }
+        if (o.c_tma) {
             uint8_t* box = stg + (turn & 1u) * 2048;
             if (lane == 0) bulk_wait_group_read<1>();
             __syncwarp();
             uint4* to = reinterpret_cast<uint4*>(box + lane * 64);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint4 v;
-                if constexpr (OUT == 1) {
-                    const float* g = f + 16 * h + 4 * j;
-                    v = make_uint4(__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]), __float_as_uint(g[3]));
-                } else {
-                    v = make_uint4(pack16<OUT>(f[8 * j], f[8 * j + 1]), pack16<OUT>(f[8 * j + 2], f[8 * j + 3]),
-                                   pack16<OUT>(f[8 * j + 4], f[8 * j + 5]), pack16<OUT>(f[8 * j + 6], f[8 * j + 7]));
-                }
-                to[j ^ ((lane >> 1) & 3)] = v;  // the 64-byte swizzle
-            }
+            for (int j = 0; j < 4; ++j) to[j ^ ((lane >> 1) & 3)] = p.w[j];  // the 64-byte swizzle
             ++turn;
             fence_proxy_async_smem();
             __syncwarp();
@@ -218,13 +264,17 @@ __device__ __forceinline__ void store_box(const BoxOut& o, uint8_t* stg, int row
                 tma_store_2d(o.map, smem_u32(box), col + h * kCols, row0);
                 bulk_commit_group();
             }
+            continue;
         }
-        return;
+        const int first = col + h * kCols;
+        T* c = static_cast<T*>(o.C) + static_cast<long long>(row0) * o.ldc + first;
+        if (sizeof(T) == 2 && o.width <= 2)
+            put_rows<T, std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>>(c, o.ldc, o.M - row0, o.N - first, stg, lane, p);
+        else if (o.width <= 4)
+            put_rows<T, uint32_t>(c, o.ldc, o.M - row0, o.N - first, stg, lane, p);
+        else
+            put_rows<T, uint2>(c, o.ldc, o.M - row0, o.N - first, stg, lane, p);
     }
-    if (row >= o.M) return;
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-        if (col + i < o.N) c[i] = from_f32<T>(f[i]);
 }
 
 __device__ __forceinline__ void tmem_chunk(uint32_t addr, float (&f)[32])
@@ -508,7 +558,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
 
     const bool epilogue = warp >= 2 && warp < 6;
     const int q = warp & 3;  // the lane quarter an epilogue warp may read
-    const BoxOut out{&tmap_c, p.C, p.ldc, p.M, p.N, p.c_tma, 0};
+    const BoxOut out{&tmap_c, p.C, p.ldc, p.M, p.N, p.c_tma, 0, p.c_width};
     uint8_t* stg = epi + q * kF8EpiWarpBytes;
     float4* sums = reinterpret_cast<float4*>(sA);  // of a shared tile: its stages have all been read by then
     uint32_t turn = 0;

@@ -42,38 +42,77 @@ struct alignas(16) Vec8 {
     T v[8];
 };
 
-// n elements (the rest become zeros).  VEC: n is at least 8 or at most 0, and the address is 16-byte aligned; then the
-// load is one predicated instruction, and several stay in flight together.
+// Elements c .. c + 7 of a row that begins at `row` and has `cols` (those it does not have become zeros).
+// VEC: rows are 16-byte aligned and cols a multiple of 8; the load is one predicated instruction, and several stay in
+// flight together.  Otherwise the two aligned 16-byte units around the elements are loaded and shifted where both lie
+// in the row, and single elements at its ends (rows of 3333 bf16: norm 56 -> 35 us against single elements everywhere).
 template <bool VEC, typename T>
-__device__ __forceinline__ Vec8<T> load8(const T* src, int n)
+__device__ __forceinline__ Vec8<T> load8(const T* row, int c, int cols)
 {
     Vec8<T> r;
+    uint4* d = reinterpret_cast<uint4*>(&r);
+    const int n = cols - c;
+    const T* src = row + (n > 0 ? c : 0);
     if constexpr (VEC) {
         const uint4* s = reinterpret_cast<const uint4*>(src);
-        uint4* d = reinterpret_cast<uint4*>(&r);
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) d[i] = n > 0 ? s[i] : make_uint4(0, 0, 0, 0);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.v[i] = i < n ? src[i] : from_f32<T>(0.f);
+        return r;
     }
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src)) & 15u;
+    if (sizeof(T) == 2 && ((off == 0 && n >= 8) || (c >= 8 && n >= 16))) {
+        const uint4* s = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(src) - off);
+        const uint4 lo = s[0], hi = off ? s[1] : make_uint4(0, 0, 0, 0);
+        uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (off & 8u) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+        }
+        if (off & 4u) {
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+        }
+        const uint32_t bits = (off & 2u) * 8;
+        *d = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                        __funnelshift_r(w[3], w[4], bits));
+        return r;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = i < n ? src[i] : from_f32<T>(0.f);
     return r;
 }
 
+// The same elements back.
 template <bool VEC, typename T>
-__device__ __forceinline__ void store8(T* dst, const Vec8<T>& r, int n)
+__device__ __forceinline__ void store8(T* row, int c, int cols, const Vec8<T>& r)
 {
+    const int n = cols - c;
+    if (n <= 0) return;
+    T* dst = row + c;
     if constexpr (VEC) {
-        if (n <= 0) return;
         const uint4* s = reinterpret_cast<const uint4*>(&r);
         uint4* d = reinterpret_cast<uint4*>(dst);
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) d[i] = s[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) dst[i] = r.v[i];
+        return;
     }
+    if (sizeof(T) == 2 && n >= 8) {  // as 32-bit pairs, with a single element at both ends when the row begins between two
+        const uint4 v = *reinterpret_cast<const uint4*>(&r);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if ((reinterpret_cast<uintptr_t>(dst) & 2u) == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(dst)[i] = w[i];
+        } else {
+            dst[0] = r.v[0];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) *reinterpret_cast<uint32_t*>(dst + 1 + 2 * i) = __funnelshift_r(w[i], w[i + 1], 16);
+            dst[7] = r.v[7];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) dst[i] = r.v[i];
 }
 
 // |v| as an integer that orders like the number, NaN above infinity above every finite value.
@@ -102,7 +141,7 @@ __device__ __forceinline__ uint32_t pack_e4m3(float2 a, float2 b)
     return lo | (hi << 16);
 }
 
-// Eight values of a block with this scale as e4m3 bytes; n of them are written.  VEC as above, and 8-byte alignment.
+// Eight values of a block with this scale as e4m3 bytes; n of them are written.  VEC: 8 or none, and 8-byte aligned.
 template <bool VEC>
 __device__ __forceinline__ void store_q8(uint8_t* dst, const float (&f)[8], uint32_t s, int n)
 {
@@ -110,9 +149,9 @@ __device__ __forceinline__ void store_q8(uint8_t* dst, const float (&f)[8], uint
     uint2 w;
     w.x = pack_e4m3(__fmul2_rn(make_float2(f[0], f[1]), make_float2(inv, inv)), __fmul2_rn(make_float2(f[2], f[3]), make_float2(inv, inv)));
     w.y = pack_e4m3(__fmul2_rn(make_float2(f[4], f[5]), make_float2(inv, inv)), __fmul2_rn(make_float2(f[6], f[7]), make_float2(inv, inv)));
-    if constexpr (VEC) {
-        if (n > 0) *reinterpret_cast<uint2*>(dst) = w;
-    } else {
+    if (VEC ? n > 0 : n >= 8 && (reinterpret_cast<uintptr_t>(dst) & 7u) == 0) {
+        *reinterpret_cast<uint2*>(dst) = w;
+    } else if (!VEC) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < n) dst[i] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
@@ -189,11 +228,11 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
     const long long row = item / quads + in / quads;
     const int blk = static_cast<int>(in % quads) * 4;
     const int c = blk * 128 + sub * 8;
-    const int left = row < p.rows ? p.cols - c : 0;
-    const T* x = static_cast<const T*>(p.x) + (left > 0 ? row * p.ldx + c : 0);
+    const int cols = row < p.rows ? p.cols : 0, left = cols - c;
+    const T* x = static_cast<const T*>(p.x) + (left > 0 ? row * p.ldx : 0);
     Vec8<T> v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = load8<VEC>(x + (left > 128 * j ? 128 * j : 0), left - 128 * j);
+    for (int j = 0; j < 4; ++j) v[j] = load8<VEC>(x, c + 128 * j, cols);
     uint32_t scales = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -223,8 +262,8 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const long long row = row0 + 16 * j;
-        const int n = row < p.rows ? p.cols - c : 0;
-        v[j] = load8<VEC>(x + (n > 0 ? row * p.ldx + c : 0), n);
+        const bool in = row < p.rows;
+        v[j] = load8<VEC>(x + (in ? row * p.ldx : 0), c, in ? p.cols : 0);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, top_of(v[j]));
@@ -293,15 +332,12 @@ __global__ void __launch_bounds__(NV == 1 ? 256 : 512) rmsnorm_fp8_kernel(const 
     Vec8<T> held[NV], res[NV], gain[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = (first + j * 32) * 8, n = p.cols - c, o = n > 0 ? c : 0;
-        held[j] = load8<VEC>(x + o, n);
-        if (p.residual != nullptr) res[j] = load8<VEC>(r + o, n);
+        const int c = (first + j * 32) * 8;
+        held[j] = load8<VEC>(x, c, p.cols);
+        if (p.residual != nullptr) res[j] = load8<VEC>(r, c, p.cols);
     }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = (first + j * 32) * 8;
-        gain[j] = load8<VEC>(w + (c < p.cols ? c : 0), p.cols - c);
-    }
+    for (int j = 0; j < NV; ++j) gain[j] = load8<VEC>(w, (first + j * 32) * 8, p.cols);
     float2 sq = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -309,7 +345,7 @@ __global__ void __launch_bounds__(NV == 1 ? 256 : 512) rmsnorm_fp8_kernel(const 
         if (p.residual != nullptr) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) held[j].v[i] = from_f32<T>(to_f32(held[j].v[i]) + to_f32(res[j].v[i]));
-            store8<VEC>(static_cast<T*>(p.h) + row * p.ldh + c, held[j], p.cols - c);
+            store8<VEC>(static_cast<T*>(p.h) + row * p.ldh, c, p.cols, held[j]);
         }
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
@@ -352,13 +388,13 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_long_kernel(const NormParams 
     const int nv = ((p.cols + 127) / 128 * 16 + 511) / 512;
     float sq = 0.f;
     for (int j = 0; j < nv; ++j) {
-        const int c = (threadIdx.x + j * 512) * 8, n = p.cols - c, o = n > 0 ? c : 0;
-        Vec8<T> a = load8<VEC>(x + o, n);
+        const int c = (threadIdx.x + j * 512) * 8;
+        Vec8<T> a = load8<VEC>(x, c, p.cols);
         if (p.residual != nullptr) {
-            const Vec8<T> b = load8<VEC>(r + o, n);
+            const Vec8<T> b = load8<VEC>(r, c, p.cols);
 #pragma unroll
             for (int i = 0; i < 8; ++i) a.v[i] = from_f32<T>(to_f32(a.v[i]) + to_f32(b.v[i]));
-            store8<VEC>(h + c, a, n);
+            store8<VEC>(h, c, p.cols, a);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -371,8 +407,8 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_long_kernel(const NormParams 
     if (threadIdx.x == 0) p.rstd[row] = rstd;
     const T* src = p.residual != nullptr ? h : x;  // this thread's own writes
     for (int j = 0; j < nv; ++j) {
-        const int c = (threadIdx.x + j * 512) * 8, n = p.cols - c, o = n > 0 ? c : 0;
-        const Vec8<T> a = load8<VEC>(src + o, n), gain = load8<VEC>(w + o, n);
+        const int c = (threadIdx.x + j * 512) * 8, n = p.cols - c;
+        const Vec8<T> a = load8<VEC>(src, c, p.cols), gain = load8<VEC>(w, c, p.cols);
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = to_f32(a.v[i]) * rstd * to_f32(gain.v[i]);
@@ -400,7 +436,7 @@ struct NormBackParams {
 };
 
 // dx = rstd * (g - xhat * mean(g * xhat)) + dres with g = dy * weight, xhat = h * rstd; dweight = sum over rows of
-// dy * xhat.  CTAs walk over the rows.  Here, any alignment and any number of columns: a thread adds its columns' share
+// dy * xhat.  CTAs walk over the rows.  Here, any number of columns: a thread adds its columns' share
 // of dweight in its CTA's row of `part` (each element belongs to one thread), and reads a row twice.
 template <typename T>
 __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const NormBackParams p)
@@ -429,10 +465,10 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const Nor
     }
 }
 
-// The same for aligned rows of at most 512 * 8 * NV columns, a multiple of 8.  Two CTAs or more per SM; rows arrive ahead
-// in shared memory (one bulk copy per tensor and row, p.stages rows deep), so that memory stays busy through the two
-// passes and the barrier of each row; dweight's share stays in registers.
-template <typename T, int NV>
+// The same for rows of at most 512 * 8 * NV columns; dweight's share stays in registers.  VEC (16-byte aligned rows, a
+// multiple of 8 columns): rows arrive ahead in shared memory, one bulk copy per tensor and row, p.stages rows deep, so
+// that memory stays busy through the two passes and the barrier of each row.  Otherwise from memory as they are needed.
+template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_kernel(const NormBackParams p)
 {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -448,7 +484,7 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_ker
         bulk_load(dst + pitch, static_cast<const T*>(p.h) + row * p.ldh, row_bytes, bar);
         if (p.dres) bulk_load(dst + 2 * pitch, static_cast<const T*>(p.dres) + row * p.lddres, row_bytes, bar);
     };
-    if (threadIdx.x == 0) {
+    if (VEC && threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) mbar_init(smem_u32(&bars[s]), 1);
         fence_mbar_init();
         fence_proxy_async_smem();
@@ -461,7 +497,7 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_ker
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int c = (threadIdx.x + j * threads) * 8;
-        gain[j] = load8<true>(w + (c < p.cols ? c : 0), p.cols - c);
+        gain[j] = load8<VEC>(w, c, p.cols);
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[j][i] = 0.f;
     }
@@ -470,39 +506,42 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_ker
     uint32_t phase = 0;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const float rstd = p.rstd[row];
-        if (!mbar_wait(smem_u32(&bars[stage]), phase, p.timeout_ns, kErrWaitProducer, stage)) break;
+        if (VEC && !mbar_wait(smem_u32(&bars[stage]), phase, p.timeout_ns, kErrWaitProducer, stage)) break;
         const uint8_t* base = smem + static_cast<size_t>(stage) * 3 * pitch;
-        Vec8<T> a[NV], b[NV];
+        const T* dy = VEC ? reinterpret_cast<const T*>(base) : static_cast<const T*>(p.dy) + row * p.lddy;
+        const T* h = VEC ? reinterpret_cast<const T*>(base + pitch) : static_cast<const T*>(p.h) + row * p.ldh;
+        const T* dres = VEC ? reinterpret_cast<const T*>(base + 2 * pitch) : static_cast<const T*>(p.dres) + row * p.lddres;
+        Vec8<T> a[NV], b[NV], d[NV];
         float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (threadIdx.x + j * threads) * 8, n = p.cols - c, o = n > 0 ? c * 2 : 0;
-            a[j] = load8<true>(reinterpret_cast<const T*>(base + o), n);
-            b[j] = load8<true>(reinterpret_cast<const T*>(base + pitch + o), n);
+            const int c = (threadIdx.x + j * threads) * 8;
+            a[j] = load8<VEC>(dy, c, p.cols);
+            b[j] = load8<VEC>(h, c, p.cols);
+            if (!VEC && p.dres) d[j] = load8<VEC>(dres, c, p.cols);
 #pragma unroll
             for (int i = 0; i < 8; ++i) dot = fmaf(to_f32(a[j].v[i]) * to_f32(gain[j].v[i]), to_f32(b[j].v[i]) * rstd, dot);
         }
         const float mean = cta_sum(dot, slots[turn]) * p.inv_cols;
         // Behind this barrier no thread reads the row before any more: its stage is free.
         const long long ahead = row + static_cast<long long>(p.stages - 1) * gridDim.x;
-        if (threadIdx.x == 0 && row != blockIdx.x && ahead < p.rows) issue(ahead, before);
+        if (VEC && threadIdx.x == 0 && row != blockIdx.x && ahead < p.rows) issue(ahead, before);
         T* dx = static_cast<T*>(p.dx) + row * p.lddx;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (threadIdx.x + j * threads) * 8, n = p.cols - c, o = n > 0 ? c * 2 : 0;
-            Vec8<T> d;
-            if (p.dres) d = load8<true>(reinterpret_cast<const T*>(base + 2 * pitch + o), n);
+            const int c = (threadIdx.x + j * threads) * 8;
+            if (VEC && p.dres) d[j] = load8<VEC>(dres, c, p.cols);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float dyf = to_f32(a[j].v[i]), xhat = to_f32(b[j].v[i]) * rstd;
                 float t = rstd * (dyf * to_f32(gain[j].v[i]) - xhat * mean);
-                if (p.dres) t += to_f32(d.v[i]);
-                d.v[i] = from_f32<T>(t);
+                if (p.dres) t += to_f32(d[j].v[i]);
+                d[j].v[i] = from_f32<T>(t);
                 acc[j][i] = fmaf(dyf, xhat, acc[j][i]);
             }
-            store8<true>(dx + c, d, n);
+            store8<VEC>(dx, c, p.cols, d[j]);
         }
-        fence_proxy_async_smem();  // read before the stage is written again
+        if (VEC) fence_proxy_async_smem();  // read before the stage is written again
         before = stage;
         if (++stage == p.stages) {
             stage = 0;
@@ -514,9 +553,15 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_ker
     for (int j = 0; j < NV; ++j) {
         const int c = (threadIdx.x + j * threads) * 8;
         if (c >= p.cols) continue;
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 4)
-            *reinterpret_cast<float4*>(part + c + i) = make_float4(acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]);
+            for (int i = 0; i < 8; i += 4)
+                *reinterpret_cast<float4*>(part + c + i) = make_float4(acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < p.cols) part[c + i] = acc[j][i];
+        }
     }
 }
 

@@ -31,7 +31,7 @@ struct WgradParams {
     long long ldx, lds;
     void* C;
     long long ldc;
-    int c_tma, accumulate;
+    int c_tma, c_width, accumulate;
     unsigned long long timeout_ns;
 };
 
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
 
     const bool epilogue = warp >= 2 && warp < 6;
     const int q = warp & 3;  // the lane quarter an epilogue warp may read
-    const BoxOut out{&tmap_c, p.C, p.ldc, p.M, p.N, p.c_tma, p.accumulate};
+    const BoxOut out{&tmap_c, p.C, p.ldc, p.M, p.N, p.c_tma, p.accumulate, p.c_width};
     uint8_t* stg = epi + q * kF8EpiWarpBytes;
     float4* sums = reinterpret_cast<float4*>(sA);  // of a shared tile: its stages have all been read by then
     uint32_t turn = 0;
