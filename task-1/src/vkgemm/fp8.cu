@@ -44,15 +44,24 @@ int bad_size(const char* name, const char* what, int64_t v)
                      (long long)v);
 }
 
-// A leading dimension of 0 stands for the row's length.
-int ld_of(const char* name, const char* what, int64_t given, int64_t row, long long* out)
+// A leading dimension of 0 stands for the row's length.  That of a single row means nothing, so it becomes one that
+// alignment cannot fail on.
+int ld_of(const char* name, const char* what, int64_t given, int64_t row, int64_t rows, long long* out)
 {
     *out = given ? given : row;
     if (given < 0 || *out < row)
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: %s = %lld is smaller than the row length %lld", name, what,
                          (long long)given, (long long)row);
     if (*out > (1LL << 40)) return set_error(VK_ERR_UNSUPPORTED, "%s: %s = %lld is too large", name, what, (long long)given);
+    if (rows <= 1) *out = (*out + 15) / 16 * 16;
     return VK_OK;
+}
+
+// Addresses that an element of the type cannot have.
+int element_aligned(const char* name, const char* what, const void* p, size_t esize)
+{
+    if (aligned(p, esize)) return VK_OK;
+    return set_error(VK_ERR_ALIGNMENT, "%s: %s is not aligned to its elements of %zu bytes", name, what, esize);
 }
 
 bool rows_at(const void* p, long long ld, size_t esize, size_t to)
@@ -232,14 +241,15 @@ extern "C" int vk_quantize_fp8(const vk_quantize_fp8_args* a)
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: unknown scaling %d", name, a->scaling);
     QuantParams p;
     const int64_t blocks = (a->cols + 127) / 128;
-    int rc = ld_of(name, "ldx", a->ldx, a->cols, &p.ldx);
-    if (rc == VK_OK) rc = ld_of(name, "ldq", a->ldq, a->cols, &p.ldq);
-    if (rc == VK_OK) rc = ld_of(name, "ld_scale", a->ld_scale, blocks, &p.lds);
+    int rc = ld_of(name, "ldx", a->ldx, a->cols, a->rows, &p.ldx);
+    if (rc == VK_OK) rc = ld_of(name, "ldq", a->ldq, a->cols, a->rows, &p.ldq);
+    if (rc == VK_OK) rc = ld_of(name, "ld_scale", a->ld_scale, blocks, 2, &p.lds);
     if (rc != VK_OK) return rc;
     if (a->rows == 0 || a->cols == 0) return VK_OK;
     if (a->X == nullptr || a->Q == nullptr || a->scale == nullptr)
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: X, Q or scale is NULL", name);
-    rc = use_device();
+    rc = element_aligned(name, "X", a->X, bytes_of(a->dtype));
+    if (rc == VK_OK) rc = use_device();
     if (rc != VK_OK) return rc;
     p.x = a->X;
     p.q = static_cast<uint8_t*>(a->Q);
@@ -305,18 +315,23 @@ extern "C" int vk_rmsnorm_fp8(const vk_rmsnorm_fp8_args* a)
     if (!(a->eps >= 0.f)) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", name);
     NormParams p;
     const int64_t blocks = (a->cols + 127) / 128;
-    int rc = ld_of(name, "ldx", a->ldx, a->cols, &p.ldx);
-    if (rc == VK_OK) rc = ld_of(name, "ld_residual", a->ld_residual, a->cols, &p.ldr);
-    if (rc == VK_OK) rc = ld_of(name, "ldq", a->ldq, a->cols, &p.ldq);
-    if (rc == VK_OK) rc = ld_of(name, "ld_scale", a->ld_scale, blocks, &p.lds);
-    if (rc == VK_OK) rc = ld_of(name, "ldh", a->ldh, a->cols, &p.ldh);
+    int rc = ld_of(name, "ldx", a->ldx, a->cols, a->rows, &p.ldx);
+    if (rc == VK_OK) rc = ld_of(name, "ld_residual", a->ld_residual, a->cols, a->rows, &p.ldr);
+    if (rc == VK_OK) rc = ld_of(name, "ldq", a->ldq, a->cols, a->rows, &p.ldq);
+    if (rc == VK_OK) rc = ld_of(name, "ld_scale", a->ld_scale, blocks, 2, &p.lds);
+    if (rc == VK_OK) rc = ld_of(name, "ldh", a->ldh, a->cols, a->rows, &p.ldh);
     if (rc != VK_OK) return rc;
     if (a->rows == 0) return VK_OK;
     if (a->X == nullptr || a->weight == nullptr || a->Q == nullptr || a->scale == nullptr || a->rstd == nullptr)
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: X, weight, Q, scale or rstd is NULL", name);
     if ((a->residual == nullptr) != (a->H == nullptr))
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: H is given with a residual and only then", name);
-    rc = use_device();
+    rc = element_aligned(name, "X", a->X, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "residual", a->residual, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "weight", a->weight, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "H", a->H, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "rstd", a->rstd, 4);
+    if (rc == VK_OK) rc = use_device();
     if (rc != VK_OK) return rc;
     p.x = a->X;
     p.residual = a->residual;
@@ -396,10 +411,10 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
     if (a->cols < 1 || a->cols > kMaxDim) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: cols = %lld is out of range", name, (long long)a->cols);
     if (a->dtype != VK_DTYPE_F16 && a->dtype != VK_DTYPE_BF16)
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: dtype must be VK_DTYPE_F16 or VK_DTYPE_BF16", name);
-    int rc = ld_of(name, "lddy", a->lddy, a->cols, &p.lddy);
-    if (rc == VK_OK) rc = ld_of(name, "ldh", a->ldh, a->cols, &p.ldh);
-    if (rc == VK_OK) rc = ld_of(name, "ld_dres", a->ld_dres, a->cols, &p.lddres);
-    if (rc == VK_OK) rc = ld_of(name, "lddx", a->lddx, a->cols, &p.lddx);
+    int rc = ld_of(name, "lddy", a->lddy, a->cols, a->rows, &p.lddy);
+    if (rc == VK_OK) rc = ld_of(name, "ldh", a->ldh, a->cols, a->rows, &p.ldh);
+    if (rc == VK_OK) rc = ld_of(name, "ld_dres", a->ld_dres, a->cols, a->rows, &p.lddres);
+    if (rc == VK_OK) rc = ld_of(name, "lddx", a->lddx, a->cols, a->rows, &p.lddx);
     if (rc == VK_OK) rc = vk_rmsnorm_fp8_workspace(a->rows, a->cols, &need);
     if (rc != VK_OK) return rc;
     if (a->dweight == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: dweight is NULL", name);
@@ -407,7 +422,14 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: dY, H, weight, rstd or dX is NULL", name);
     if (a->rows > 0 && (a->workspace == nullptr || a->workspace_bytes < need || !aligned(a->workspace, 16)))
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %zu bytes, 16-byte aligned (vk_rmsnorm_fp8_workspace)", name, need);
-    rc = use_device();
+    rc = element_aligned(name, "dweight", a->dweight, 4);
+    if (rc == VK_OK) rc = element_aligned(name, "dY", a->dY, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "H", a->H, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "weight", a->weight, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "rstd", a->rstd, 4);
+    if (rc == VK_OK) rc = element_aligned(name, "dres", a->dres, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "dX", a->dX, 2);
+    if (rc == VK_OK) rc = use_device();
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     const NormBackPlan plan = norm_backward_plan(a->rows, a->cols);
@@ -511,17 +533,18 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     const int64_t kb = (a->k + 127) / 128;
     const int64_t b_row = a->trans_b ? a->k : a->n;
     long long lda, ldb, ldc, ldas, ldbs;
-    int rc = ld_of(name, "lda", a->lda, a->k, &lda);
-    if (rc == VK_OK) rc = ld_of(name, "ldb", a->ldb, b_row, &ldb);
-    if (rc == VK_OK) rc = ld_of(name, "ldc", a->ldc, a->n, &ldc);
-    if (rc == VK_OK) rc = ld_of(name, "ld_a_scale", a->ld_a_scale, kb, &ldas);
-    if (rc == VK_OK) rc = ld_of(name, "ld_b_scale", a->ld_b_scale, (b_row + 127) / 128, &ldbs);
+    int rc = ld_of(name, "lda", a->lda, a->k, a->m, &lda);
+    if (rc == VK_OK) rc = ld_of(name, "ldb", a->ldb, b_row, a->trans_b ? a->n : a->k, &ldb);
+    if (rc == VK_OK) rc = ld_of(name, "ldc", a->ldc, a->n, a->m, &ldc);
+    if (rc == VK_OK) rc = ld_of(name, "ld_a_scale", a->ld_a_scale, kb, 2, &ldas);
+    if (rc == VK_OK) rc = ld_of(name, "ld_b_scale", a->ld_b_scale, (b_row + 127) / 128, 2, &ldbs);
     if (rc != VK_OK) return rc;
     if (a->m == 0 || a->n == 0) return VK_OK;
     if (a->C == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: C is NULL", name);
     if (a->k > 0 && (a->A == nullptr || a->B == nullptr || a->a_scale == nullptr || a->b_scale == nullptr))
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: A, B, a_scale or b_scale is NULL", name);
-    rc = use_device();
+    rc = element_aligned(name, "C", a->C, bytes_of(a->dtype));
+    if (rc == VK_OK) rc = use_device();
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     if (a->k > 0 && tma_ok(a->A, lda, 1) && tma_ok(a->B, ldb, 1)) {
@@ -614,16 +637,18 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: unknown out_dtype %d", name, a->out_dtype);
     if (a->accumulate != 0 && a->accumulate != 1) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: accumulate must be 0 or 1", name);
     long long lddy, ldx, ldxs, lddw;
-    int rc = ld_of(name, "lddy", a->lddy, a->n, &lddy);
-    if (rc == VK_OK) rc = ld_of(name, "ldx", a->ldx, a->k, &ldx);
-    if (rc == VK_OK) rc = ld_of(name, "ld_x_scale", a->ld_x_scale, (a->k + 127) / 128, &ldxs);
-    if (rc == VK_OK) rc = ld_of(name, "lddw", a->lddw, a->k, &lddw);
+    int rc = ld_of(name, "lddy", a->lddy, a->n, a->tokens, &lddy);
+    if (rc == VK_OK) rc = ld_of(name, "ldx", a->ldx, a->k, a->tokens, &ldx);
+    if (rc == VK_OK) rc = ld_of(name, "ld_x_scale", a->ld_x_scale, (a->k + 127) / 128, 2, &ldxs);
+    if (rc == VK_OK) rc = ld_of(name, "lddw", a->lddw, a->k, a->n, &lddw);
     if (rc != VK_OK) return rc;
     if (a->n == 0 || a->k == 0) return VK_OK;
     if (a->dW == nullptr) return set_error(VK_ERR_INVALID_ARGUMENT, "%s: dW is NULL", name);
     if (a->tokens > 0 && (a->dY == nullptr || a->X == nullptr || a->x_scale == nullptr))
         return set_error(VK_ERR_INVALID_ARGUMENT, "%s: dY, X or x_scale is NULL", name);
-    rc = use_device();
+    rc = element_aligned(name, "dY", a->dY, 2);
+    if (rc == VK_OK) rc = element_aligned(name, "dW", a->dW, bytes_of(a->out_dtype));
+    if (rc == VK_OK) rc = use_device();
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     if (a->tokens > 0 && tma_ok(a->dY, lddy, 2) && tma_ok(a->X, ldx, 1)) {

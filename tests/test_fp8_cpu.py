@@ -13,7 +13,7 @@ import vibekernel_b200 as vk
 from oracle import fp8
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-BAD, UNSUPPORTED = vk.VK_ERR_INVALID_ARGUMENT, vk.VK_ERR_UNSUPPORTED
+BAD, UNSUPPORTED, ALIGNMENT = vk.VK_ERR_INVALID_ARGUMENT, vk.VK_ERR_UNSUPPORTED, vk.VK_ERR_ALIGNMENT
 P = 0x1000
 
 
@@ -67,6 +67,12 @@ def test_null_arguments(name):
     ("wgrad_fp8", dict(tokens=-1), BAD), ("wgrad_fp8", dict(dtype=1), BAD), ("wgrad_fp8", dict(out_dtype=4), BAD),
     ("wgrad_fp8", dict(accumulate=2), BAD), ("wgrad_fp8", dict(lddy=7), BAD), ("wgrad_fp8", dict(dW=None), BAD),
     ("wgrad_fp8", dict(X=None), BAD), ("wgrad_fp8", dict(k=300, ld_x_scale=2), BAD),
+    ("quantize_fp8", dict(X=P + 1), ALIGNMENT), ("quantize_fp8", dict(X=P + 2, dtype=1), ALIGNMENT),
+    ("rmsnorm_fp8", dict(X=P + 1), ALIGNMENT), ("rmsnorm_fp8", dict(weight=P + 1), ALIGNMENT), ("rmsnorm_fp8", dict(rstd=P + 2), ALIGNMENT),
+    ("rmsnorm_fp8", dict(residual=P, H=P + 1), ALIGNMENT), ("rmsnorm_fp8_backward", dict(dX=P + 1), ALIGNMENT),
+    ("rmsnorm_fp8_backward", dict(dweight=P + 2), ALIGNMENT), ("rmsnorm_fp8_backward", dict(dres=P + 1), ALIGNMENT),
+    ("gemm_fp8", dict(C=P + 1), ALIGNMENT), ("gemm_fp8", dict(C=P + 2, dtype=1), ALIGNMENT), ("wgrad_fp8", dict(dY=P + 1), ALIGNMENT),
+    ("wgrad_fp8", dict(dW=P + 2, out_dtype=1), ALIGNMENT),
 ])
 def test_bad_arguments(name, fields, code):
     assert _call(name, **{**_good(name), **fields}) == code

@@ -569,3 +569,157 @@ def test_calls_on_a_given_stream(vk):
     st.synchronize()
     for got, name in ((q, "q"), (y, "y"), (dn, "dn"), (dw, "dw"), (dx, "dx"), (dwn, "dwn")):
         assert torch.equal(got.view(torch.uint8), want[name].view(torch.uint8)), name
+
+
+# ------------------------------------------------------------------------------------------ far and odd places
+def test_single_rows_of_any_width(vk):
+    """A single row's stride means nothing: whatever the width, it runs where wider matrices run."""
+    for k, n in ((1, 1), (333, 129), (3001, 515)):
+        x, w = _rand((1, k), BF16, 130), _rand((k,), BF16, 131)
+        q, s, h, rstd = vk.rmsnorm_fp8(x, w, residual=x)
+        _check_norm(x, w, x, 1e-6, q, s, h, rstd)
+        b, sb = _quantized((n, k), 132, True)
+        av, bv = _deq(q, s), _deq(b, sb, True).t()
+        _check_product(vk.gemm_fp8(q, s, b, sb, trans_b=True, out_dtype=F32), av @ bv, av.abs() @ bv.abs(), k)
+        dy = _rand((1, n), BF16, 133)
+        d = dy.double().t()
+        _check_product(vk.wgrad_fp8(dy, q, s, out_dtype=F32), d @ av, d.abs() @ av.abs(), 1)
+        dx, dw = vk.rmsnorm_fp8_backward(x, h, w, rstd)
+        _check_norm_back(x, h, w, rstd, None, dx, dw)
+
+
+ROWS, COLS = 66000, 33000  # 2.18e9 elements: beyond 31 bits
+
+
+@pytest.fixture(scope="module")
+def far(vk):
+    """A matrix of zeros whose last rows are not."""
+    x = torch.zeros((ROWS, COLS), dtype=BF16, device="cuda")
+    x[-3:] = _rand((3, COLS), BF16, 140)
+    yield x
+    del x
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("tile", [False, True])
+def test_far_rows_quantized(vk, far, tile):
+    q, s = vk.quantize_fp8(far, tile=tile)
+    first = ROWS // 128 * 128 if tile else ROWS - 5
+    codes, scale = fp8.quantize(far[first:].double().cpu().numpy(), tile)
+    np.testing.assert_array_equal(_bytes(q[first:]), codes)
+    np.testing.assert_array_equal(_bytes(s[-scale.shape[0]:]), scale)
+    assert (q[:1000].view(torch.uint8) == 0).all()
+
+
+def test_far_rows_normalised_and_back(vk, far):
+    w = _rand((COLS,), BF16, 141)
+    q, s, h, rstd = vk.rmsnorm_fp8(far, w, residual=far)
+    _check_norm(far[-4:], w, far[-4:], 1e-6, q[-4:], s[-4:], h[-4:], rstd[-4:])
+    del q, s
+    dx, dw = vk.rmsnorm_fp8_backward(far, h, w, rstd)
+    _check_norm_back(far[-4:], h[-4:], w, rstd[-4:], None, dx[-4:], dw)
+
+
+def test_far_rows_multiplied(vk, far):
+    """The 8-bit operands' and the result's last rows lie beyond 31 bits."""
+    q, s = vk.quantize_fp8(far)
+    b, sb = _quantized((16, COLS), 142, True)
+    bv = _deq(b, sb, True).t()
+    av = _deq(q[-4:], s[-4:])
+    c = vk.gemm_fp8(q, s, b, sb, trans_b=True, out_dtype=F32)  # q is A
+    _check_product(c[-4:], av @ bv, av.abs() @ bv.abs(), COLS)
+    c = vk.gemm_fp8(b, sb, q, s, trans_b=True, out_dtype=F32)  # q is B
+    _check_product(c[:, -4:], bv.t() @ av.t(), bv.t().abs() @ av.t().abs(), COLS)
+    dy = torch.zeros((ROWS, 8), dtype=BF16, device="cuda")
+    dy[-4:] = _rand((4, 8), BF16, 143)
+    d = dy[-4:].double().t()
+    _check_product(vk.wgrad_fp8(dy, q, s, out_dtype=F32), d @ av, d.abs() @ av.abs(), 4)
+    del q
+    a, sa = _quantized((ROWS, 128), 144)
+    b, sb = _quantized((128, COLS), 145, True)
+    out = torch.empty((ROWS, COLS), dtype=BF16, device="cuda")
+    vk.gemm_fp8(a, sa, b, sb, out)
+    av, bv = _deq(a[-3:], sa[-3:]), _deq(b, sb, True)
+    _check_product(out[-3:], av @ bv, av.abs() @ bv.abs(), 128)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("byte", [127 - 40, 127 - 14, 127, 127 + 7, 127 + 20])
+def test_wgrad_scale_range(vk, dtype, byte):
+    """One token, dY = 1: dW is X's values in dY's type, for scales far beyond the usual ones."""
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    codes = codes[(codes & 127) != 127]
+    x = torch.zeros((1, 256), dtype=torch.uint8, device="cuda")
+    x[0, :254] = codes
+    s = torch.full((1, 2), byte, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    x = x.view(torch.float8_e4m3fn)
+    dw = vk.wgrad_fp8(torch.ones((1, 8), dtype=dtype, device="cuda"), x, s, out_dtype=F32)
+    want = _deq(x, s).float()
+    want = (want.clamp(-65504, 65504) if dtype is F16 else want).to(dtype).double()
+    assert torch.equal(dw[3].double(), want[0])
+
+
+def test_wgrad_nan_stays_in_its_columns(vk):
+    dy = _rand((300, 264), BF16, 146)
+    x, s = _quantized((300, 400), 147)
+    clean = vk.wgrad_fp8(dy, x, s, out_dtype=F32)
+    s.view(torch.uint8)[17, 1] = 255       # columns 128 .. 255
+    x.view(torch.uint8)[40, 399] = 0x7f    # a NaN value under a finite scale
+    dw = vk.wgrad_fp8(dy, x, s, out_dtype=F32)
+    bad = torch.zeros(400, dtype=torch.bool, device="cuda")
+    bad[128:256] = True
+    bad[399] = True
+    assert dw[:, bad].isnan().all() and torch.equal(dw[:, ~bad], clean[:, ~bad])
+
+
+def test_calls_at_the_same_time_on_two_streams(vk):
+    """Eager calls that overlap on the GPU share nothing."""
+    data = [_layer_inputs(150 + 10 * i, 600, 1032, 776) for i in range(2)]
+    want = [_layer(vk, *d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(_layer(vk, *data[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            for name, v in o.items():
+                assert torch.equal(v.view(torch.uint8), want[i][name].view(torch.uint8)), name
+
+
+def test_first_calls_of_a_process_captured(vk):
+    """Nothing has to run before a capture: the first calls of a process are recorded and replayed."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch, vibekernel_b200 as vk
+x = torch.randn(300, 640, device="cuda").bfloat16()
+w = torch.ones(640, device="cuda").bfloat16()
+wt = torch.randn(512, 640, device="cuda").bfloat16()
+dy = torch.randn(300, 512, device="cuda").bfloat16()
+torch.cuda.synchronize()
+def layer():
+    q, s, h, rstd = vk.rmsnorm_fp8(x, w, residual=x)
+    wq, ws = vk.quantize_fp8(wt, tile=True)
+    y = vk.gemm_fp8(q, s, wq, ws, trans_b=True)
+    y1 = vk.gemm_fp8(q[:5], s[:5], wq, ws, trans_b=True)
+    dyq, dys = vk.quantize_fp8(dy)
+    dn = vk.gemm_fp8(dyq, dys, wq, ws, out_dtype=torch.bfloat16)
+    return [y, y1, vk.wgrad_fp8(dy, q, s), *vk.rmsnorm_fp8_backward(dn, h, w, rstd)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = layer()
+g.replay()
+torch.cuda.synchronize()
+for a, b in zip(out, layer()):
+    assert torch.equal(a, b)
+assert vk.device_error(0) == 0
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
