@@ -491,7 +491,7 @@ template <int NPAD, int OUT>
 static int launch_thin(ThinParams p, const CUtensorMap& tb, const CUtensorMap& ta, cudaStream_t stream)
 {
     using Cfg = ThinCfg<NPAD>;
-    constexpr int kId = 16 + 3 * (NPAD == 16 ? 0 : NPAD == 32 ? 1 : 2) + OUT;
+    constexpr int kId = 16 + 3 * (NPAD == 16 ? 0 : NPAD == 32 ? 1 : NPAD == 64 ? 2 : 3) + OUT;
     int fit[4];
     const int rc = prepare_kernel(gemm_fp8_thin_kernel<NPAD, OUT>, kId, Cfg::kSmemBytes, kThinThreads, fit);
     if (rc != VK_OK) return rc;
@@ -548,7 +548,7 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     if (a->k > 0 && tma_ok(a->A, lda, 1) && tma_ok(a->B, ldb, 1)) {
-        if (a->trans_b && a->m <= 64) {
+        if (a->trans_b && a->m <= 128) {
             ThinParams p;
             p.M = static_cast<int>(a->m);
             p.N = static_cast<int>(a->n);
@@ -558,7 +558,7 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
             p.C = a->C;
             p.ldc = ldc;
             p.timeout_ns = wait_timeout_ns();
-            const int npad = a->m <= 16 ? 16 : a->m <= 32 ? 32 : 64;
+            const int npad = a->m <= 16 ? 16 : a->m <= 32 ? 32 : a->m <= 64 ? 64 : 128;
             CUtensorMap tb, ta;
             rc = make_map(&tb, a->B, a->n, a->k, ldb, 1, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
             if (rc == VK_OK) rc = make_map(&ta, a->A, a->m, a->k, lda, 1, 128, npad, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -567,7 +567,8 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
                 constexpr int kOut = decltype(out)::value;
                 return npad == 16   ? launch_thin<16, kOut>(p, tb, ta, stream)
                        : npad == 32 ? launch_thin<32, kOut>(p, tb, ta, stream)
-                                    : launch_thin<64, kOut>(p, tb, ta, stream);
+                       : npad == 64 ? launch_thin<64, kOut>(p, tb, ta, stream)
+                                    : launch_thin<128, kOut>(p, tb, ta, stream);
             };
             return a->dtype == VK_DTYPE_F16   ? launch(std::integral_constant<int, VK_DTYPE_F16>())
                    : a->dtype == VK_DTYPE_F32 ? launch(std::integral_constant<int, VK_DTYPE_F32>())

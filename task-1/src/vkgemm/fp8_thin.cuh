@@ -1,6 +1,6 @@
-// C = A * B^T of 8-bit operands with at most 64 rows of A (single tokens of a few sequences): bound by B's bytes.
+// C = A * B^T of 8-bit operands with at most 128 rows of A (single tokens of a few sequences): bound by B's bytes.
 //
-// The roles of the operands are swapped: 128 rows of B are the MMA's M, the few rows of A its N (16, 32 or 64), so that no
+// The roles of the operands are swapped: 128 rows of B are the MMA's M, the few rows of A its N (16 to 128), so that no
 // tensor work is spent on rows that do not exist and B streams through the whole GPU.  A tile of 128 rows of B is shared
 // by a cluster of up to 8 CTAs, each with its part of k; they add their sums through shared memory, in the order of k.  A CTA
 // has as many loads in flight as its shared memory holds (200 KB), which for common sizes is all it will ever load.
@@ -30,6 +30,8 @@ template <int NPAD>
 struct ThinCfg {
     static constexpr int kStageBytes = 128 * 128 + NPAD * 128;
     static constexpr int kStages = 204800 / kStageBytes;
+    static constexpr int kSfCol = NPAD < 64 ? 64 : NPAD;  // tensor memory: sums, then two sets of scales
+    static constexpr int kTmemCols = 2 * kSfCol;
     static constexpr int kBars = 2 * kStages + 2 * kThinSfSlots + 1;
     static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kThinSfSlots * kThinSfBytes + kBars * 8 + 16;
     static_assert(kSmemBytes <= 232448, "shared memory per CTA");
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc<1>(smem_u32(tmem_slot), 128);
+        tmem_alloc<1>(smem_u32(tmem_slot), Cfg::kTmemCols);
         tmem_relinquish<1>();
     }
     tc_fence_before();
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
             if (in == 0 && !mbar_wait_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) break;
             if (!mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) break;
             tc_fence_after();
-            const uint32_t sfa = base + 64 + set * 16, sfb = sfa + 8;
+            const uint32_t sfa = base + Cfg::kSfCol + set * 16, sfb = sfa + 8;
             const bool last = in == 3 || kb + 1 == kb1;
             if (one) {
                 if (in == 0) {
@@ -155,15 +157,15 @@ __global__ void __launch_bounds__(kThinThreads, 1)
     } else if (warp == 6) {
         Ring sf(kThinSfSlots);
         for (int kb = kb0; kb < kb1; kb += 4, sf.next()) {
-            uint32_t b[4], a[2];
+            uint32_t b[4], a[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) b[i] = p.sb.word(n0 + lane + 32 * i, kb, num_kb);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) a[i] = 32 * i < NPAD ? p.sa.word(lane + 32 * i, kb, num_kb) : 0x7f7f7f7fu;
+            for (int i = 0; i < 4; ++i) a[i] = 32 * i < NPAD ? p.sa.word(lane + 32 * i, kb, num_kb) : 0x7f7f7f7fu;
             if (!mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at)) break;
             uint4* dst = reinterpret_cast<uint4*>(sSf + sf.at * kThinSfBytes) + lane;
             dst[0] = make_uint4(b[0], b[1], b[2], b[3]);
-            dst[32] = make_uint4(a[0], a[1], 0x7f7f7f7fu, 0x7f7f7f7fu);
+            dst[32] = make_uint4(a[0], a[1], a[2], a[3]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(sf_full_bar(sf.at));
@@ -200,35 +202,36 @@ __global__ void __launch_bounds__(kThinThreads, 1)
     if (p.slices > 1) {
         __syncthreads();
         cluster_sync_all();
-        if (epilogue && n0 + t < p.N && ok) {
-            // four rows of A at a time, all slices' sums on their way together
-            for (int g = slice; g * 4 < p.M; g += p.slices) {
-                const uint32_t at = smem_u32(sums + g * 128 + t);
-                float4 v[8];
+        // by all warps: four rows of A and 32 of B at a time, all slices' sums on their way together
+        for (int i = warp; ; i += kThinThreads / 32) {
+            const int g = slice + (i >> 2) * p.slices, n = (i & 3) * 32 + lane;
+            if (g * 4 >= p.M) break;
+            const uint32_t at = smem_u32(sums + g * 128 + n);
+            float4 v[8];
 #pragma unroll
-                for (int s = 0; s < 8; ++s)
-                    if (s < p.slices) v[s] = ld_cluster_f4(mapa_shared(at, static_cast<uint32_t>(s)));
-                float4 f = v[0];
+            for (int s = 0; s < 8; ++s)
+                if (s < p.slices) v[s] = ld_cluster_f4(mapa_shared(at, static_cast<uint32_t>(s)));
+            float4 f = v[0];
 #pragma unroll
-                for (int s = 1; s < 8; ++s) {
-                    if (s >= p.slices) break;
-                    f.x += v[s].x;
-                    f.y += v[s].y;
-                    f.z += v[s].z;
-                    f.w += v[s].w;
-                }
-                const float row[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (g * 4 + i < p.M) c[(g * 4 + i) * p.ldc] = from_f32<T>(row[i]);
+            for (int s = 1; s < 8; ++s) {
+                if (s >= p.slices) break;
+                f.x += v[s].x;
+                f.y += v[s].y;
+                f.z += v[s].z;
+                f.w += v[s].w;
             }
+            const float row[4] = {f.x, f.y, f.z, f.w};
+            T* to = static_cast<T*>(p.C) + n0 + n;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (g * 4 + j < p.M && n0 + n < p.N) to[(g * 4 + j) * p.ldc] = from_f32<T>(row[j]);
         }
         cluster_sync_all();
     }
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc<1>(tmem, 128);
+        tmem_dealloc<1>(tmem, Cfg::kTmemCols);
     }
 #endif
 }

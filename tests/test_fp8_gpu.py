@@ -190,7 +190,7 @@ def test_norm_strides_and_surroundings(vk, cols, lead, tail):
         _untouched(room, sh, lead)
 
 
-@pytest.mark.parametrize("cols", [1000, 4096, 9000])
+@pytest.mark.parametrize("cols", [1000, 1001, 4096, 8191, 9001])
 def test_norm_in_place(vk, cols):
     x, r, w = _rand((7, cols), F16, 9), _rand((7, cols), F16, 10), _rand((cols,), F16, 11)
     want = vk.rmsnorm_fp8(x, w, residual=r)
@@ -335,7 +335,7 @@ def test_gemm_waves(vk, shape, layout):
 
 
 # few rows of A: clusters of every size, more tiles than SMs, more k than fits in flight
-@pytest.mark.parametrize("shape", [(1, 500, 4096), (16, 1500, 1600), (17, 2000, 5000), (40, 3000, 1000), (5, 4096, 4096), (64, 20000, 300),
+@pytest.mark.parametrize("shape", [(1, 500, 4096), (16, 1500, 1600), (17, 2000, 5000), (40, 3000, 1000), (5, 4096, 4096), (64, 20000, 300), (100, 1000, 3000), (128, 700, 4096),
                                    (2, 300, 20000)])
 @pytest.mark.parametrize("layout", ["nt_tile", "nt_row"])
 def test_gemm_few_rows(vk, shape, layout):
