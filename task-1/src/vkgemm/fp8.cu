@@ -582,6 +582,7 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
         p.K = static_cast<int>(a->k);
         p.work.tiles_m = static_cast<int>((a->m + 255) / 256);
         p.work.tiles_n = static_cast<int>((a->n + 255) / 256);
+        p.work.n = p.N;
         p.work.stages = static_cast<int>((a->k + 255) / 256);
         p.work.grain = 2;  // a slice begins with a whole set of scales
         p.sa = scales(a->a_scale, ldas, a->m, a->a_scaling, true);
@@ -661,6 +662,7 @@ extern "C" int vk_wgrad_fp8(const vk_wgrad_fp8_args* a)
         p.K = static_cast<int>(a->tokens);
         p.work.tiles_m = static_cast<int>((a->n + 255) / 256);
         p.work.tiles_n = static_cast<int>((a->k + 255) / 256);
+        p.work.n = p.N;
         p.work.stages = static_cast<int>((a->tokens + kWgBK - 1) / kWgBK);
         p.work.grain = 1;
         p.X = static_cast<const uint8_t*>(a->X);

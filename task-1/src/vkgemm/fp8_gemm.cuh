@@ -56,6 +56,7 @@ struct ScaleSource {
 // How the 256 x 256 tiles of an output are shared out over clusters.
 struct TileWork {
     int tiles_m, tiles_n, raster_group;
+    int n;       // columns of the output
     int stages;  // k-stages of a tile
     int grain;   // stages that a share of k begins at multiples of
     int pairs;   // pairs of CTAs that share each tile through their cluster's shared memory (1: none)
@@ -89,7 +90,7 @@ __device__ __forceinline__ Work work_unit(const TileWork& w, int u, int part)
     const int in = t - g * per_group;
     r.tm = first_m + in % rows;
     r.n0 = in / rows * 256 + (u < whole ? 0 : (u - whole) % 2 * 128);
-    r.cols = u < whole ? 256 : 128;
+    r.cols = u < whole && w.n - r.n0 > 128 ? 256 : 128;  // a ragged last column needs no more
     return r;
 }
 
@@ -118,6 +119,7 @@ constexpr int kF8Threads = 224;
 constexpr int kF8Acc1 = 224;  // first column of the second accumulator
 constexpr int kF8SfCol = 480;
 static_assert(kF8SmemBytes <= 232448, "shared memory per CTA");
+static_assert(kF8Stages * kF8StageBytes >= 128 * 256 * 4 + 16 * kF8EpiWarpBytes, "a shared tile's sums and staging fit the stages");
 
 // D (+)= (A * scale_a) * (B * scale_b), e4m3, K = 32.
 __device__ __forceinline__ void umma_mxf8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
@@ -320,34 +322,39 @@ __device__ __forceinline__ void finish_unit(const Work& u, const BoxOut& out, ui
     }
 }
 
-// The columns of a shared tile that fall to pair `part`, added from all pairs' shared memory.
+// The columns of a shared tile that fall to pair `part`, added from all pairs' shared memory: boxes of 32 x 32, by every
+// warp of the CTA.  stg: staging of the first 16 warps, behind the sums.
 template <int OUT>
 __device__ __forceinline__ void finish_shared(const TileWork& w, const Work& u, const BoxOut& out, uint8_t* stg, const float4* sums,
-                                              int part, int half, int q, int lane, uint32_t& turn)
+                                              int part, int half, int warp, int warps, int lane)
 {
-    const int row0 = u.tm * 256 + half * 128 + q * 32;
+    if (warp >= 16) return;
+    const int first = 8 * part / w.pairs, chunks = 8 * (part + 1) / w.pairs - first;
+    stg += warp * kF8EpiWarpBytes;
+    uint32_t turn = 0;
 #pragma unroll 1
-    for (int ch = 8 * part / w.pairs; ch < 8 * (part + 1) / w.pairs; ++ch) {
-        const int col = u.n0 + ch * 32;
+    for (int i = warp; i < 4 * chunks; i += min(warps, 16)) {
+        const int ch = first + (i >> 2), q = i & 3, col = u.n0 + ch * 32;
         if (col >= out.N) break;
         const uint32_t at = smem_u32(sums + ch * 8 * 128 + q * 32 + lane);
         float f[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = 0.f;
+        for (int j = 0; j < 32; ++j) f[j] = 0.f;
 #pragma unroll 1
         for (int s = 0; s < w.pairs; ++s) {
             const uint32_t from = mapa_shared(at, static_cast<uint32_t>(2 * s + half));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 v = ld_cluster_f4(from + static_cast<uint32_t>(i * 128 * 16));
-                f[4 * i] += v.x;
-                f[4 * i + 1] += v.y;
-                f[4 * i + 2] += v.z;
-                f[4 * i + 3] += v.w;
+            for (int j = 0; j < 8; ++j) {
+                const float4 v = ld_cluster_f4(from + static_cast<uint32_t>(j * 128 * 16));
+                f[4 * j] += v.x;
+                f[4 * j + 1] += v.y;
+                f[4 * j + 2] += v.z;
+                f[4 * j + 3] += v.w;
             }
         }
-        store_box<OUT>(out, stg, row0, lane, col, f, turn);
+        store_box<OUT>(out, stg, u.tm * 256 + half * 128 + q * 32, lane, col, f, turn);
     }
+    if (out.c_tma && lane == 0) bulk_wait_group_all();
 }
 
 // A place in a ring of stages and the parity of its barriers.
@@ -581,7 +588,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     if (p.work.pairs > 1) {
         __syncthreads();
         cluster_sync_all();
-        if (epilogue) finish_shared<OUT>(p.work, work_unit(p.work, cluster_id, part), out, stg, sums, part, half, q, lane, turn);
+        finish_shared<OUT>(p.work, work_unit(p.work, cluster_id, part), out, sA + 128 * 256 * 4, sums, part, half, warp, kF8Threads / 32, lane);
     }
     if (epilogue && p.c_tma && lane == 0) bulk_wait_group_all();
 

@@ -42,9 +42,9 @@ constexpr int kWgBars = 2 * kWgStages + 4;
 constexpr int kWgSmemBytes = 1024 + kWgStages * (kWgABytes + kWgBBytes) + 4 * kF8EpiWarpBytes + kWgBars * 8 + 16;
 constexpr int kWgThreads = 192 + 128 * kWgStages;
 static_assert(kWgSmemBytes <= 232448, "shared memory per CTA");
-static_assert(kWgStages * (kWgABytes + kWgBBytes) >= 128 * 256 * 4, "a shared tile's sums fit the stages");
+static_assert(kWgStages * (kWgABytes + kWgBBytes) >= 128 * 256 * 4 + 16 * kF8EpiWarpBytes, "a shared tile's sums and staging fit the stages");
 
-// The first n (below 16; none if negative) bytes at src, and zeros.
+// The first n (below 16) bytes at src, and zeros.
 __device__ __noinline__ uint4 first_bytes(const uint8_t* src, int n)
 {
     uint64_t lo = 0, hi = 0;
@@ -225,10 +225,12 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             for (int i = 0; i < 8; ++i) {
                 const int row = (whole ? 4 : 8) * i;
                 v[i] = make_uint4(0, 0, 0, 0);
-                if ((whole || i < 4) && t0 + g + row < p.K) {
+                if (n > 0 && (whole || i < 4) && t0 + g + row < p.K) {
                     // a row's last chunk reads into the row's padding, which every row but the last is sure to have
-                    v[i] = n >= 16 || (n > 0 && t0 + g + row + 1 < p.K) ? *reinterpret_cast<const uint4*>(src + row * p.ldx)
-                                                                        : first_bytes(src + row * p.ldx, n);
+                    if (n >= 16 || t0 + g + row + 1 < p.K)
+                        v[i] = *reinterpret_cast<const uint4*>(src + row * p.ldx);
+                    else
+                        v[i] = first_bytes(src + row * p.ldx, n);
                 }
             }
             const int blk = w.n0 / 128 + (whole ? half : 0);
@@ -293,7 +295,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     if (p.work.pairs > 1) {
         __syncthreads();
         cluster_sync_all();
-        if (epilogue) finish_shared<OUT>(p.work, work_unit(p.work, cluster_id, part), out, stg, sums, part, half, q, lane, turn);
+        finish_shared<OUT>(p.work, work_unit(p.work, cluster_id, part), out, sA + 128 * 256 * 4, sums, part, half, warp, kWgThreads / 32, lane);
     }
     if (epilogue && p.c_tma && lane == 0) bulk_wait_group_all();
 
