@@ -286,21 +286,26 @@ extern "C" int vk_quantize_fp8(const vk_quantize_fp8_args* a)
 // ------------------------------------------------------------------------------------------
 // RMS norm
 // ------------------------------------------------------------------------------------------
+// Vectors of 8 columns to a thread.  Two from 65 vectors on: half the warps to add up and to launch (8000 x 1000 bf16 with a
+// residual 8.8 us, with one 10.2; 8192 x 1600 14.9 and 16.6; at 200 columns, one 6.1 us and two 6.3).  Four only where two
+// would not do: 4001 x 5120 21.5 us for 20.9, unaligned rows of 3333 49 us for 36, for their registers.
 template <typename T, bool VEC>
 static int launch_norm(const NormParams& p, int64_t rows, cudaStream_t stream)
 {
     const unsigned grid = static_cast<unsigned>(rows);
     const int vectors = (p.cols + 127) / 128 * 16;  // of 8 columns, whole blocks
-    if (vectors > 1024) {
+    if (vectors > 2048) {
         rmsnorm_fp8_long_kernel<T, VEC><<<grid, 512, 0, stream>>>(p);
         return launched();
     }
-    const int nv = vectors > 256 ? 2 : 1;
+    const int nv = vectors > 1024 ? 4 : vectors > 64 ? 2 : 1;
     const int threads = ((vectors + nv - 1) / nv + 31) / 32 * 32;
     if (nv == 1)
         rmsnorm_fp8_kernel<T, 1, VEC><<<grid, threads, 0, stream>>>(p);
-    else
+    else if (nv == 2)
         rmsnorm_fp8_kernel<T, 2, VEC><<<grid, threads, 0, stream>>>(p);
+    else
+        rmsnorm_fp8_kernel<T, 4, VEC><<<grid, threads, 0, stream>>>(p);
     return launched();
 }
 

@@ -202,6 +202,34 @@ def test_norm_in_place(vk, cols):
             assert torch.equal(g.view(torch.uint8), e.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("cols,pitch", [(8320, 8320), (16376, 16380), (16384, 16384), (16385, 16385), (16392, 16400), (16392, 16397), (24576, 24576)])
+def test_norm_of_long_rows(vk, cols, pitch, dtype):
+    """Where a row stops fitting its threads' registers; `h` in x's place."""
+    w, r = _rand((cols,), dtype, 13), _rand((3, cols), dtype, 14)
+    x = _rand((3, pitch), dtype, 15)[:, :cols]
+    want = x.clone()
+    q, s, h, rstd = vk.rmsnorm_fp8(x, w, residual=r, h=x)
+    assert h is x
+    _check_norm(want, w, r, 1e-6, q, s, h, rstd)
+    _check_norm(want, w, None, 1e-6, *vk.rmsnorm_fp8(want, w))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_norm_adds_over_the_whole_range(vk, dtype):
+    """h is the fp32 sum rounded once (the sum of two 16-bit numbers is exact in fp32, or too lopsided for the rounding to
+    matter): subnormal numbers, signed zeros, cancellation, ties, sums that overflow."""
+    gen = _gen(16)
+    bits = torch.randint(0, 1 << 16, (2, 64, 1024), generator=gen, device="cuda", dtype=torch.int32).to(torch.int16).view(dtype)
+    x, r = torch.where(bits.float().isfinite(), bits, torch.zeros_like(bits))
+    r[32:] = -x[32:] * (1 + torch.randint(0, 3, (32, 1024), generator=gen, device="cuda") * torch.finfo(dtype).eps).to(dtype)
+    r[~r.float().isfinite()] = 0
+    x[0, :4] = torch.tensor([0.0, -0.0, 0.0, -0.0], dtype=dtype)
+    r[0, :4] = torch.tensor([0.0, -0.0, -0.0, 0.0], dtype=dtype)
+    h = vk.rmsnorm_fp8(x, torch.ones(1024, dtype=dtype, device="cuda"), residual=r)[2]
+    assert torch.equal(h.view(torch.int16), (x.float() + r.float()).to(dtype).view(torch.int16))
+
+
 def test_norm_rows_of_zeros_and_non_finite_rows(vk):
     x = _rand((4, 512), BF16, 12)
     x[1] = 0
