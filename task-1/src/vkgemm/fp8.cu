@@ -169,10 +169,14 @@ int prepare_kernel(Kernel fn, int id, int smem, int threads, int clusters[4])
     return VK_OK;
 }
 
-// Shares the tiles out.  Fewer tiles than clusters of several pairs: as many pairs to a tile as can all run at once, each
-// with at least `least` grains of k.  Otherwise the tiles of a last wave that at most half of the pairs would have are
-// halved.
-int plan_work(TileWork& w, const int clusters[4], int least)
+// Shares the tiles out.  Fewer tiles than clusters of several pairs: as many pairs to a tile as can all run at once, where
+// that saves each of them kShareSaves stages: the join takes as long as 15 or so (512 x 4096 x 4096, two pairs, 8 stages
+// saved: 16.1 us, unshared 13.6; k = 8192, 16 saved: 21.7 and 22.3; k = 16384: 33.4 and 38.9.  Weight gradients of
+// 1000 x 1000, three pairs: 2048 tokens, 10 saved: 18.1 and 15.5; 3500, 18 saved: 20.8 and 22.0; 5000: 24.9 and 28.9).
+// Otherwise the tiles of a last wave that at most half of the pairs would have are halved (4000 x 5120 x 3000 51.2 us,
+// with whole tiles 52.8; weight gradient 8192 x 4096 x 4096 211 and 217).
+constexpr int kShareSaves = 16;
+int plan_work(TileWork& w, const int clusters[4])
 {
     const long long tiles = static_cast<long long>(w.tiles_m) * w.tiles_n;
     const int grains = (w.stages + w.grain - 1) / w.grain;
@@ -180,7 +184,7 @@ int plan_work(TileWork& w, const int clusters[4], int least)
     w.pairs = 1;
     w.halved = 0;
     for (int s = 4; s >= 2; --s)
-        if (tiles <= clusters[s - 1] && grains >= s * least) {
+        if (tiles <= clusters[s - 1] && w.stages - (grains + s - 1) / s * w.grain >= kShareSaves) {
             w.pairs = s;
             return static_cast<int>(tiles);
         }
@@ -488,7 +492,7 @@ static int launch_gemm(F8GemmParams p, const CUtensorMap& ta, const CUtensorMap&
     int fit[4];
     const int rc = prepare_kernel(gemm_fp8_kernel<OUT>, OUT, kF8SmemBytes, kF8Threads, fit);
     if (rc != VK_OK) return rc;
-    const int clusters = plan_work(p.work, fit, 2);
+    const int clusters = plan_work(p.work, fit);
     return launch_clusters(gemm_fp8_kernel<OUT>, clusters, 2 * p.work.pairs, kF8Threads, kF8SmemBytes, stream, ta, tb, tc, p);
 }
 
@@ -509,7 +513,7 @@ static int launch_thin(ThinParams p, const CUtensorMap& tb, const CUtensorMap& t
 }
 
 // Scales as the tensor-core kernels read them: strides per output index (or tile) and per k-block.
-static ScaleSource scales(const void* p, long long ld, int64_t count, int scaling, bool along_row)
+static ScaleSource scales(const void* p, long long ld, int64_t count, int scaling, bool along_row, int num_kb)
 {
     ScaleSource s;
     s.p = static_cast<const uint8_t*>(p);
@@ -517,7 +521,8 @@ static ScaleSource scales(const void* p, long long ld, int64_t count, int scalin
     s.st = along_row ? 1 : ld;
     s.count = static_cast<int>(count);
     s.tile = scaling == VK_FP8_TILE;
-    s.words = along_row && rows_at(p, ld, 1, 4);
+    s.aligned = along_row && rows_at(p, ld, 1, 4);
+    s.end = s.p + ((scaling == VK_FP8_TILE ? (count + 127) / 128 : count) - 1) * s.si + (num_kb - 1) * s.st + 1;
     return s;
 }
 
@@ -553,13 +558,14 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     if (a->k > 0 && tma_ok(a->A, lda, 1) && tma_ok(a->B, ldb, 1)) {
+        const int num_kb = static_cast<int>(kb);
         if (a->trans_b && a->m <= 128) {
             ThinParams p;
             p.M = static_cast<int>(a->m);
             p.N = static_cast<int>(a->n);
             p.K = static_cast<int>(a->k);
-            p.sa = scales(a->a_scale, ldas, a->m, a->a_scaling, true);
-            p.sb = scales(a->b_scale, ldbs, a->n, a->b_scaling, true);
+            p.sa = scales(a->a_scale, ldas, a->m, a->a_scaling, true, num_kb);
+            p.sb = scales(a->b_scale, ldbs, a->n, a->b_scaling, true, num_kb);
             p.C = a->C;
             p.ldc = ldc;
             p.timeout_ns = wait_timeout_ns();
@@ -590,8 +596,8 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
         p.work.n = p.N;
         p.work.stages = static_cast<int>((a->k + 255) / 256);
         p.work.grain = 2;  // a slice begins with a whole set of scales
-        p.sa = scales(a->a_scale, ldas, a->m, a->a_scaling, true);
-        p.sb = scales(a->b_scale, ldbs, a->n, a->b_scaling, a->trans_b);
+        p.sa = scales(a->a_scale, ldas, a->m, a->a_scaling, true, num_kb);
+        p.sb = scales(a->b_scale, ldbs, a->n, a->b_scaling, a->trans_b, num_kb);
         p.b_k = a->trans_b;
         p.C = a->C;
         p.ldc = ldc;
@@ -627,7 +633,7 @@ static int launch_wgrad(WgradParams p, const CUtensorMap& ta, const CUtensorMap&
     int fit[4];
     const int rc = prepare_kernel(wgrad_fp8_kernel<T, OUT>, kId, kWgSmemBytes, kWgThreads, fit);
     if (rc != VK_OK) return rc;
-    const int clusters = plan_work(p.work, fit, 4);
+    const int clusters = plan_work(p.work, fit);
     return launch_clusters(wgrad_fp8_kernel<T, OUT>, clusters, 2 * p.work.pairs, kWgThreads, kWgSmemBytes, stream, ta, tc, p);
 }
 

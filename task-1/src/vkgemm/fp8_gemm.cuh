@@ -8,7 +8,7 @@
 //
 // Roles (224 threads per CTA, one CTA per SM, pairs of CTAs on one 256 x 256 tile, persistent over tiles):
 //   warp 0      TMA loads: 256-deep stages of A (128 rows) and B (this CTA's 128 of the tile's 256 columns), 64 KB each.
-//   warp 1      tensor memory, and in the pair's leader the MMAs (one lane).
+//   warp 1      tensor memory, and in the pair's leader the MMAs.
 //   warps 2..5  epilogue: tensor memory -> registers -> swizzled staging -> TMA stores.
 //   warp 6      scales: global bytes -> the 512-byte units that tcgen05.cp copies to tensor memory.
 //
@@ -31,27 +31,111 @@
 
 namespace vk {
 
-// The scales of one operand: the word of four k-blocks for an output index (a row of A, a row or column of B).
+// Four scales that are st apart, one by one; those from `left` on are 1.
+__device__ __noinline__ uint32_t scale_bytes(const uint8_t* at, long long st, int left)
+{
+    uint32_t w = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) w |= (b < left ? static_cast<uint32_t>(at[b * st]) : 127u) << (8 * b);
+    return w;
+}
+
+// A word of scales of which only the first `left` k-blocks exist.
+__device__ __forceinline__ uint32_t scale_word(uint32_t w, int left)
+{
+    return left >= 4 ? w : (w & ~(0xffffffffu << (8 * left))) | (0x7f7f7f7fu << (8 * left));
+}
+
+// The scales of one operand, as words of four k-blocks for each output index (a row of A, a row or column of B).  (40 bytes:
+// with 48, the kernel for few rows of A is compiled to a slower join, 128 x 4096 x 4096 11.6 us for 9.5.)
 struct ScaleSource {
     const uint8_t* p;
-    long long si, st;  // strides per output index (or tile of 128) and per k-block
-    int count;         // output indexes
-    int tile;          // a scale for 128 output indexes
-    int words;         // four k-blocks from a multiple of four are an aligned 32-bit word
+    const uint8_t* end;  // behind the last scale
+    long long si, st;    // strides per output index (or tile of 128) and per k-block
+    int count;           // output indexes
+    unsigned tile : 1;     // a scale for 128 output indexes
+    unsigned aligned : 1;  // four k-blocks from a multiple of four are an aligned 32-bit word
 
-    // k-blocks kb..kb+3 of output index i; what does not exist is 1
-    __device__ __forceinline__ uint32_t word(int i, int kb, int num_kb) const
+    __device__ __forceinline__ const uint8_t* at(int i, int kb) const
     {
-        if (i >= count) return 0x7f7f7f7fu;
-        const uint8_t* s = p + static_cast<long long>(tile ? i >> 7 : i) * si;
-        if (words && (kb & 3) == 0 && kb + 4 <= num_kb) return *reinterpret_cast<const uint32_t*>(s + kb);
-        uint32_t w = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b)
-            w |= (kb + b < num_kb ? static_cast<uint32_t>(s[static_cast<long long>(kb + b) * st]) : 127u) << (8 * b);
-        return w;
+        return i < count ? p + static_cast<long long>(tile ? i >> 7 : i) * si + static_cast<long long>(kb) * st : nullptr;
     }
 };
+
+// The words of k-blocks kb..kb+3 of N output indexes, k-blocks being neighbours: out of the one or two aligned words around
+// them, as rows of scales may begin anywhere (k = 11008 has 86 blocks: 4096 x 4096 x 11008 byte by byte 230 us, against 135).
+// What would reach beyond the first or the last scale is left to the bytes.  Apart: the loads, and their use, so that those
+// of both operands are in flight together.  Used by whole warps.
+template <int N>
+struct ScaleWords {
+    const uint8_t* from[N];  // what is left to the bytes
+    uint32_t lo[N], hi[N], bits[N];
+    bool todo;
+
+    __device__ __forceinline__ void load(const ScaleSource& s, int i0, int step, int kb)
+    {
+        todo = false;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint8_t* at = s.at(i0 + step * j, kb);
+            const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at)) & 3u;
+            const uint8_t* w = at - off;
+            const bool in = w >= s.p && w + (off ? 8 : 4) <= s.end;  // (not of nullptr)
+            lo[j] = in ? *reinterpret_cast<const uint32_t*>(w) : 0x7f7f7f7fu;
+            hi[j] = in && off ? *reinterpret_cast<const uint32_t*>(w + 4) : 0x7f7f7f7fu;
+            bits[j] = off * 8;
+            from[j] = in ? nullptr : at;
+            todo |= from[j] != nullptr;
+        }
+    }
+    // left: the k-blocks that exist
+    __device__ __forceinline__ void use(uint32_t (&out)[N], int left)
+    {
+        const bool any = __any_sync(0xffffffffu, todo);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            out[j] = scale_word(__funnelshift_r(lo[j], hi[j], bits[j]), left);
+            if (any && from[j] != nullptr) out[j] = scale_bytes(from[j], 1, left);
+        }
+    }
+};
+
+// The same, whole: words of k-blocks kb..kb+3 of output indexes i0 + step * j (step 32 or 128).
+template <int N>
+__device__ __forceinline__ void fetch_words(uint32_t (&out)[N], const ScaleSource& s, int i0, int step, int kb, int left)
+{
+    if (s.aligned && left >= 4) {  // one load for each (4000 x 5120 x 3000, scales by rows: with two 54.7 us, against 51.5)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint8_t* at = s.at(i0 + step * j, kb);
+            out[j] = at != nullptr ? *reinterpret_cast<const uint32_t*>(at) : 0x7f7f7f7fu;
+        }
+    } else if (s.st == 1) {
+        ScaleWords<N> w;
+        w.load(s, i0, step, kb);
+        w.use(out, left);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint8_t* at = s.at(i0 + step * j, kb);
+            out[j] = at != nullptr ? scale_bytes(at, s.st, left) : 0x7f7f7f7fu;
+        }
+    }
+}
+
+// Output indexes 32 apart from i0, which is less than 32 above a multiple of 128: four of them share a tile's scale.
+template <int N>
+__device__ __forceinline__ void fetch_words(uint32_t (&out)[N], const ScaleSource& s, int i0, int kb, int left)
+{
+    if (s.tile) {
+        uint32_t w[N / 4];
+        fetch_words(w, s, i0, 128, kb, left);
+#pragma unroll
+        for (int j = 0; j < N; ++j) out[j] = w[j / 4];
+    } else {
+        fetch_words(out, s, i0, 32, kb, left);
+    }
+}
 
 // How the 256 x 256 tiles of an output are shared out over clusters.
 struct TileWork {
@@ -540,27 +624,23 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             const Work w = work_unit(p.work, u, part);
             const int m0 = w.tm * 256 + half * 128 + lane, n0 = w.n0 + lane;
             for (int kb = w.st0 * 2; kb < min(num_kb, w.st1 * 2); kb += 4, sf.next()) {
-                uint32_t s[12];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[i] = p.sa.word(m0 + 32 * i, kb, num_kb);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s[4 + i] = p.sb.word(n0 + 32 * i, kb, num_kb);
-                if (!mbar_wait(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at)) {
-                    ok = false;
-                    break;
-                }
+                uint32_t a[4], b[8];
+                fetch_words(a, p.sa, m0, kb, num_kb - kb);
+                fetch_words(b, p.sb, n0, kb, num_kb - kb);
+                ok = mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at);
+                if (!ok) break;
                 uint4* dst = reinterpret_cast<uint4*>(sSf + sf.at * kF8SfBytes) + lane;
-#pragma unroll
-                for (int i = 0; i < 3; ++i) dst[32 * i] = make_uint4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+                dst[0] = make_uint4(a[0], a[1], a[2], a[3]);
+                dst[32] = make_uint4(b[0], b[1], b[2], b[3]);
+                dst[64] = make_uint4(b[4], b[5], b[6], b[7]);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_pair(mapa_shared(sf_full_bar(sf.at), lead));
             }
-            ok = __all_sync(0xffffffffu, ok);
         }
         // as above
         for (int i = 0; ok && i < kF8SfSlots; ++i, sf.next())
-            ok = mbar_wait(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitTail, 200 + sf.at);
+            ok = mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitTail, 200 + sf.at);
     }
 
     const bool epilogue = warp >= 2 && warp < 6;

@@ -157,15 +157,18 @@ __global__ void __launch_bounds__(kThinThreads, 1)
     } else if (warp == 6) {
         Ring sf(kThinSfSlots);
         for (int kb = kb0; kb < kb1; kb += 4, sf.next()) {
-            uint32_t b[4], a[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = p.sb.word(n0 + lane + 32 * i, kb, num_kb);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = 32 * i < NPAD ? p.sa.word(lane + 32 * i, kb, num_kb) : 0x7f7f7f7fu;
+            constexpr int kWords = (NPAD + 31) / 32;
+            uint32_t b[4], a[kWords];
+            ScaleWords<4> of_b;
+            ScaleWords<kWords> of_a;
+            of_b.load(p.sb, n0 + lane, 32, kb);
+            of_a.load(p.sa, lane, 32, kb);
+            of_b.use(b, num_kb - kb);
+            of_a.use(a, num_kb - kb);
             if (!mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at)) break;
             uint4* dst = reinterpret_cast<uint4*>(sSf + sf.at * kThinSfBytes) + lane;
             dst[0] = make_uint4(b[0], b[1], b[2], b[3]);
-            dst[32] = make_uint4(a[0], a[1], a[2], a[3]);
+            dst[32] = make_uint4(a[0], a[kWords > 1 ? 1 : 0], a[kWords > 2 ? 2 : 0], a[kWords > 2 ? 3 : 0]);  // (of rows that the MMA does not have: any)
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(sf_full_bar(sf.at));

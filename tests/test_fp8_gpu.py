@@ -371,6 +371,36 @@ def test_gemm_few_rows(vk, shape, layout):
     test_gemm(vk, shape, layout, F32)
 
 
+# few tiles and a long sum: two, three and four pairs to a tile
+@pytest.mark.parametrize("shape", [(300, 520, 6000), (1000, 1200, 7000), (1024, 1900, 9000), (257, 1001, 8192), (130, 100, 20000)])
+@pytest.mark.parametrize("layout", ["nt_tile", "nt_row", "nn"])
+@pytest.mark.parametrize("out", [F16, F32])
+def test_gemm_shared_tiles(vk, shape, layout, out):
+    test_gemm(vk, shape, layout, out)
+
+
+@pytest.mark.parametrize("m", [5, 300])
+@pytest.mark.parametrize("k", [100, 500, 700, 1100, 1700, 2100, 8000])
+@pytest.mark.parametrize("lead,tail", [(0, 0), (0, 1), (1, 0), (2, 1), (3, 2), (1, 3), (4, 4)])
+def test_gemm_scales_anywhere(vk, lead, tail, k, m):
+    """Rows of scales at any byte of a larger matrix of NaN scales: the same bits as packed ones."""
+    n = 200
+    a, sa = _quantized((m, k), 46)
+    b, sb = _quantized((n, k), 47)
+    want = vk.gemm_fp8(a, sa, b, sb, trans_b=True, out_dtype=F32)
+    for tile in (False, True):
+        if tile:
+            b, sb = _quantized((n, k), 47, True)
+            want = vk.gemm_fp8(a, sa, b, sb, trans_b=True, out_dtype=F32)
+        moved = []
+        for sc in (sa, sb):
+            view, _ = _inside(tuple(sc.shape), torch.float8_e8m0fnu, lead, tail, 0xff)
+            view.view(torch.uint8).copy_(sc.view(torch.uint8))
+            moved.append(view)
+        got = vk.gemm_fp8(a, moved[0], b, moved[1], trans_b=True, out_dtype=F32)
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("m", [4, 200])
 def test_gemm_tile_scales_of_a(vk, m):
     a, sa = _quantized((m, 1000), 32, True)
@@ -472,6 +502,13 @@ def test_wgrad(vk, shape, dtype, out):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_wgrad_waves(vk, shape, dtype):
     test_wgrad(vk, shape, dtype, None)
+
+
+@pytest.mark.parametrize("shape", [(3000, 300, 520), (4001, 1000, 1000), (5000, 1024, 1900), (12000, 64, 100)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("out", [None, F32])
+def test_wgrad_shared_tiles(vk, shape, dtype, out):
+    test_wgrad(vk, shape, dtype, out)
 
 
 @pytest.mark.parametrize("lead,tail", [(1, 2), (16, 16)])
