@@ -197,7 +197,8 @@ int vk_matmul_f32(int version, size_t m, size_t n, size_t k, const float* A, con
  * These calls are asynchronous on `stream`, allocate nothing, and can be captured into a CUDA graph.  A leading
  * dimension of 0 stands for the row's length.  The results of a call do not change from run to run.  Rows of operands
  * that start at 16-byte boundaries run on the tensor cores; any other alignment is taken by a (slow) CUDA-core kernel.
- * Outputs must not overlap inputs, except where said. */
+ * Bytes between rows of scales may be read, but take no part in the result.  Outputs must not overlap inputs, except
+ * where said. */
 typedef enum vk_fp8_scaling { VK_FP8_ROW = 0, VK_FP8_TILE = 1 } vk_fp8_scaling;
 
 /* Q, scale = the 8-bit form of X[rows x cols] (fp16, bf16 or fp32). */

@@ -363,7 +363,8 @@ extern "C" int vk_rmsnorm_fp8(const vk_rmsnorm_fp8_args* a)
 
 // How the backward pass is laid out: threads of a CTA with nv vectors of 8 columns each (nv = 0: the kernel for any number
 // of columns), and CTAs, each with a row of fp32 partial sums in the workspace.  Narrow rows need several CTAs on an SM
-// to keep memory busy; a CTA has four rows at least, so that the partial sums stay few.
+// to keep memory busy (8000 x 1000: 18.6 us, with one on each 46.9); a CTA has four rows at least, so that the partial sums
+// stay few.
 struct NormBackPlan {
     int nv, threads, per_sm;
     int64_t parts;
@@ -559,6 +560,8 @@ extern "C" int vk_gemm_fp8(const vk_gemm_fp8_args* a)
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);
     if (a->k > 0 && tma_ok(a->A, lda, 1) && tma_ok(a->B, ldb, 1)) {
         const int num_kb = static_cast<int>(kb);
+        // Up to 128 rows of A, B is the MMA's M: 128 x 4096 x 4096 9.6 us, as pairs of CTAs 15.4; 100 x 1000 x 1000 8.4 and 7.9;
+        // 128 x 16384 x 4096 20.0 and 19.8.  (With B stored k x n there is no such kernel.)
         if (a->trans_b && a->m <= 128) {
             ThinParams p;
             p.M = static_cast<int>(a->m);

@@ -16,6 +16,10 @@
 // accumulator begins at column 224: the two share 32 columns, which the epilogue reads first; the next tile's MMAs start
 // once it has.  Columns 480..511 hold two sets of scales (4 columns for A's 128 rows, 8 for B's 256), each for 512 of k.
 //
+// Bound by the MMAs: a stage of a whole tile takes 990 of the 1024 clocks that eight 256 x 256 x 32 instructions are rated at
+// (8192 x 8192 x 8192 bf16 out 376 us, 2.9 PFLOP/s, until the power limit lowers the clock; 4096 x 4096 x 4096 51.5 us, B
+// stored k x n 53.7).  Half tiles read as much of A for half the work, 0.48 us a stage instead of 0.3.
+//
 // How tiles are handed out (TileWork): pairs walk over whole tiles; when the last wave would leave half of them or more
 // without one, its tiles are cut into column halves.  (Cutting them along k, with the partial sums joined through
 // global memory, was built and measured first: writing the sums took 5 us and adding them 10, which held up the next

@@ -74,7 +74,8 @@ __device__ __forceinline__ Vec8<T> sum8(const Vec8<T>& a, const Vec8<T>& b)
 // Elements c .. c + 7 of a row that begins at `row` and has `cols` (those it does not have become zeros).
 // VEC: rows are 16-byte aligned and cols a multiple of 8; the load is one predicated instruction, and several stay in
 // flight together.  Otherwise the two aligned 16-byte units around the elements are loaded and shifted where both lie
-// in the row, and single elements at its ends (rows of 3333 bf16: norm 56 -> 35 us against single elements everywhere).
+// in the row, and single elements at its ends (4001 x 3333 bf16: norm 36 us, against 56 with single elements
+// everywhere).
 template <bool VEC, typename T>
 __device__ __forceinline__ Vec8<T> load8(const T* row, int c, int cols)
 {
@@ -244,8 +245,8 @@ struct QuantParams {
 };
 
 // Rows: 16 lanes hold one block, 8 values each, and have four neighbouring blocks of a row, so that four loads are in
-// flight and the four scales leave in one store.  16 such quads to a CTA.  (Blocks one by one, a grid apart: 8192 x 8192
-// bf16 45 us.)
+// flight and the four scales leave in one store.  16 such quads to a CTA.  Bound by memory: 8192 x 8192 bf16 31.5 us, 6.4 TB/s
+// (blocks one by one, a grid apart: 45 us).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
 {
@@ -280,6 +281,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
 }
 
 // One 128 x 128 tile per CTA, held in registers between its maximum and its rounding: 16 lanes per row, 16 rows at a time.
+// Bound by memory: 16384 x 4096 bf16 31 us, 6.5 TB/s.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p)
 {
@@ -516,7 +518,8 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const Nor
 
 // The same for rows of at most 512 * 8 * NV columns; dweight's share stays in registers.  VEC (16-byte aligned rows, a
 // multiple of 8 columns): rows arrive ahead in shared memory, one bulk copy per tensor and row, p.stages rows deep, so
-// that memory stays busy through the two passes and the barrier of each row.  Otherwise from memory as they are needed.
+// that memory stays busy through the two passes and the barrier of each row: 8192 x 8192 bf16 with dres 86.5 us, 6.2 TB/s.
+// Otherwise from memory as they are needed (4001 x 3333: 61 us).
 template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_kernel(const NormBackParams p)
 {

@@ -1,5 +1,6 @@
 // CUDA-core products of 8-bit operands: any strides, alignment and layout (what the tensor-core kernels' TMA
-// loads cannot describe), fp32 accumulation in the order of the contraction.
+// loads cannot describe), fp32 accumulation in the order of the contraction.  Bound by the CUDA cores; a fallback that
+// is not tuned further.
 #pragma once
 
 #include <type_traits>

@@ -3,7 +3,8 @@
 // The roles of the operands are swapped: 128 rows of B are the MMA's M, the few rows of A its N (16 to 128), so that no
 // tensor work is spent on rows that do not exist and B streams through the whole GPU.  A tile of 128 rows of B is shared
 // by a cluster of up to 8 CTAs, each with its part of k; they add their sums through shared memory, in the order of k.  A CTA
-// has as many loads in flight as its shared memory holds (200 KB), which for common sizes is all it will ever load.
+// has as many loads in flight as its shared memory holds (200 KB), which for common sizes is all it will ever load.  1 x 16384 x
+// 4096 15 us, 4.5 TB/s; 8 x 4096 x 4096 6.2 us, of which 3 are setup, one trip to memory and the join.
 //
 // Roles (224 threads): warp 0 TMA loads, warp 1 tensor memory and MMAs, warps 2..5 epilogue, warp 6 scales (as in
 // fp8_gemm.cuh).
