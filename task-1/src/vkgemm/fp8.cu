@@ -363,8 +363,8 @@ extern "C" int vk_rmsnorm_fp8(const vk_rmsnorm_fp8_args* a)
 
 // How the backward pass is laid out: threads of a CTA with nv vectors of 8 columns each (nv = 0: the kernel for any number
 // of columns), and CTAs, each with a row of fp32 partial sums in the workspace.  Narrow rows need several CTAs on an SM
-// to keep memory busy (8000 x 1000: 18.6 us, with one on each 46.9); a CTA has four rows at least, so that the partial sums
-// stay few.
+// to keep memory busy (8000 x 1000: 18.6 us, with one on each 46.9); where rows are few, a CTA has two (777 x 1000: 6.4 us, with four
+// 7.2).
 struct NormBackPlan {
     int nv, threads, per_sm;
     int64_t parts;
@@ -376,7 +376,7 @@ static NormBackPlan norm_backward_plan(int64_t rows, int64_t cols)
     plan.nv = cols <= 512 * 8 ? 1 : cols <= 512 * 16 ? 2 : 0;
     plan.threads = plan.nv ? static_cast<int>(((cols + 7) / 8 + plan.nv - 1) / plan.nv + 31) / 32 * 32 : 512;
     plan.per_sm = plan.nv != 1 ? 1 : plan.threads <= 128 ? 8 : plan.threads <= 256 ? 4 : 2;
-    const int64_t most = 148 * plan.per_sm, wanted = (rows + 3) / 4;
+    const int64_t most = 148 * plan.per_sm, wanted = (rows + 1) / 2;
     plan.parts = wanted < 148 ? (rows < 148 ? rows : 148) : wanted < most ? wanted : most;
     return plan;
 }
