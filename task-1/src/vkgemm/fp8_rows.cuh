@@ -495,7 +495,9 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const Nor
     __shared__ float slots[2][16];
     const T* w = static_cast<const T*>(p.weight);
     float* part = p.part + static_cast<long long>(blockIdx.x) * p.cols;
-    for (int c = threadIdx.x; c < p.cols; c += blockDim.x) part[c] = 0.f;
+    // (unsigned: a thread's last column and blockDim.x add up to more than an int where cols is near its end)
+    const unsigned cols = static_cast<unsigned>(p.cols);
+    for (unsigned c = threadIdx.x; c < cols; c += blockDim.x) part[c] = 0.f;
     int turn = 0;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
@@ -504,9 +506,9 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const Nor
         T* dx = static_cast<T*>(p.dx) + row * p.lddx;
         const float rstd = p.rstd[row];
         float dot = 0.f;
-        for (int c = threadIdx.x; c < p.cols; c += blockDim.x) dot = fmaf(to_f32(dy[c]) * to_f32(w[c]), to_f32(h[c]) * rstd, dot);
+        for (unsigned c = threadIdx.x; c < cols; c += blockDim.x) dot = fmaf(to_f32(dy[c]) * to_f32(w[c]), to_f32(h[c]) * rstd, dot);
         const float mean = cta_sum(dot, slots[turn]) * p.inv_cols;
-        for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
+        for (unsigned c = threadIdx.x; c < cols; c += blockDim.x) {
             const float dyf = to_f32(dy[c]), xhat = to_f32(h[c]) * rstd;
             float t = rstd * (dyf * to_f32(w[c]) - xhat * mean);
             if (dres != nullptr) t += to_f32(dres[c]);

@@ -788,3 +788,55 @@ print("captured")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+# ------------------------------------------------------------------------------------------ largest sizes
+WIDEST = 2 ** 31 - 256  # the most columns a matrix may have
+END = 384               # whole blocks; what lies between both ends is zero
+
+
+def _widest(dtype, seed):
+    x = torch.zeros((1, WIDEST), dtype=dtype, device="cuda")
+    x[:, :END], x[:, -END:] = _rand((1, END), dtype, seed), _rand((1, END), dtype, seed + 1)
+    return x
+
+
+def _ends(t, n=END):
+    return torch.cat([t[..., :n], t[..., -n:]], dim=-1)
+
+
+@pytest.mark.parametrize("tile", [False, True])
+def test_widest_rows_quantized(vk, tile):
+    x = _widest(BF16, 160)
+    q, s = vk.quantize_fp8(x, tile=tile)
+    codes, scale = fp8.quantize(_ends(x).double().cpu().numpy(), tile)
+    np.testing.assert_array_equal(_bytes(_ends(q)), codes)
+    np.testing.assert_array_equal(_bytes(_ends(s, END // 128)), scale)
+    assert torch.count_nonzero(q.view(torch.uint8)) == np.count_nonzero(codes)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_widest_rows_normalised_and_back(vk, dtype):
+    x, w = _widest(dtype, 162), _widest(dtype, 164)[0]
+    q, s, h, rstd = vk.rmsnorm_fp8(x, w, residual=x)
+    he, we = _ends(h).double(), _ends(w).double()
+    assert torch.equal(_ends(h), (2 * _ends(x).float()).to(dtype))
+    r64 = (he.square().sum() / WIDEST + 1e-6).rsqrt()
+    assert abs(rstd[0].double() - r64) <= 100 * U * r64
+    y = he * r64 * we
+    per = torch.from_numpy(fp8.E8M0).cuda()[_ends(s, END // 128).view(torch.uint8).long()].repeat_interleave(128, 1)
+    off = (_deq(_ends(q), _ends(s, END // 128)) - y).abs()
+    assert (off <= torch.maximum(2.0 ** -4 * y.abs(), 2.0 ** -10 * per) * (1 + 2.0 ** -12) + 104 * U * y.abs()).all()
+    assert torch.count_nonzero(q.view(torch.uint8)[:, END:-END]) == 0
+    del q, s, x
+    dy = _widest(dtype, 166)
+    dx, dw = vk.rmsnorm_fp8_backward(dy, h, w, rstd)
+    d, r = _ends(dy).double(), rstd.double()
+    g, xhat = d * we, he * r
+    want = r * (g - xhat * (g * xhat).sum() / WIDEST)
+    size = r * (g.abs() + xhat.abs() * (g * xhat).abs().sum() / WIDEST)
+    assert ((_ends(dx).double() - want).abs() <= 104 * U * size + HALF[dtype] * (1 + 2.0 ** -8) * want.abs() + TINY[dtype]).all()
+    assert ((_ends(dw).double() - (d * xhat)[0]).abs() <= 4 * U * (d * xhat).abs()[0]).all()
+    assert torch.count_nonzero(dx[:, END:-END]) == 0 and torch.count_nonzero(dw[END:-END]) == 0
+    del dx, dw, dy, h
+    torch.cuda.empty_cache()
