@@ -481,8 +481,8 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
 template <typename LA, typename LB>
 static int launch_simt(const LA& la, const LB& lb, const F8Output& out, int64_t m, int64_t n, int64_t k, cudaStream_t stream)
 {
-    const dim3 grid(static_cast<unsigned>((n + 63) / 64), static_cast<unsigned>((m + 63) / 64));
-    if (grid.y > 65535u) return set_error(VK_ERR_UNSUPPORTED, "m too large for the CUDA-core kernel");
+    const int64_t rows = (m + 63) / 64;  // of tiles
+    const dim3 grid(static_cast<unsigned>((n + 63) / 64), static_cast<unsigned>(rows < 65535 ? rows : 65535));
     fp8_simt_kernel<<<grid, 256, 0, stream>>>(la, lb, out, m, n, k);
     return launched();
 }

@@ -76,37 +76,40 @@ __device__ __forceinline__ void put_output(const F8Output& o, long long row, lon
     }
 }
 
-// C[i][j] = sum over t of a(i, t) * b(j, t): 64 x 64 tile, 256 threads of 4 x 4 outputs, 16 steps of t at a time.
+// C[i][j] = sum over t of a(i, t) * b(j, t): 64 x 64 tile, 256 threads of 4 x 4 outputs, 16 steps of t at a time.  A grid has
+// at most 65535 rows of CTAs, so a CTA walks over tile rows.
 template <typename LA, typename LB>
 __global__ void __launch_bounds__(256) fp8_simt_kernel(const LA a, const LB b, const F8Output out, long long M, long long N, long long K)
 {
     __shared__ float sa[16][65], sb[16][65];
-    const long long i0 = static_cast<long long>(blockIdx.y) * 64, j0 = static_cast<long long>(blockIdx.x) * 64;
+    const long long j0 = static_cast<long long>(blockIdx.x) * 64;
     const int ti = threadIdx.x >> 4, tj = threadIdx.x & 15;
-    float acc[4][4] = {};
-    for (long long t0 = 0; t0 < K; t0 += 16) {
+    for (long long i0 = static_cast<long long>(blockIdx.y) * 64; i0 < M; i0 += static_cast<long long>(gridDim.y) * 64) {
+        float acc[4][4] = {};
+        for (long long t0 = 0; t0 < K; t0 += 16) {
 #pragma unroll
-        for (int e = threadIdx.x; e < 1024; e += 256) {
-            const int t = e & 15, i = e >> 4;
-            sa[t][i] = (i0 + i < M && t0 + t < K) ? a.at(i0 + i, t0 + t) : 0.f;
-            sb[t][i] = (j0 + i < N && t0 + t < K) ? b.at(j0 + i, t0 + t) : 0.f;
+            for (int e = threadIdx.x; e < 1024; e += 256) {
+                const int t = e & 15, i = e >> 4;
+                sa[t][i] = (i0 + i < M && t0 + t < K) ? a.at(i0 + i, t0 + t) : 0.f;
+                sb[t][i] = (j0 + i < N && t0 + t < K) ? b.at(j0 + i, t0 + t) : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) acc[y][x] = fmaf(sa[t][ti + 16 * y], sb[t][tj + 16 * x], acc[y][x]);
+            __syncthreads();
         }
-        __syncthreads();
 #pragma unroll
-        for (int t = 0; t < 16; ++t)
+        for (int y = 0; y < 4; ++y)
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) acc[y][x] = fmaf(sa[t][ti + 16 * y], sb[t][tj + 16 * x], acc[y][x]);
-        __syncthreads();
+            for (int x = 0; x < 4; ++x) {
+                const long long i = i0 + ti + 16 * y, j = j0 + tj + 16 * x;
+                if (i < M && j < N) put_output(out, i, j, acc[y][x]);
+            }
     }
-#pragma unroll
-    for (int y = 0; y < 4; ++y)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const long long i = i0 + ti + 16 * y, j = j0 + tj + 16 * x;
-            if (i < M && j < N) put_output(out, i, j, acc[y][x]);
-        }
 }
 
 }  // namespace vk

@@ -840,3 +840,33 @@ def test_widest_rows_normalised_and_back(vk, dtype):
     assert torch.count_nonzero(dx[:, END:-END]) == 0 and torch.count_nonzero(dw[END:-END]) == 0
     del dx, dw, dy, h
     torch.cuda.empty_cache()
+
+
+TALL = 2 * 64 * 65535 + 33  # rows of tiles of the CUDA-core kernel: two grids' height and one more
+
+
+@pytest.mark.parametrize("k", [0, 3])
+def test_gemm_of_many_unaligned_rows(vk, k):
+    """More rows than a grid of the CUDA-core kernel has: every row is the product of its own operands."""
+    codes = torch.randint(0, 0x70, (TALL, max(k, 1)), generator=_gen(170), device="cuda", dtype=torch.uint8)[:, :k]
+    a = codes.contiguous().view(torch.float8_e4m3fn)
+    sa = torch.full((TALL, 1 if k else 0), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    b, sb = _quantized((2, k), 171, pad=False) if k else (a[:2], sa[:2])
+    c, room = _inside((TALL, 2), F32, 1, 1)
+    vk.gemm_fp8(a, sa, b, sb, c, trans_b=True)
+    if k:
+        av, bv = _deq(a, sa), _deq(b, sb).t()
+        _check_product(c, av @ bv, av.abs() @ bv.abs(), k)
+    else:
+        assert torch.count_nonzero(c) == 0
+    _untouched(room, (TALL, 2), 1)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_wgrad_of_many_unaligned_columns(vk, dtype):
+    dy = _rand((2, TALL), dtype, 172)
+    x, s = _quantized((2, 1), 173, pad=False)
+    base = _rand((TALL, 1), F32, 174)
+    d, xv = dy.double().t(), _deq(x, s)
+    _check_product(vk.wgrad_fp8(dy, x, s, out_dtype=F32), d @ xv, d.abs() @ xv.abs(), 2)
+    _check_product(vk.wgrad_fp8(dy, x, s, base.clone(), accumulate=True), d @ xv, d.abs() @ xv.abs(), 2, base)
