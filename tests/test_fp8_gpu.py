@@ -870,3 +870,16 @@ def test_wgrad_of_many_unaligned_columns(vk, dtype):
     d, xv = dy.double().t(), _deq(x, s)
     _check_product(vk.wgrad_fp8(dy, x, s, out_dtype=F32), d @ xv, d.abs() @ xv.abs(), 2)
     _check_product(vk.wgrad_fp8(dy, x, s, base.clone(), accumulate=True), d @ xv, d.abs() @ xv.abs(), 2, base)
+
+
+@pytest.mark.parametrize("m", [2, 300])
+@pytest.mark.parametrize("n", [40, 300])
+def test_gemm_of_nothing_not_transposed(vk, m, n):
+    """An empty sum with B stored k x n: zeros, whatever C held."""
+    a = torch.empty((m, 0), dtype=torch.float8_e4m3fn, device="cuda")
+    b = torch.empty((0, n), dtype=torch.float8_e4m3fn, device="cuda")
+    sa = torch.empty((m, 0), dtype=torch.float8_e8m0fnu, device="cuda")
+    sb = torch.empty((0, (n + 127) // 128), dtype=torch.float8_e8m0fnu, device="cuda")
+    c, room = _inside((m, n), BF16, 8, 8)
+    assert torch.count_nonzero(vk.gemm_fp8(a, sa, b, sb, c)) == 0
+    _untouched(room, (m, n), 8)

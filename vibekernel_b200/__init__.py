@@ -852,8 +852,8 @@ def gemm_fp8(A, a_scale, B, b_scale, C=None, *, trans_b: bool = False, out_dtype
         raise ValueError(f"A is {(m, k)} and B is {(b_rows, b_cols)} with trans_b={bool(trans_b)}")
     a_scaling, ldas = _scaling(F, a_scale, m, k, "a_scale", index)
     b_scaling, ldbs = _scaling(F, b_scale, b_rows, b_cols, "b_scale", index)
-    if not trans_b and b_rows == 1:
-        b_scaling = FP8_TILE  # one row: both forms are the same scales
+    if not trans_b and b_rows <= 1:
+        b_scaling = FP8_TILE  # one row or none: both forms are the same scales
     if out_dtype is None:
         out_dtype = F.f16 if C is None else C.dtype
     code = F.codes.get(out_dtype)
