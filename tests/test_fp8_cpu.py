@@ -163,3 +163,22 @@ def test_oracle_scales():
     assert s.tolist() == [[127, 128, 119, 0, 127, 255]]
     assert codes[0, 0] == 126 and (codes[0, 640:] == 127).all()
     assert not re.search("nan", str(fp8.values(codes, s)[0, :640]))
+
+
+def test_stream_of_another_device_is_refused():
+    """Torch would switch to the stream's device, and the call would then run on another stream of its own."""
+    class Tensor:
+        device = torch.device("cuda", 0)
+
+        def get_device(self):
+            return 0
+
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 0x1000
+
+    t, st = Tensor(), Stream()
+    for call in (lambda: vk.quantize_fp8(t, stream=st), lambda: vk.rmsnorm_fp8(t, t, stream=st),
+                 lambda: vk.rmsnorm_fp8_backward(t, t, t, t, stream=st), lambda: vk.gemm_fp8(t, t, t, t, stream=st),
+                 lambda: vk.wgrad_fp8(t, t, t, stream=st)):
+        with pytest.raises(ValueError, match="stream is on cuda:1"):
+            call()

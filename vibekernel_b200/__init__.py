@@ -627,6 +627,8 @@ def _elsewhere(F, t, stream):
     import contextlib
     guard = contextlib.ExitStack()
     if index >= 0:
+        if stream is not None and getattr(getattr(stream, "device", None), "index", index) != index:
+            raise ValueError(f"stream is on {stream.device}, the operands are on cuda:{index}")
         guard.enter_context(F.torch.cuda.device(index))
         if stream is not None:
             if not hasattr(stream, "cuda_stream"):
