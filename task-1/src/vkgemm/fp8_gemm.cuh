@@ -570,12 +570,12 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             for (int u = cluster_id; u < units; u += num_clusters, ++it) {
                 const Work w = work_unit(p.work, u, part);
                 // the unit before has left the columns the two accumulators share (and, before that, this one's)
-                if (!mbar_wait_warp(tempty_bar, static_cast<uint32_t>(it & 1) ^ 1u, p.timeout_ns, kErrWaitMma, 100)) return;
+                if (!mbar_wait_pair_warp(tempty_bar, static_cast<uint32_t>(it & 1) ^ 1u, p.timeout_ns, kErrWaitMma, 100)) return;
                 const uint32_t d = base + ((it & 1) ? kF8Acc1 : 0);
                 for (int st = w.st0; st < w.st1; ++st) {
                     const uint32_t sfa = base + kF8SfCol + set * 16, sfb = sfa + 4;
-                    if ((st & 1) == 0 && !mbar_wait_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) return;
-                    if (!mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) return;
+                    if ((st & 1) == 0 && !mbar_wait_pair_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) return;
+                    if (!mbar_wait_pair_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) return;
                     tc_fence_after();
                     const bool last = (st & 1) || st + 1 == w.st1;  // of its set of scales
                     if (one) {

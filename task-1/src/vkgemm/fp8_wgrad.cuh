@@ -165,11 +165,11 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             for (int u = cluster_id; ok && u < units; u += num_clusters, ++it) {
                 const Work w = work_unit(p.work, u, part);
                 const int acc = it & 1;
-                if (!mbar_wait_warp(tempty_bar(acc), (static_cast<uint32_t>(it >> 1) & 1u) ^ 1u, p.timeout_ns, kErrWaitMma, 100 + acc)) break;
+                if (!mbar_wait_pair_warp(tempty_bar(acc), (static_cast<uint32_t>(it >> 1) & 1u) ^ 1u, p.timeout_ns, kErrWaitMma, 100 + acc)) break;
                 const uint32_t d = base + static_cast<uint32_t>(acc * 256);
                 const uint32_t idesc = w.cols == 256 ? kIdesc : kIdescHalf;
                 for (int st = w.st0; st < w.st1; ++st, r.next()) {
-                    ok = mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at);
+                    ok = mbar_wait_pair_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at);
                     if (!ok) break;
                     tc_fence_after();
                     if (one) {

@@ -182,3 +182,18 @@ def test_stream_of_another_device_is_refused():
                  lambda: vk.wgrad_fp8(t, t, t, stream=st)):
         with pytest.raises(ValueError, match="stream is on cuda:1"):
             call()
+
+
+def test_arrivals_in_other_ctas_have_the_clusters_scope():
+    """An arrival without a scope is a release at the CTA's: it orders nothing for a waiting thread of another CTA."""
+    src = os.path.join(ROOT, "task-1", "src", "vkgemm")
+    for name in sorted(os.listdir(src)):
+        text = open(os.path.join(src, name)).read()
+        for line in re.findall(r'"[^"]*mbarrier\.arrive[^"]*shared::cluster[^"]*"', text):
+            if "tcgen05" not in line:
+                assert ".cluster.shared::cluster" in line, (name, line)
+    # the two data-carrying arrivals, and the waits of the pair's leader on them
+    for name in ("fp8_gemm.cuh", "fp8_wgrad.cuh"):
+        text = open(os.path.join(src, name)).read()
+        for bar in ("tempty_bar", "full_bar(r.at)" if name == "fp8_wgrad.cuh" else "sf_full_bar(sf.at)"):
+            assert re.search(r"mbar_wait_pair_warp\(" + re.escape(bar), text), (name, bar)
