@@ -516,11 +516,11 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    bool ok = true;  // no wait of this thread has given up
 
     if (warp == 0) {
         if (lane == 0) {
             Ring r(kF8Stages);
-            bool ok = true;
             for (int u = cluster_id; ok && u < units; u += num_clusters) {
                 const Work w = work_unit(p.work, u, part);
                 const int m0 = w.tm * 256 + half * 128, n0 = w.n0 + half * (w.cols / 2);
@@ -567,15 +567,16 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             Ring r(kF8Stages), sf(kF8SfSlots);
             int it = 0;
             uint32_t set = 0;
-            for (int u = cluster_id; u < units; u += num_clusters, ++it) {
+            for (int u = cluster_id; ok && u < units; u += num_clusters, ++it) {
                 const Work w = work_unit(p.work, u, part);
                 // the unit before has left the columns the two accumulators share (and, before that, this one's)
-                if (!mbar_wait_pair_warp(tempty_bar, static_cast<uint32_t>(it & 1) ^ 1u, p.timeout_ns, kErrWaitMma, 100)) return;
+                ok = mbar_wait_pair_warp(tempty_bar, static_cast<uint32_t>(it & 1) ^ 1u, p.timeout_ns, kErrWaitMma, 100);
                 const uint32_t d = base + ((it & 1) ? kF8Acc1 : 0);
-                for (int st = w.st0; st < w.st1; ++st) {
+                for (int st = w.st0; ok && st < w.st1; ++st) {
                     const uint32_t sfa = base + kF8SfCol + set * 16, sfb = sfa + 4;
-                    if ((st & 1) == 0 && !mbar_wait_pair_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) return;
-                    if (!mbar_wait_pair_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) return;
+                    if ((st & 1) == 0) ok = mbar_wait_pair_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at);
+                    ok = ok && mbar_wait_pair_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at);
+                    if (!ok) break;
                     tc_fence_after();
                     const bool last = (st & 1) || st + 1 == w.st1;  // of its set of scales
                     if (one) {
@@ -623,7 +624,6 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     } else if (warp == 6) {
         Ring sf(kF8SfSlots);
         const int num_kb = (p.K + 127) / 128;
-        bool ok = true;
         for (int u = cluster_id; ok && u < units; u += num_clusters) {
             const Work w = work_unit(p.work, u, part);
             const int m0 = w.tm * 256 + half * 128 + lane, n0 = w.n0 + lane;
@@ -658,7 +658,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         for (int u = cluster_id; u < units; u += num_clusters, ++it) {
             const Work w = work_unit(p.work, u, part);
             const int acc = it & 1;
-            if (!mbar_wait(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, p.timeout_ns, kErrWaitEpilogue, acc)) break;
+            ok = mbar_wait_warp(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, p.timeout_ns, kErrWaitEpilogue, acc);
+            if (!ok) break;
             tc_fence_after();
             // the shared columns first: the last 32 of accumulator 0, the first 32 of accumulator 1
             finish_unit<OUT>(w, out, stg, p.work.pairs > 1 ? sums : nullptr, tmem + (acc ? kF8Acc1 : 0), acc ? 0 : 7, half, q, lane, turn, [&] {
@@ -677,7 +678,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     if (epilogue && p.c_tma && lane == 0) bulk_wait_group_all();
 
     tc_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(!ok)) settle();
     cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();

@@ -558,9 +558,11 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_ker
     __syncthreads();
     int stage = 0, before = p.stages - 1, turn = 0;
     uint32_t phase = 0;
+    bool ok = true;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const float rstd = p.rstd[row];
-        if (VEC && !mbar_wait(smem_u32(&bars[stage]), phase, p.timeout_ns, kErrWaitProducer, stage)) break;
+        // A thread whose wait gives up goes on with whatever lies there: the others may not have, and count on it at the barrier.
+        if (VEC && ok) ok = mbar_wait(smem_u32(&bars[stage]), phase, p.timeout_ns, kErrWaitProducer, stage);
         const uint8_t* base = smem + static_cast<size_t>(stage) * 3 * pitch;
         const T* dy = VEC ? reinterpret_cast<const T*>(base) : static_cast<const T*>(p.dy) + row * p.lddy;
         const T* h = VEC ? reinterpret_cast<const T*>(base + pitch) : static_cast<const T*>(p.h) + row * p.ldh;
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_ker
         const float mean = cta_sum(dot.x + dot.y, slots[turn]) * p.inv_cols;
         // Behind this barrier no thread reads the row before any more: its stage is free.
         const long long ahead = row + static_cast<long long>(p.stages - 1) * gridDim.x;
-        if (VEC && threadIdx.x == 0 && row != blockIdx.x && ahead < p.rows) issue(ahead, before);
+        if (VEC && threadIdx.x == 0 && ok && row != blockIdx.x && ahead < p.rows) issue(ahead, before);
         T* dx = static_cast<T*>(p.dx) + row * p.lddx;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -602,6 +604,7 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_ker
             phase ^= 1u;
         }
     }
+    if (VEC && threadIdx.x == 0 && !ok) settle();
     float* part = p.part + static_cast<long long>(blockIdx.x) * p.cols;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {

@@ -101,13 +101,14 @@ __global__ void __launch_bounds__(kThinThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    bool ok = true;
+    bool ok = true;  // no wait of this thread has given up
 
     if (warp == 0) {
         if (lane == 0) {
             Ring r(kStages);
             for (int kb = kb0; kb < kb1; ++kb, r.next()) {
-                if (!mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitProducer, r.at)) break;
+                ok = mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitProducer, r.at);
+                if (!ok) break;
                 mbar_arrive_expect_tx(full_bar(r.at), Cfg::kStageBytes);
                 const uint32_t dst = smem_u32(stages + r.at * Cfg::kStageBytes);
                 tma_load_2d(dst, &tmap_b, full_bar(r.at), kb * 128, n0);
@@ -124,8 +125,9 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         uint32_t set = 0;
         for (int kb = kb0; kb < kb1; ++kb, r.next()) {
             const int in = (kb - kb0) & 3;  // of a set of scales
-            if (in == 0 && !mbar_wait_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) break;
-            if (!mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) break;
+            if (in == 0) ok = mbar_wait_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at);
+            ok = ok && mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at);
+            if (!ok) break;
             tc_fence_after();
             const uint32_t sfa = base + Cfg::kSfCol + set * 16, sfb = sfa + 8;
             const bool last = in == 3 || kb + 1 == kb1;
@@ -166,7 +168,8 @@ __global__ void __launch_bounds__(kThinThreads, 1)
             of_a.load(p.sa, lane, 32, kb);
             of_b.use(b, num_kb - kb);
             of_a.use(a, num_kb - kb);
-            if (!mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at)) break;
+            ok = mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at);
+            if (!ok) break;
             uint4* dst = reinterpret_cast<uint4*>(sSf + sf.at * kThinSfBytes) + lane;
             dst[0] = make_uint4(b[0], b[1], b[2], b[3]);
             dst[32] = make_uint4(a[0], a[kWords > 1 ? 1 : 0], a[kWords > 2 ? 2 : 0], a[kWords > 2 ? 3 : 0]);  // (of rows that the MMA does not have: any)
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         }
         cluster_sync_all();
     }
-    __syncthreads();
+    if (__syncthreads_or(!ok)) settle();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc<1>(tmem, Cfg::kTmemCols);

@@ -125,11 +125,11 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    bool ok = true;  // no wait of this thread has given up
 
     if (warp == 0) {
         if (lane == 0) {
             Ring r(kWgStages);
-            bool ok = true;
             for (int u = cluster_id; ok && u < units; u += num_clusters) {
                 const Work w = work_unit(p.work, u, part);
                 const int m0 = w.tm * 256 + half * 128;
@@ -161,11 +161,11 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             const uint64_t b_desc = smem_desc_sw128(smem_u32(sB), kWgBK * 128, 1024);
             Ring r(kWgStages);
             int it = 0;
-            bool ok = true;
             for (int u = cluster_id; ok && u < units; u += num_clusters, ++it) {
                 const Work w = work_unit(p.work, u, part);
                 const int acc = it & 1;
-                if (!mbar_wait_pair_warp(tempty_bar(acc), (static_cast<uint32_t>(it >> 1) & 1u) ^ 1u, p.timeout_ns, kErrWaitMma, 100 + acc)) break;
+                ok = mbar_wait_pair_warp(tempty_bar(acc), (static_cast<uint32_t>(it >> 1) & 1u) ^ 1u, p.timeout_ns, kErrWaitMma, 100 + acc);
+                if (!ok) break;
                 const uint32_t d = base + static_cast<uint32_t>(acc * 256);
                 const uint32_t idesc = w.cols == 256 ? kIdesc : kIdescHalf;
                 for (int st = w.st0; st < w.st1; ++st, r.next()) {
@@ -260,7 +260,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         uint8_t* dst = sB + group * kWgBBytes;
         if (u < units) fetch();
         while (u < units) {
-            if (!mbar_wait_warp(empty_bar(group), phase ^ 1u, p.timeout_ns, kErrWaitMma, 400 + group)) break;
+            ok = mbar_wait_warp(empty_bar(group), phase ^ 1u, p.timeout_ns, kErrWaitMma, 400 + group);
+            if (!ok) break;
             if (w.cols == 256)
                 convert(std::true_type{}, dst);
             else
@@ -285,7 +286,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         for (int u = cluster_id; u < units; u += num_clusters, ++it) {
             const Work w = work_unit(p.work, u, part);
             const int acc = it & 1;
-            if (!mbar_wait(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, p.timeout_ns, kErrWaitEpilogue, acc)) break;
+            ok = mbar_wait_warp(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, p.timeout_ns, kErrWaitEpilogue, acc);
+            if (!ok) break;
             tc_fence_after();
             finish_unit<OUT>(w, out, stg, p.work.pairs > 1 ? sums : nullptr, tmem + static_cast<uint32_t>(acc * 256), 0, half, q, lane, turn, [] {});
             tc_fence_before();
@@ -301,7 +303,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     if (epilogue && p.c_tma && lane == 0) bulk_wait_group_all();
 
     tc_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(!ok)) settle();
     cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();

@@ -194,6 +194,14 @@ __device__ __forceinline__ bool mbar_wait_pair(uint32_t bar, uint32_t parity, ui
     return ok;
 }
 
+// For a CTA in which a wait has given up, before it frees or leaves its memory: copies and MMAs that it issued may still be on
+// their way, and the barriers that would tell may never complete.  They take microseconds; this takes 20 ms.
+__device__ __forceinline__ void settle()
+{
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 20000000ull) __nanosleep(1000);
+}
+
 // ------------------------------------------------------------------------------------------
 // TMA (cp.async.bulk.tensor): every load fills only the issuing CTA's own shared memory.
 // ------------------------------------------------------------------------------------------

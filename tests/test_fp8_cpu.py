@@ -197,3 +197,21 @@ def test_arrivals_in_other_ctas_have_the_clusters_scope():
         text = open(os.path.join(src, name)).read()
         for bar in ("tempty_bar", "full_bar(r.at)" if name == "fp8_wgrad.cuh" else "sf_full_bar(sf.at)"):
             assert re.search(r"mbar_wait_pair_warp\(" + re.escape(bar), text), (name, bar)
+
+
+def test_waits_that_give_up_leave_in_order():
+    """What a kernel does once a bounded wait has run out, from its source (no call makes one run out on purpose): the lanes of
+    a warp with warp-wide instructions decide together, a CTA keeps its barriers, and it settles before it leaves."""
+    src = os.path.join(ROOT, "task-1", "src", "vkgemm")
+    for name in ("fp8_gemm.cuh", "fp8_wgrad.cuh", "fp8_thin.cuh"):
+        text = open(os.path.join(src, name)).read()
+        body = text[text.index("__global__"):]
+        # waits by single threads: only in the loading warp's one lane, and none whose answer is dropped
+        single = re.findall(r"(\S+ = |\bif \(!)?mbar_wait\((\w+)_bar", body)
+        assert single and all(how == "ok = " and bar == "empty" or how == "if (!" and bar == "empty" for how, bar in single), (name, single)
+        assert not re.search(r"if \(!mbar_wait\w*_warp\(", body), name
+        assert "__syncthreads_or(!ok)) settle();" in body, name
+        assert body.index("settle()") < body.index("tmem_dealloc"), name
+    text = open(os.path.join(src, "fp8_rows.cuh")).read()
+    body = text[text.index("rmsnorm_fp8_backward_kernel(const NormBackParams p)"):text.index("norm_weight_grad_kernel(")]
+    assert "break" not in body and "return" not in body and "if (VEC && threadIdx.x == 0 && !ok) settle();" in body
