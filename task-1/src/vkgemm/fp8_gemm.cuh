@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         for (int u = cluster_id; u < units; u += num_clusters, ++it) {
             const Work w = work_unit(p.work, u, part);
             const int acc = it & 1;
-            ok = mbar_wait_warp(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, p.timeout_ns, kErrWaitEpilogue, acc);
+            ok = mbar_wait_warp(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, sum_timeout_ns(p.timeout_ns, w.st1 - w.st0), kErrWaitEpilogue, acc);
             if (!ok) break;
             tc_fence_after();
             // the shared columns first: the last 32 of accumulator 0, the first 32 of accumulator 1

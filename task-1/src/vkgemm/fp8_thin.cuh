@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
             if (lane == 0) mbar_arrive(sf_full_bar(sf.at));
         }
     } else {
-        ok = mbar_wait_warp(done_bar, 0, p.timeout_ns, kErrWaitEpilogue, 0);
+        ok = mbar_wait_warp(done_bar, 0, sum_timeout_ns(p.timeout_ns, kb1 - kb0), kErrWaitEpilogue, 0);
         tc_fence_after();
     }
 

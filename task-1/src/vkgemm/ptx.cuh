@@ -194,6 +194,13 @@ __device__ __forceinline__ bool mbar_wait_pair(uint32_t bar, uint32_t parity, ui
     return ok;
 }
 
+// Limit of a wait for a whole sum, of `steps` stages that have a limit of timeout_ns each: 10 us for each of them (they take
+// 0.1 to 0.7 us) on top, so that a long sum that gets on is not given up.
+__device__ __forceinline__ uint64_t sum_timeout_ns(uint64_t timeout_ns, int steps)
+{
+    return timeout_ns + static_cast<uint64_t>(steps) * 10000u;
+}
+
 // For a CTA in which a wait has given up, before it frees or leaves its memory: copies and MMAs that it issued may still be on
 // their way, and the barriers that would tell may never complete.  They take microseconds; this takes 20 ms.
 __device__ __forceinline__ void settle()

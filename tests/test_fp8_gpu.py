@@ -883,3 +883,52 @@ def test_gemm_of_nothing_not_transposed(vk, m, n):
     c, room = _inside((m, n), BF16, 8, 8)
     assert torch.count_nonzero(vk.gemm_fp8(a, sa, b, sb, c)) == 0
     _untouched(room, (m, n), 8)
+
+
+@pytest.fixture
+def short_waits(vk):
+    vk.set_option("wait_timeout_ns", 1000000)
+    yield
+    vk.set_option("wait_timeout_ns", 2000000000)
+
+
+def _ones(rows, cols):
+    q = torch.full((rows, cols), 0x38, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    return q, torch.full((rows, (cols + 127) // 128), 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+
+
+@pytest.mark.parametrize("m,k", [(1, 2 ** 27), (130, 2 ** 25)])
+def test_gemm_sums_longer_than_the_wait_limit(vk, short_waits, m, k):
+    """A sum that takes many times the limit of a wait, each of its stages far less.  Every partial sum is exact."""
+    a, sa = _ones(m, k)
+    b, sb = _ones(8, k)
+    c = vk.gemm_fp8(a, sa, b, sb, trans_b=True, out_dtype=F32)
+    assert (c == k).all()
+    assert vk.device_error(0) == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_wgrad_sums_longer_than_the_wait_limit(vk, short_waits, dtype):
+    tokens = 2 ** 23
+    x, s = _ones(tokens, 16)
+    dw = vk.wgrad_fp8(torch.ones((tokens, 8), dtype=dtype, device="cuda"), x, s, out_dtype=F32)
+    assert (dw == tokens).all()
+    assert vk.device_error(0) == 0
+
+
+def test_longest_sums(vk):
+    """As many terms as a sum may have, those in the middle zero: the last ones' indexes end just below 2^31."""
+    x = _widest(BF16, 176)
+    q, s = vk.quantize_fp8(x)
+    b, sb = vk.quantize_fp8(_widest(BF16, 178))
+    del x
+    c = vk.gemm_fp8(q, s, b, sb, trans_b=True, out_dtype=F32)
+    av = _deq(_ends(q), _ends(s, END // 128))
+    bv = _deq(_ends(b), _ends(sb, END // 128)).t()
+    _check_product(c, av @ bv, av.abs() @ bv.abs(), 2 * END)
+    dy = _rand((1, 8), BF16, 180)
+    dw = vk.wgrad_fp8(dy, q, s, out_dtype=BF16)  # as wide an output
+    want = dy.double().t() @ av
+    _check_product(_ends(dw), want, want.abs(), 1)
+    del dw, b, sb, q, s
+    torch.cuda.empty_cache()
