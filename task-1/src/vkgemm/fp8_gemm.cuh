@@ -472,6 +472,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     uint8_t* sSf = epi + 4 * kF8EpiWarpBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sSf + kF8SfSlots * kF8SfBytes);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kF8Bars);
+    volatile uint32_t* gave_up = tmem_slot + 1;  // a wait of this CTA has
 
     const uint32_t bar0 = smem_u32(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -506,6 +507,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             mbar_init(sf_empty_bar(s), 1);
         }
         fence_mbar_init();
+        *gave_up = 0;
     }
     if (warp == 1) {
         tmem_alloc<2>(smem_u32(tmem_slot), 512);
@@ -516,11 +518,11 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    bool ok = true;  // no wait of this thread has given up
 
     if (warp == 0) {
         if (lane == 0) {
             Ring r(kF8Stages);
+            bool ok = true;
             for (int u = cluster_id; ok && u < units; u += num_clusters) {
                 const Work w = work_unit(p.work, u, part);
                 const int m0 = w.tm * 256 + half * 128, n0 = w.n0 + half * (w.cols / 2);
@@ -551,6 +553,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             // the MMAs' signals to this CTA's barriers have all arrived before the CTA may exit
             for (int i = 0; ok && i < kF8Stages; ++i, r.next())
                 ok = mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitTail, r.at);
+            if (!ok) *gave_up = 1;
         }
     } else if (warp == 1) {
         // The whole warp walks through the loop and one lane issues: what the instructions take is then the same in every
@@ -567,6 +570,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             Ring r(kF8Stages), sf(kF8SfSlots);
             int it = 0;
             uint32_t set = 0;
+            bool ok = true;
             for (int u = cluster_id; ok && u < units; u += num_clusters, ++it) {
                 const Work w = work_unit(p.work, u, part);
                 // the unit before has left the columns the two accumulators share (and, before that, this one's)
@@ -614,6 +618,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
                     }
                 }
             }
+            if (!ok) *gave_up = 1;
         };
         if (half == 0) {
             if (p.b_k)
@@ -624,6 +629,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     } else if (warp == 6) {
         Ring sf(kF8SfSlots);
         const int num_kb = (p.K + 127) / 128;
+        bool ok = true;
         for (int u = cluster_id; ok && u < units; u += num_clusters) {
             const Work w = work_unit(p.work, u, part);
             const int m0 = w.tm * 256 + half * 128 + lane, n0 = w.n0 + lane;
@@ -645,6 +651,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         // as above
         for (int i = 0; ok && i < kF8SfSlots; ++i, sf.next())
             ok = mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitTail, 200 + sf.at);
+        if (!ok) *gave_up = 1;
     }
 
     const bool epilogue = warp >= 2 && warp < 6;
@@ -658,8 +665,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         for (int u = cluster_id; u < units; u += num_clusters, ++it) {
             const Work w = work_unit(p.work, u, part);
             const int acc = it & 1;
-            ok = mbar_wait_warp(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, sum_timeout_ns(p.timeout_ns, w.st1 - w.st0), kErrWaitEpilogue, acc);
-            if (!ok) break;
+            if (!mbar_wait_warp(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, sum_timeout_ns(p.timeout_ns, w.st1 - w.st0), kErrWaitEpilogue, acc)) {
+                *gave_up = 1;
+                break;
+            }
             tc_fence_after();
             // the shared columns first: the last 32 of accumulator 0, the first 32 of accumulator 1
             finish_unit<OUT>(w, out, stg, p.work.pairs > 1 ? sums : nullptr, tmem + (acc ? kF8Acc1 : 0), acc ? 0 : 7, half, q, lane, turn, [&] {
@@ -678,7 +687,8 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     if (epilogue && p.c_tma && lane == 0) bulk_wait_group_all();
 
     tc_fence_before();
-    if (__syncthreads_or(!ok)) settle();
+    __syncthreads();
+    if (warp == 1 && *gave_up != 0) settle();
     cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();

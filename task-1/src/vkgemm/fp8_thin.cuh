@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
     uint8_t* sSf = stages + kStages * Cfg::kStageBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sSf + kThinSfSlots * kThinSfBytes);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
+    volatile uint32_t* gave_up = tmem_slot + 1;  // a wait of this CTA has
     const uint32_t bar0 = smem_u32(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * s; };
     auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
@@ -92,6 +93,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         }
         mbar_init(done_bar, 1);
         fence_mbar_init();
+        *gave_up = 0;
     }
     if (warp == 1) {
         tmem_alloc<1>(smem_u32(tmem_slot), Cfg::kTmemCols);
@@ -101,14 +103,16 @@ __global__ void __launch_bounds__(kThinThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    bool ok = true;  // no wait of this thread has given up
+    bool ok = true;
 
     if (warp == 0) {
         if (lane == 0) {
             Ring r(kStages);
             for (int kb = kb0; kb < kb1; ++kb, r.next()) {
-                ok = mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitProducer, r.at);
-                if (!ok) break;
+                if (!mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitProducer, r.at)) {
+                    *gave_up = 1;
+                    break;
+                }
                 mbar_arrive_expect_tx(full_bar(r.at), Cfg::kStageBytes);
                 const uint32_t dst = smem_u32(stages + r.at * Cfg::kStageBytes);
                 tma_load_2d(dst, &tmap_b, full_bar(r.at), kb * 128, n0);
@@ -125,9 +129,11 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         uint32_t set = 0;
         for (int kb = kb0; kb < kb1; ++kb, r.next()) {
             const int in = (kb - kb0) & 3;  // of a set of scales
-            if (in == 0) ok = mbar_wait_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at);
-            ok = ok && mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at);
-            if (!ok) break;
+            if ((in == 0 && !mbar_wait_warp(sf_full_bar(sf.at), sf.phase, p.timeout_ns, kErrWaitMma, 200 + sf.at)) ||
+                !mbar_wait_warp(full_bar(r.at), r.phase, p.timeout_ns, kErrWaitMma, r.at)) {
+                *gave_up = 1;
+                break;
+            }
             tc_fence_after();
             const uint32_t sfa = base + Cfg::kSfCol + set * 16, sfb = sfa + 8;
             const bool last = in == 3 || kb + 1 == kb1;
@@ -168,8 +174,10 @@ __global__ void __launch_bounds__(kThinThreads, 1)
             of_a.load(p.sa, lane, 32, kb);
             of_b.use(b, num_kb - kb);
             of_a.use(a, num_kb - kb);
-            ok = mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at);
-            if (!ok) break;
+            if (!mbar_wait_warp(sf_empty_bar(sf.at), sf.phase ^ 1u, p.timeout_ns, kErrWaitProducer, 200 + sf.at)) {
+                *gave_up = 1;
+                break;
+            }
             uint4* dst = reinterpret_cast<uint4*>(sSf + sf.at * kThinSfBytes) + lane;
             dst[0] = make_uint4(b[0], b[1], b[2], b[3]);
             dst[32] = make_uint4(a[0], a[kWords > 1 ? 1 : 0], a[kWords > 2 ? 2 : 0], a[kWords > 2 ? 3 : 0]);  // (of rows that the MMA does not have: any)
@@ -179,6 +187,7 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         }
     } else {
         ok = mbar_wait_warp(done_bar, 0, sum_timeout_ns(p.timeout_ns, kb1 - kb0), kErrWaitEpilogue, 0);
+        if (!ok) *gave_up = 1;
         tc_fence_after();
     }
 
@@ -235,7 +244,8 @@ __global__ void __launch_bounds__(kThinThreads, 1)
         }
         cluster_sync_all();
     }
-    if (__syncthreads_or(!ok)) settle();
+    __syncthreads();
+    if (warp == 1 && *gave_up != 0) settle();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc<1>(tmem, Cfg::kTmemCols);

@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     uint8_t* epi = sB + kWgStages * kWgBBytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(epi + 4 * kF8EpiWarpBytes);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kWgBars);
+    volatile uint32_t* gave_up = tmem_slot + 1;  // a wait of this CTA has
 
     const uint32_t bar0 = smem_u32(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -115,6 +116,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             mbar_init(tempty_bar(a), 8);  // the epilogue warps of both CTAs
         }
         fence_mbar_init();
+        *gave_up = 0;
     }
     if (warp == 1) {
         tmem_alloc<2>(smem_u32(tmem_slot), 512);
@@ -125,11 +127,11 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    bool ok = true;  // no wait of this thread has given up
 
     if (warp == 0) {
         if (lane == 0) {
             Ring r(kWgStages);
+            bool ok = true;
             for (int u = cluster_id; ok && u < units; u += num_clusters) {
                 const Work w = work_unit(p.work, u, part);
                 const int m0 = w.tm * 256 + half * 128;
@@ -148,6 +150,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             // the MMAs' signals to this CTA's barriers have all arrived before the CTA may exit
             for (int i = 0; ok && i < kWgStages; ++i, r.next())
                 ok = mbar_wait(empty_bar(r.at), r.phase ^ 1u, p.timeout_ns, kErrWaitTail, r.at);
+            if (!ok) *gave_up = 1;
         }
     } else if (warp == 1) {
         if (half == 0) {  // the whole warp, one lane issuing: see gemm_fp8_kernel
@@ -161,6 +164,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
             const uint64_t b_desc = smem_desc_sw128(smem_u32(sB), kWgBK * 128, 1024);
             Ring r(kWgStages);
             int it = 0;
+            bool ok = true;
             for (int u = cluster_id; ok && u < units; u += num_clusters, ++it) {
                 const Work w = work_unit(p.work, u, part);
                 const int acc = it & 1;
@@ -191,6 +195,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
                     __syncwarp();
                 }
             }
+            if (!ok) *gave_up = 1;
         }
     } else if (warp >= 6) {
         // A warp has 32 tokens of its stages.  Whole tiles: lanes 8g .. 8g+7 hold the 16-byte chunks c of two rows, 0..3 of
@@ -260,8 +265,10 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         uint8_t* dst = sB + group * kWgBBytes;
         if (u < units) fetch();
         while (u < units) {
-            ok = mbar_wait_warp(empty_bar(group), phase ^ 1u, p.timeout_ns, kErrWaitMma, 400 + group);
-            if (!ok) break;
+            if (!mbar_wait_warp(empty_bar(group), phase ^ 1u, p.timeout_ns, kErrWaitMma, 400 + group)) {
+                *gave_up = 1;
+                break;
+            }
             if (w.cols == 256)
                 convert(std::true_type{}, dst);
             else
@@ -286,8 +293,10 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         for (int u = cluster_id; u < units; u += num_clusters, ++it) {
             const Work w = work_unit(p.work, u, part);
             const int acc = it & 1;
-            ok = mbar_wait_warp(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, sum_timeout_ns(p.timeout_ns, w.st1 - w.st0), kErrWaitEpilogue, acc);
-            if (!ok) break;
+            if (!mbar_wait_warp(tfull_bar(acc), static_cast<uint32_t>(it >> 1) & 1u, sum_timeout_ns(p.timeout_ns, w.st1 - w.st0), kErrWaitEpilogue, acc)) {
+                *gave_up = 1;
+                break;
+            }
             tc_fence_after();
             finish_unit<OUT>(w, out, stg, p.work.pairs > 1 ? sums : nullptr, tmem + static_cast<uint32_t>(acc * 256), 0, half, q, lane, turn, [] {});
             tc_fence_before();
@@ -303,7 +312,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     if (epilogue && p.c_tma && lane == 0) bulk_wait_group_all();
 
     tc_fence_before();
-    if (__syncthreads_or(!ok)) settle();
+    __syncthreads();
+    if (warp == 1 && *gave_up != 0) settle();
     cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();

@@ -206,11 +206,12 @@ def test_waits_that_give_up_leave_in_order():
     for name in ("fp8_gemm.cuh", "fp8_wgrad.cuh", "fp8_thin.cuh"):
         text = open(os.path.join(src, name)).read()
         body = text[text.index("__global__"):]
-        # waits by single threads: only in the loading warp's one lane, and none whose answer is dropped
-        single = re.findall(r"(\S+ = |\bif \(!)?mbar_wait\((\w+)_bar", body)
-        assert single and all(how == "ok = " and bar == "empty" or how == "if (!" and bar == "empty" for how, bar in single), (name, single)
-        assert not re.search(r"if \(!mbar_wait\w*_warp\(", body), name
-        assert "__syncthreads_or(!ok)) settle();" in body, name
+        # waits by single threads: only in the loading warp's one lane
+        single = re.findall(r"mbar_wait\((\w+)_bar", body)
+        assert single and set(single) == {"empty"}, (name, single)
+        # each role that can give up says so, and the CTA's last warp looks behind the last barrier
+        assert body.count("*gave_up = 1;") == 4, name
+        assert re.search(r"__syncthreads\(\);\s+if \(warp == 1 && \*gave_up != 0\) settle\(\);", body), name
         assert body.index("settle()") < body.index("tmem_dealloc"), name
     text = open(os.path.join(src, "fp8_rows.cuh")).read()
     body = text[text.index("rmsnorm_fp8_backward_kernel(const NormBackParams p)"):text.index("norm_weight_grad_kernel(")]
