@@ -1,5 +1,5 @@
 // C ABI of the 8-bit linear layer (include/vkgemm.h, "8-bit operands"): argument checks, kernel choice, launches.
-// No call here allocates, keeps anything between calls but tensor maps and kernel attributes, or synchronises, so all
+// No call here allocates, synchronises or keeps anything between calls but kernel attributes and how many clusters fit, so all
 // of them can be captured into CUDA graphs.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -134,7 +134,7 @@ int make_out_map(CUtensorMap* map, void* c, int64_t m, int64_t n, long long ldc,
 }
 
 // Clusters of 2, 4, 6 and 8 CTAs of each kernel that fit on each device (0: not asked yet; the kernel's shared-memory
-// attribute is set by then).
+// attribute is set by then.  Kernels without clusters: 1 once that is set).
 constexpr int kKernels = 32, kDevices = 64;
 std::atomic<int> g_clusters[kKernels][kDevices][4];
 
@@ -166,6 +166,19 @@ int prepare_kernel(Kernel fn, int id, int smem, int threads, int clusters[4])
         }
     }
     for (int i = 0; i < 4; ++i) clusters[i] = known[i].load(std::memory_order_acquire);
+    return VK_OK;
+}
+
+// For a kernel without clusters: its shared memory.
+template <typename Kernel>
+int prepare_smem(Kernel fn, int id, int smem)
+{
+    int dev = 0;
+    F8_CUDA_TRY(cudaGetDevice(&dev));
+    std::atomic<int>& known = g_clusters[id][dev][0];
+    if (known.load(std::memory_order_acquire) != 0) return VK_OK;
+    F8_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    known.store(1, std::memory_order_release);
     return VK_OK;
 }
 
@@ -402,8 +415,7 @@ static int launch_norm_backward(NormBackParams p, int id, const NormBackPlan& pl
         return launched();
     }
     const int pitch = (p.cols * 2 + 127) / 128 * 128;
-    int clusters[4];
-    const int rc = prepare_kernel(rmsnorm_fp8_backward_kernel<T, NV, VEC>, id, kNormBackBytes / (NV == 1 ? 2 : 1), 512, clusters);
+    const int rc = prepare_smem(rmsnorm_fp8_backward_kernel<T, NV, VEC>, id, kNormBackBytes / (NV == 1 ? 2 : 1));
     if (rc != VK_OK) return rc;
     p.stages = kNormBackBytes / plan.per_sm / (3 * pitch);
     if (p.stages > 8) p.stages = 8;
