@@ -132,6 +132,10 @@ class WgradFp8Args(ctypes.Structure):
     ]
 
 
+_FP8_ARGS = {"quantize_fp8": QuantizeFp8Args, "rmsnorm_fp8": RmsnormFp8Args, "rmsnorm_fp8_backward": RmsnormFp8BackwardArgs,
+             "gemm_fp8": GemmFp8Args, "wgrad_fp8": WgradFp8Args}
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -209,8 +213,7 @@ def _load() -> ctypes.CDLL:
     lib.vk_debug_watchdog.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, i32p,
                                       ctypes.POINTER(ctypes.c_int64)]
     lib.vk_debug_watchdog.restype = ctypes.c_int
-    for name, args in (("quantize_fp8", QuantizeFp8Args), ("rmsnorm_fp8", RmsnormFp8Args), ("gemm_fp8", GemmFp8Args),
-                       ("rmsnorm_fp8_backward", RmsnormFp8BackwardArgs), ("wgrad_fp8", WgradFp8Args)):
+    for name, args in _FP8_ARGS.items():
         fn = getattr(lib, "vk_" + name)
         fn.argtypes = [ctypes.POINTER(args)]
         fn.restype = ctypes.c_int
@@ -598,7 +601,7 @@ class _Fp8:
         self.q, self.scale = torch.float8_e4m3fn, torch.float8_e8m0fnu
         self.current_device = torch.cuda.current_device
         self.raw_stream = torch._C._cuda_getCurrentRawStream
-        # the argument structures of include/vkgemm.h, packed in one call each
+        # the argument structures, packed in one call each
         for name, fmt in _FP8_STRUCTS.items():
             fn = lib["vk_" + name]
             fn.argtypes = [ctypes.c_char_p]
@@ -606,8 +609,8 @@ class _Fp8:
             setattr(self, name, (fn, struct.Struct(fmt).pack))
 
 
-_FP8_STRUCTS = {"quantize_fp8": "3P5q2iP", "rmsnorm_fp8": "7P7qfiP", "rmsnorm_fp8_backward": "8PN6qiP", "gemm_fp8": "5P8q4iP",
-                "wgrad_fp8": "4P7q3iP"}
+_FP8_STRUCTS = {name: "".join({_P: "P", _I64: "q", _I32: "i", ctypes.c_float: "f", ctypes.c_size_t: "N"}[kind] for _, kind in args._fields_)
+                for name, args in _FP8_ARGS.items()}
 _fp8_cache = None
 
 
