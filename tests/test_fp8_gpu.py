@@ -932,3 +932,54 @@ def test_longest_sums(vk):
     _check_product(_ends(dw), want, want.abs(), 1)
     del dw, b, sb, q, s
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------------ the norm's backward pass over many rows
+# A CTA has 2 rows until there are more than 2 * 148 to each that fits an SM (8 at most 1024 wide, 4 at most 2048, 2 at most 4096, else
+# 1); these have 7 to 17, so that every stage of the ring of rows in shared memory is filled again, several times over.
+RINGS = [(20001, 128), (9001, 1000), (9000, 1024), (5001, 2048), (3001, 4096), (1501, 4104), (1501, 8192)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("with_res", [False, True])
+@pytest.mark.parametrize("shape", RINGS)
+def test_norm_backward_of_many_rows(vk, shape, with_res, dtype):
+    test_norm_backward(vk, shape, with_res, dtype)
+
+
+@pytest.mark.parametrize("shape", [(9001, 1000), (3001, 4096), (1501, 8192)])
+def test_norm_backward_of_many_rows_in_place(vk, shape):
+    """dx in dy's or dres's place on the aligned path: the same bits, and the same every time."""
+    mats = [_rand(shape, BF16, 190 + i) for i in range(3)]
+    w = _rand((shape[1],), BF16, 193)
+    rstd = torch.rand(shape[0], generator=_gen(194), device="cuda") + 0.5
+    dx, dw = vk.rmsnorm_fp8_backward(mats[0], mats[1], w, rstd, dres=mats[2])
+    _check_norm_back(mats[0], mats[1], w, rstd, mats[2], dx, dw)
+    for which in (0, 2, 0, 2):
+        copies = [m.clone() for m in mats]
+        got, dw2 = vk.rmsnorm_fp8_backward(copies[0], copies[1], w, rstd, dres=copies[2], dx=copies[which])
+        assert got is copies[which] and torch.equal(got, dx) and torch.equal(dw2, dw)
+
+
+@pytest.mark.parametrize("shape", [(1, 8), (149, 1000), (3001, 4096), (1501, 8192), (300, 8200), (301, 333)])
+def test_norm_backward_stays_in_its_workspace(vk, shape):
+    """The C call with a workspace of exactly the size asked for, and what lies around it and around the outputs."""
+    import ctypes
+    rows, cols = shape
+    need = ctypes.c_size_t(0)
+    assert vk.lib.vk_rmsnorm_fp8_workspace(rows, cols, ctypes.byref(need)) == vk.VK_OK
+    room = torch.full((need.value + 8192,), 0x55, dtype=torch.uint8, device="cuda")
+    at = 4096 - room.data_ptr() % 16
+    dy, h, w = _rand(shape, F16, 196), _rand(shape, F16, 197), _rand((cols,), F16, 198)
+    rstd = torch.rand(rows, generator=_gen(199), device="cuda") + 0.5
+    dx, dxroom = _inside(shape, F16, 8, 8)
+    dw = torch.full((cols + 16,), 5.0, device="cuda")
+    args = vk.RmsnormFp8BackwardArgs(dY=dy.data_ptr(), H=h.data_ptr(), weight=w.data_ptr(), rstd=rstd.data_ptr(), dX=dx.data_ptr(),
+                                     dweight=dw[8:].data_ptr(), workspace=room.data_ptr() + at, workspace_bytes=need.value,
+                                     rows=rows, cols=cols, lddx=dx.stride(0), dtype=vk.DTYPE_F16,
+                                     stream=torch.cuda.current_stream().cuda_stream)
+    assert vk.lib.vk_rmsnorm_fp8_backward(ctypes.byref(args)) == vk.VK_OK
+    _check_norm_back(dy, h, w, rstd, None, dx, dw[8:-8])
+    assert (room[:at] == 0x55).all() and (room[at + need.value:] == 0x55).all()
+    assert (dw[:8] == 5).all() and (dw[-8:] == 5).all()
+    _untouched(dxroom, shape, 8)
