@@ -279,8 +279,10 @@ int vk_gemm_fp8(const vk_gemm_fp8_args* args);
 
 /* dW[n x k] = dY^T * X (accumulate = 1: dW += it): a layer's weight gradient from its output's gradient dY[tokens x n]
  * in 16 bits and its input X[tokens x k] as the forward pass kept it, in 8 bits with VK_FP8_ROW scales.  X's values are
- * used in dY's type: bf16 holds each of them exactly; fp16 rounds what lies below its smallest normal number and
- * holds what lies above its largest at that.  fp32 accumulation; dW in fp16, bf16 or fp32. */
+ * used in dY's type.  bf16 holds each of them exactly for scales of 2^-124 and more, up to 2^128, where they become
+ * infinite (vk_quantize_fp8 writes such a value only for a block whose largest is 248 * 2^120 or more); under smaller
+ * scales what lies below bf16's smallest step, 2^-133, is rounded to it.  fp16 rounds what lies below its smallest
+ * normal number and holds what lies above its largest at that.  fp32 accumulation; dW in fp16, bf16 or fp32. */
 typedef struct vk_wgrad_fp8_args {
     const void* dY;
     const void* X;

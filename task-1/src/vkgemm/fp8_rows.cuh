@@ -4,8 +4,8 @@
 // The 8-bit form.  A block is 128 neighbouring values of a row, or a tile of 128 x 128.  Its scale is the
 // smallest 2^e with max|v| <= 448 * 2^e (448 is e4m3's largest value), held as the e8m0 byte e + 127; the
 // values are v * 2^-e, rounded once to nearest even.  v * 2^-e is exact in fp32 (or far below e4m3's smallest
-// step), so that rounding is the only one, and q * 2^e is exact in bf16 again: what reads the 8-bit form later
-// loses nothing more.  A block of zeros has scale 1; one that holds an infinity or a NaN has the NaN scale
+// step), so that rounding is the only one, and q * 2^e is exact in bf16 again from e = -124 on and below 2^128 (a block's
+// largest value of 248 * 2^120 or more is rounded to that): what reads the 8-bit form later loses nothing more.  A block of zeros has scale 1; one that holds an infinity or a NaN has the NaN scale
 // (255) and NaN values, so that it shows.
 #pragma once
 

@@ -33,7 +33,8 @@ struct F8Operand {
     }
 };
 
-// The same with each value rounded to the type of the operand it meets: exact in bf16, within fp16's finite range.
+// The same with each value rounded to the type of the operand it meets: exact in bf16 (see fp8_rows.cuh), within
+// fp16's finite range.
 template <typename T>
 struct F8OperandAs {
     F8Operand f;

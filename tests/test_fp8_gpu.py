@@ -983,3 +983,39 @@ def test_norm_backward_stays_in_its_workspace(vk, shape):
     assert (room[:at] == 0x55).all() and (room[at + need.value:] == 0x55).all()
     assert (dw[:8] == 5).all() and (dw[-8:] == 5).all()
     _untouched(dxroom, shape, 8)
+
+
+# ------------------------------------------------------------------------------------------ both ends of the scales
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("byte", [0, 1, 2, 3, 246, 247, 254, 255])
+@pytest.mark.parametrize("tokens,n", [(1, 8), (2, 7)])
+def test_wgrad_of_the_first_and_last_scales(vk, dtype, byte, tokens, n):
+    """Every e4m3 value under the smallest and largest scales, on both kernels: rounded once to dY's type below its smallest step
+    (bf16: 2^-133, met by bytes below 3), infinite in bf16 from 2^128 on (byte 247 and up), fp16's largest number in fp16."""
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    x = torch.zeros((tokens, 256), dtype=torch.uint8, device="cuda")
+    x[0, :254] = codes[(codes & 127) != 127]
+    s = torch.full((tokens, 2), byte, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+    x = x.view(torch.float8_e4m3fn)
+    dy = torch.zeros((tokens, n), dtype=dtype, device="cuda")
+    dy[0] = 1
+    dw = vk.wgrad_fp8(dy, x, s, out_dtype=F32)
+    want = _deq(x, s)[0].float()  # exact, or infinite
+    want = (want.clamp(-65504, 65504) if dtype is F16 else want).to(dtype).float()
+    assert want.isnan().all() if byte == 255 else not want.isnan().any()
+    assert torch.equal(dw.nan_to_num(nan=1.5, posinf=float("inf"), neginf=-float("inf")),
+                       want.nan_to_num(nan=1.5, posinf=float("inf"), neginf=-float("inf")).expand(n, 256))
+    if dtype is BF16:
+        assert bool(want.isinf().any()) == (247 <= byte < 255)
+
+
+def test_wgrad_of_a_block_at_the_top_of_bf16(vk):
+    """The largest value that stays finite through the 8-bit form, and the smallest that does not."""
+    x = torch.zeros((8, 256), dtype=BF16, device="cuda")
+    x[0, 0], x[0, 128] = 247 * 2.0 ** 120, 248 * 2.0 ** 120
+    q, s = vk.quantize_fp8(x)
+    assert _bytes(s)[0].tolist() == [247, 247]
+    dw = vk.wgrad_fp8(torch.ones((8, 8), dtype=BF16, device="cuda"), q, s, out_dtype=F32)
+    assert (dw[:, 0] == 240 * 2.0 ** 120).all() and dw[:, 128].isposinf().all()
+    dw[:, [0, 128]] = 0
+    assert torch.count_nonzero(dw) == 0
