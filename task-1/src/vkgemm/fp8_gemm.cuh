@@ -16,9 +16,10 @@
 // accumulator begins at column 224: the two share 32 columns, which the epilogue reads first; the next tile's MMAs start
 // once it has.  Columns 480..511 hold two sets of scales (4 columns for A's 128 rows, 8 for B's 256), each for 512 of k.
 //
-// Bound by the MMAs: a stage of a whole tile takes 990 of the 1024 clocks that eight 256 x 256 x 32 instructions are rated at
-// (8192 x 8192 x 8192 bf16 out 376 us, 2.9 PFLOP/s, until the power limit lowers the clock; 4096 x 4096 x 4096 51.5 us, B
-// stored k x n 53.7).  Half tiles read as much of A for half the work, 0.48 us a stage instead of 0.3.
+// Bound by the MMAs: at 8192 x 8192 x 8192, bf16 out, the tensor pipe is active for 93 % of the time (519 thousand cycles for 14
+// rounds of 32 stages, 1160 a stage with all that is around them; its eight 256 x 256 x 32 instructions are rated at 1024).  373 to
+// 388 us, 2.8 to 2.9 PFLOP/s, until the power limit lowers the clock (455 us at 1.07 GHz); 4096 x 4096 x 4096 52.4 to 53.3 us, B stored
+// k x n 55.0.  512 x 4096 x 4096, 64 half tiles of 16 stages, 13.3 to 14.2 us: the pipe is active for a third of the time.  Half tiles read as much of A for half the work, 0.48 us a stage instead of 0.3.
 //
 // How tiles are handed out (TileWork): pairs walk over whole tiles; when the last wave would leave half of them or more
 // without one, its tiles are cut into column halves.  (Cutting them along k, with the partial sums joined through
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     } else if (warp == 1) {
         // The whole warp walks through the loop and one lane issues: what the instructions take is then the same in every
         // lane and stays in uniform registers.  With one lane in the loop, issuing the eight MMAs of a stage took longer
-        // than running them (1422 clocks a stage instead of 1024).
+        // than running them (the step that changed it, among others, took 8192 x 8192 x 8192 from 512 to 474 us in a loop).
         auto mma_loop = [&](auto b_k_tag) {
             constexpr bool B_K = decltype(b_k_tag)::value;
             constexpr uint32_t kIdesc = idesc_mxf8(256, 256, !B_K), kIdescHalf = idesc_mxf8(256, 128, !B_K);

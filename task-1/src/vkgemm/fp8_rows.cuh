@@ -246,7 +246,7 @@ struct QuantParams {
 
 // Rows: 16 lanes hold one block, 8 values each, and have four neighbouring blocks of a row, so that four loads are in
 // flight and the four scales leave in one store.  16 such quads to a CTA.  Bound by memory: 8192 x 8192 bf16 31.5 us, 6.4 TB/s
-// (blocks one by one, a grid apart: 45 us).
+// (blocks one by one, a grid apart: 45 us); 8192 x 4096 fp32 26.6 us, 6.3 TB/s.  Rows at any alignment: 4001 x 3333 15.3 us, 2.6 TB/s.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
 {
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantParams p)
 }
 
 // One 128 x 128 tile per CTA, held in registers between its maximum and its rounding: 16 lanes per row, 16 rows at a time.
-// Bound by memory: 16384 x 4096 bf16 31 us, 6.5 TB/s.
+// Bound by memory: 16384 x 4096 bf16 31 us, 6.5 TB/s; 8192 x 4096 fp32 30.2 us, 5.6 TB/s.  Rows at any alignment: 4001 x 3333 16.0 us.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_tiles_kernel(const QuantParams p)
 {
@@ -385,7 +385,9 @@ __device__ __forceinline__ void norm_row_out(const NormParams& p, long long row,
 // stores their scales at once (a byte at a time costs memory more than the row's values do).  VEC: rows and weight are
 // aligned for 16-byte accesses (q: 8) and cols is a multiple of 8.  Bound by memory: 4001 x 5120 fp16 with a residual
 // 20.9 us, 6.9 TB/s (part of it from L2); 8192 x 8192 bf16 70.3 us, 6.7 TB/s; without a residual by the instructions of
-// the second pass: 8192 x 4096 22.9 us, 4.4 TB/s.  (CTAs that walk over rows, which arrive ahead in shared memory by
+// the second pass, which fewer bytes hide (issue slots 69 % busy with 89 % of the warps there, 18.4 instructions for an
+// element): 8192 x 4096 22.5 us, 4.5 TB/s; 4096 x 12288 39.6 us, 3.8 TB/s.  Rows at any alignment hold 57 registers for 32, so that 41 %
+// of the warps are there and wait for memory: 4001 x 3333 35.8 us, 2.6 TB/s.  (CTAs that walk over rows, which arrive ahead in shared memory by
 // bulk copies: 24.3, 85.6 and 26.0 us.)
 template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(NV == 1 ? 256 : 512) rmsnorm_fp8_kernel(const NormParams p)
@@ -488,7 +490,8 @@ struct NormBackParams {
 
 // dx = rstd * (g - xhat * mean(g * xhat)) + dres with g = dy * weight, xhat = h * rstd; dweight = sum over rows of
 // dy * xhat.  CTAs walk over the rows.  Here, any number of columns: a thread adds its columns' share
-// of dweight in its CTA's row of `part` (each element belongs to one thread), and reads a row twice.
+// of dweight in its CTA's row of `part` (each element belongs to one thread), and reads a row twice, one 16-bit element at a time.
+// Far from memory's rate: 4096 x 12288 bf16 with dres 799 us, 0.5 TB/s; 2000 x 16384 531.  It runs for rows over 8192 wide only.
 template <typename T>
 __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const NormBackParams p)
 {
@@ -520,7 +523,9 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_backward_any_kernel(const Nor
 
 // The same for rows of at most 512 * 8 * NV columns; dweight's share stays in registers.  VEC (16-byte aligned rows, a
 // multiple of 8 columns): rows arrive ahead in shared memory, one bulk copy per tensor and row, p.stages rows deep, so
-// that memory stays busy through the two passes and the barrier of each row: 8192 x 8192 bf16 with dres 86.5 us, 6.2 TB/s.
+// that memory stays busy through the two passes and the barrier of each row: 8192 x 8192 bf16 with dres 85.8 us, 6.3 TB/s.
+// Narrower rows wait more at their barrier for each byte: 4096 x 4096 27.7 us, 4.9 TB/s; 8000 x 1000 18.7 us, 3.4 TB/s, 15 of them
+// here (issue slots 41 % busy, a warp's waits about even between the barrier and memory) and the rest in the sum of 1184 partial rows.
 // Otherwise from memory as they are needed (4001 x 3333: 61 us).
 template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) rmsnorm_fp8_backward_kernel(const NormBackParams p)
