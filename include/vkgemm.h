@@ -217,7 +217,8 @@ int vk_quantize_fp8(const vk_quantize_fp8_args* args);
 /* RMS norm of each row with an 8-bit output (fp16 or bf16; statistics and products in fp32):
  *   H = X + residual (rounded to the type; without a residual H is X and must be NULL here)
  *   rstd = 1 / sqrt(mean(H^2) + eps);   Q, scale = 8-bit form (VK_FP8_ROW) of H * rstd * weight
- * H may be X or residual itself (same leading dimension).  cols >= 1. */
+ * H may be X or residual itself (same leading dimension).  cols >= 1.  A row whose squares or their sum leave fp32's range
+ * has rstd 0 and values of 0 (bf16 above 1.8e19). */
 typedef struct vk_rmsnorm_fp8_args {
     const void* X;
     const void* residual; /* may be NULL */

@@ -64,6 +64,13 @@ int element_aligned(const char* name, const char* what, const void* p, size_t es
     return set_error(VK_ERR_ALIGNMENT, "%s: %s is not aligned to its elements of %zu bytes", name, what, esize);
 }
 
+// An output in an input's place whose rows would lie elsewhere.
+int in_place(const char* name, const char* what, const void* out, long long ldo, const void* in, long long ldi, int64_t rows)
+{
+    if (out == nullptr || out != in || ldo == ldi || rows <= 1) return VK_OK;
+    return set_error(VK_ERR_INVALID_ARGUMENT, "%s: %s in place needs the same leading dimension (%lld, not %lld)", name, what, ldi, ldo);
+}
+
 bool rows_at(const void* p, long long ld, size_t esize, size_t to)
 {
     return aligned(p, to) && (static_cast<unsigned long long>(ld) * esize) % to == 0;
@@ -353,6 +360,8 @@ extern "C" int vk_rmsnorm_fp8(const vk_rmsnorm_fp8_args* a)
     if (rc == VK_OK) rc = element_aligned(name, "weight", a->weight, 2);
     if (rc == VK_OK) rc = element_aligned(name, "H", a->H, 2);
     if (rc == VK_OK) rc = element_aligned(name, "rstd", a->rstd, 4);
+    if (rc == VK_OK) rc = in_place(name, "H", a->H, p.ldh, a->X, p.ldx, a->rows);
+    if (rc == VK_OK) rc = in_place(name, "H", a->H, p.ldh, a->residual, p.ldr, a->rows);
     if (rc == VK_OK) rc = use_device();
     if (rc != VK_OK) return rc;
     p.x = a->X;
@@ -451,6 +460,8 @@ extern "C" int vk_rmsnorm_fp8_backward(const vk_rmsnorm_fp8_backward_args* a)
     if (rc == VK_OK) rc = element_aligned(name, "rstd", a->rstd, 4);
     if (rc == VK_OK) rc = element_aligned(name, "dres", a->dres, 2);
     if (rc == VK_OK) rc = element_aligned(name, "dX", a->dX, 2);
+    if (rc == VK_OK) rc = in_place(name, "dX", a->dX, p.lddx, a->dY, p.lddy, a->rows);
+    if (rc == VK_OK) rc = in_place(name, "dX", a->dX, p.lddx, a->dres, p.lddres, a->rows);
     if (rc == VK_OK) rc = use_device();
     if (rc != VK_OK) return rc;
     const cudaStream_t stream = static_cast<cudaStream_t>(a->stream);

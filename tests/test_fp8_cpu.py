@@ -216,3 +216,19 @@ def test_waits_that_give_up_leave_in_order():
     text = open(os.path.join(src, "fp8_rows.cuh")).read()
     body = text[text.index("rmsnorm_fp8_backward_kernel(const NormBackParams p)"):text.index("norm_weight_grad_kernel(")]
     assert "break" not in body and "return" not in body and "if (VEC && threadIdx.x == 0 && !ok) settle();" in body
+
+
+@pytest.mark.parametrize("name,fields", [
+    ("rmsnorm_fp8", dict(residual=2 * P, H=P, ldx=16, ldh=24)), ("rmsnorm_fp8", dict(residual=2 * P, H=2 * P, ld_residual=16, ldh=8)),
+    ("rmsnorm_fp8_backward", dict(dX=P, dY=P, lddy=16)), ("rmsnorm_fp8_backward", dict(dX=2 * P, dres=2 * P, dY=P, lddx=16, ld_dres=8)),
+])
+def test_in_place_with_another_pitch_is_refused(name, fields):
+    """Rows would be overwritten before they are read."""
+    assert _call(name, **{**_good(name), **fields}) == BAD
+    assert "in place" in vk.last_error()
+    # one row has no pitch, and the same pitch is what the header allows: neither is refused for it
+    for ok in (dict(rows=1), {k: 16 for k in fields if k.startswith("ld")} | {"ldh": 16, "lddx": 16, "lddy": 16, "ldx": 16, "ld_residual": 16, "ld_dres": 16}):
+        args = {**_good(name), **fields, **ok}
+        names = [f for f, _ in {"rmsnorm_fp8": vk.RmsnormFp8Args, "rmsnorm_fp8_backward": vk.RmsnormFp8BackwardArgs}[name]._fields_]
+        if not torch.cuda.is_available():
+            assert _call(name, **{k: v for k, v in args.items() if k in names}) in (vk.VK_ERR_CUDA, vk.VK_ERR_NO_DEVICE)
