@@ -366,7 +366,8 @@ int vk_device_error(int device, uint64_t* out_word, int clear);
  * clears the device error word again), VK_OK never. */
 int vk_selftest_wait_timeout(int device, int64_t timeout_us);
 
-/* Per-call device-side wait limit for the GEMM kernels, nanoseconds (default 2e9). */
+/* Per-call device-side wait limit for the GEMM kernels, nanoseconds (default 2e9).  Where the 8-bit products wait for a
+ * whole sum, it grows by 10 us for each of the sum's stages (128 or 256 terms). */
 int vk_set_wait_timeout_ns(uint64_t ns);
 
 /* Process-wide tuning knobs (no counterpart in the reference, whose versions hard-code them):

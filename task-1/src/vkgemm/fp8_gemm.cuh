@@ -19,7 +19,8 @@
 // Bound by the MMAs: at 8192 x 8192 x 8192, bf16 out, the tensor pipe is active for 93 % of the time (519 thousand cycles for 14
 // waves of 32 stages, 1160 a stage with all that is around them; its eight 256 x 256 x 32 instructions are rated at 1024).  373 to
 // 388 us, 2.8 to 2.9 PFLOP/s, until the power limit lowers the clock (455 us at 1.07 GHz); 4096 x 4096 x 4096 52.4 to 53.3 us, B stored
-// k x n 55.0.  512 x 4096 x 4096, 64 half tiles of 16 stages, 13.3 to 14.2 us: the pipe is active for a third of the time.  Half tiles read as much of A for half the work, 0.48 us a stage instead of 0.3.
+// k x n 55.0.  512 x 4096 x 4096, 64 half tiles of 16 stages, 13.3 to 14.2 us: the pipe is active for a third of the time.  Half
+// tiles read as much of A for half the work, 0.48 us a stage instead of 0.3.
 //
 // How tiles are handed out (TileWork): pairs walk over whole tiles; when the last wave would leave half of them or more
 // without one, its tiles are cut into column halves.  (Cutting them along k, with the partial sums joined through

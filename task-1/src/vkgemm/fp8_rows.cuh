@@ -5,8 +5,8 @@
 // smallest 2^e with max|v| <= 448 * 2^e (448 is e4m3's largest value), held as the e8m0 byte e + 127; the
 // values are v * 2^-e, rounded once to nearest even.  v * 2^-e is exact in fp32 (or far below e4m3's smallest
 // step), so that rounding is the only one, and q * 2^e is exact in bf16 again from e = -124 on and below 2^128 (a block's
-// largest value of 248 * 2^120 or more is rounded to that): what reads the 8-bit form later loses nothing more.  A block of zeros has scale 1; one that holds an infinity or a NaN has the NaN scale
-// (255) and NaN values, so that it shows.
+// largest value of 248 * 2^120 or more is rounded to that): what reads the 8-bit form later loses nothing more.  A block of
+// zeros has scale 1; one that holds an infinity or a NaN has the NaN scale (255) and NaN values, so that it shows.
 #pragma once
 
 #include <cstdint>
@@ -386,9 +386,9 @@ __device__ __forceinline__ void norm_row_out(const NormParams& p, long long row,
 // aligned for 16-byte accesses (q: 8) and cols is a multiple of 8.  Bound by memory: 4001 x 5120 fp16 with a residual
 // 20.9 us, 6.9 TB/s (part of it from L2); 8192 x 8192 bf16 70.3 us, 6.7 TB/s; without a residual by the instructions of
 // the second pass, which fewer bytes hide (issue slots 69 % busy with 89 % of the warps there, 18.4 instructions for an
-// element): 8192 x 4096 22.5 us, 4.5 TB/s; 4096 x 12288 39.6 us, 3.8 TB/s.  Rows at any alignment hold 57 registers for 32, so that 41 %
-// of the warps are there and wait for memory: 4001 x 3333 35.8 us, 2.6 TB/s.  (CTAs that walk over rows, which arrive ahead in shared memory by
-// bulk copies: 24.3, 85.6 and 26.0 us.)
+// element): 8192 x 4096 22.5 us, 4.5 TB/s; 4096 x 12288 39.6 us, 3.8 TB/s.  Rows at any alignment hold 57 registers for 32, so
+// that 41 % of the warps are there and wait for memory: 4001 x 3333 35.8 us, 2.6 TB/s.  (CTAs that walk over rows, which arrive
+// ahead in shared memory by bulk copies: 24.3, 85.6 and 26.0 us.)
 template <typename T, int NV, bool VEC>
 __global__ void __launch_bounds__(NV == 1 ? 256 : 512) rmsnorm_fp8_kernel(const NormParams p)
 {

@@ -3,8 +3,8 @@
 //
 // X's scale changes along the sum (the tokens), so neither the tensor core's block scales nor the epilogue can apply
 // it, and one MMA takes both operands in the same type.  Four warps therefore turn each stage of X into dY's type on
-// its way to the MMAs: q * 2^e is exact in bf16 (see fp8_rows.cuh), and the product is that of the 16-bit kernel.  X costs half the bytes of a
-// 16-bit checkpoint in memory and on the way into the SM.  Bound by the conversion: at 8192 x 4096 x 4096 the
+// its way to the MMAs: q * 2^e is exact in bf16 (see fp8_rows.cuh), and the product is that of the 16-bit kernel.  X costs half
+// the bytes of a 16-bit checkpoint in memory and on the way into the SM.  Bound by the conversion: at 8192 x 4096 x 4096 the
 // tensor pipe is active for 70 % of the time, in fp16, which takes two multiplies, a conversion, a minimum and a maximum for a pair
 // of values where bf16 takes a conversion and a multiply, for 61 %.  bf16 214 to 219 us, 1.27 PFLOP/s; fp16 236; bf16 into fp32 222,
 // added to an fp32 dW 234 (4000 x 1000 x 3333, whose rows take no TMA stores: 44 and 82, C being read a row to a lane).

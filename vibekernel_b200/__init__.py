@@ -880,9 +880,9 @@ def wgrad_fp8(dY, X, x_scale, dW=None, *, accumulate: bool = False, out_dtype=No
 
     dY is [tokens, n], float16 or bfloat16; X is [tokens, k] in 8 bits with scales by rows, as the forward pass kept it
     (:func:`quantize_fp8`, or the output of :func:`rmsnorm_fp8`).  dW is [n, k] in ``out_dtype`` (default dY's type;
-    float32 too), fp32 accumulation.  X's values enter the product in dY's type: exact in
-    bfloat16 for scales from 2^-124 on and values below 2^128 (infinite from there on); float16 rounds below its smallest normal
-    number and holds larger values at its largest.
+    float32 too), fp32 accumulation.  X's values enter the product in dY's type: exact in bfloat16 for scales
+    from 2^-124 on and values below 2^128 (infinite from there on); float16 rounds below its smallest normal number and
+    holds larger values at its largest.
     """
     F = _fp8()
     guard = _elsewhere(F, dY, stream)
